@@ -23,6 +23,17 @@ from ._plan import (
     set_plan_cache_capacity,
     set_window_policy,
 )
+from .selection import (
+    TokenRoute,
+    check_selection_ids,
+    flagsparse_embedding,
+    flagsparse_embedding_grad,
+    flagsparse_token_combine,
+    flagsparse_token_combine_grad,
+    flagsparse_token_dispatch,
+    flagsparse_token_dispatch_grad,
+    prepare_token_route,
+)
 from .spmm import (
     SPMM_OP_CONJ_TRANS,
     SPMM_OP_NON,
@@ -71,6 +82,15 @@ __all__ = [
     "prepare_spmv_coo_tocsr",
     "coo_to_csr_for_spmv",
     "csr_to_csc",
+    "flagsparse_embedding",
+    "flagsparse_embedding_grad",
+    "prepare_token_route",
+    "TokenRoute",
+    "flagsparse_token_dispatch",
+    "flagsparse_token_dispatch_grad",
+    "flagsparse_token_combine",
+    "flagsparse_token_combine_grad",
+    "check_selection_ids",
     "install",
     "clear_plan_cache",
     "set_plan_cache_capacity",

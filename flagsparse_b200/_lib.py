@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import c_char_p, c_int, c_int64, c_void_p
+from ctypes import c_char_p, c_double, c_int, c_int64, c_void_p
 from pathlib import Path
 
 import torch
@@ -109,6 +109,24 @@ SIGNATURES = {
     "b2s_csr2csc": (c_int, [c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_int64, c_int64,
                             c_int64, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int64,
                             c_void_p]),
+    "b2s_select_rows": (c_int, [c_int, c_int, c_void_p, c_int64, c_int, c_int64, c_void_p, c_int64,
+                                c_int64, c_int64, c_void_p, c_int64, c_double, c_double, c_void_p,
+                                c_void_p]),
+    "b2s_select_grad_bytes": (c_int64, [c_int, c_int64, c_int64, c_int64]),
+    "b2s_select_grad": (c_int, [c_int, c_int, c_int, c_void_p, c_int64, c_int, c_int64, c_void_p,
+                                c_int64, c_int64, c_int64, c_void_p, c_int64, c_double, c_double,
+                                c_void_p, c_int64, c_void_p, c_void_p]),
+    "b2s_route_plan_bytes": (c_int64, [c_int64, c_int64, c_int64]),
+    "b2s_route_plan": (c_int, [c_int, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p,
+                               c_void_p, c_void_p, c_int64, c_void_p, c_void_p]),
+    "b2s_route_dispatch": (c_int, [c_int, c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p,
+                                   c_void_p, c_void_p, c_int64, c_void_p]),
+    "b2s_route_combine": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int64,
+                                  c_int64, c_int64, c_void_p, c_int64, c_double, c_double,
+                                  c_void_p]),
+    "b2s_route_combine_grad": (c_int, [c_int, c_void_p, c_int64, c_void_p, c_int64, c_void_p,
+                                       c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64,
+                                       c_double, c_void_p, c_int64, c_void_p, c_void_p]),
 }
 
 _lib = None

@@ -1,0 +1,376 @@
+// Stable counting sort of ids: tokens by vocabulary row (embedding gradient), assignments by
+// expert (token route).  Least significant digit first; one digit of up to 11 bits per pass, so
+// that a route needs one pass and a vocabulary of 2^17 rows two.
+//
+// A pass cuts the list into at most 128 chunks, one CTA each.  The first kernel counts the
+// digits of each chunk; the second sums those counts itself (every CTA reads the whole
+// chunks x digits table, which L2 holds) and places its entries in order.  A list of one chunk
+// needs one launch for all passes: the CTA counts, places and goes on to the next digit.
+#pragma once
+#include <type_traits>
+
+#include "b2s_tile.cuh"
+
+namespace b2s {
+
+constexpr int kSortThreads = 512;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortRounds = 2;                           // entries per thread and tile
+constexpr int kSortTile = kSortThreads * kSortRounds;
+constexpr int kSortMaxChunks = 128;
+constexpr int kSortOneChunk = 4 * kSortTile;             // lists up to this: one CTA, one launch
+constexpr int kSortMaxBits = 11;
+constexpr int kSortMaxBins = 1 << kSortMaxBits;
+constexpr int64_t kSortMaxEntries = 0x7fffffff - (1 << 25);  // positions are int32
+constexpr int64_t kSortMaxKeys = 0x7ffffffe;             // keys are uint32, n_keys stands for masked
+
+inline int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
+
+// Caller's ids -> keys: 0 .. n_keys - 1, or n_keys for a masked id (sorted behind all others).
+// An id outside the range that is not the masked one is treated as masked and reported.
+template <class I> struct IdKeys {
+  const I* ids;
+  uint32_t n_keys;
+  bool has_ignore;
+  int64_t ignore;
+  int32_t* status;  // may be NULL; host-visible word, set (not ORed) on error
+
+  __device__ uint32_t operator()(int64_t i) const {
+    const int64_t id = static_cast<int64_t>(ids[i]);
+    if (has_ignore && id == ignore) return n_keys;
+    if (static_cast<uint64_t>(id) >= n_keys) {
+      if (status) *reinterpret_cast<volatile int32_t*>(status) = 1 << B2S_ERR_BOUNDS;
+      return n_keys;
+    }
+    return static_cast<uint32_t>(id);
+  }
+};
+
+struct StoredKeys {
+  const uint32_t* keys;
+  __device__ uint32_t operator()(int64_t i) const { return keys[i]; }
+};
+
+// ---- where the sorted entries go ---------------------------------------------------------------
+struct BufferOut {  // between two passes
+  uint32_t* keys;
+  int32_t* vals;
+  __device__ void operator()(uint32_t key, int32_t val, int dst) const {
+    keys[dst] = key;
+    vals[dst] = val;
+  }
+  __device__ void first(int, int) const {}
+};
+struct RunsOut {  // embedding gradient: the sorted list, and which rows are named at all
+  static constexpr bool kOnePass = false;
+  uint32_t* keys;
+  int32_t* vals;
+  uint8_t* named;
+  uint32_t n_keys;
+  __device__ void operator()(uint32_t key, int32_t val, int dst) const {
+    keys[dst] = key;
+    vals[dst] = val;
+    if (key < n_keys) named[key] = 1;
+  }
+  __device__ void first(int, int) const {}
+};
+struct PlanOut {  // token route: slot of each assignment, token of each slot, first slot per expert
+  static constexpr bool kOnePass = true;  // its keys fit one digit: no kernel for a second pass
+  int32_t* slots;
+  int32_t* indptr;
+  int32_t* indices;
+  uint32_t n_experts, k;
+  __device__ void operator()(uint32_t key, int32_t val, int dst) const {
+    slots[val] = key < n_experts ? dst : -1;
+    indices[dst] = static_cast<int32_t>(static_cast<uint32_t>(val) / k);
+  }
+  __device__ void first(int bin, int at) const {
+    if (bin <= static_cast<int>(n_experts)) indptr[bin] = at;
+  }
+};
+
+// ---- device pieces of a pass ---------------------------------------------------------------------
+// counts the digits of entries [lo, hi) into hist[bins] (shared, zeroed by the caller)
+template <class Key>
+__device__ inline void sort_count(const Key& key, int64_t lo, int64_t hi, int shift, int bins,
+                                  int* hist) {
+  const int lane = threadIdx.x & 31;
+  for (int64_t i0 = lo; i0 < hi; i0 += kSortThreads) {
+    const int64_t i = i0 + threadIdx.x;
+    unsigned d = 0xffffffffu;
+    if (i < hi) d = (key(i) >> shift) & (bins - 1);
+    const unsigned peers = __match_any_sync(0xffffffffu, d);
+    if (i < hi && (peers & ((1u << lane) - 1u)) == 0) atomicAdd(hist + d, __popc(peers));
+  }
+}
+
+// exclusive prefix sum of v[bins] (shared) in place; thread t holds bins t * 4 .. t * 4 + 3
+__device__ inline void sort_scan(int* v, int bins, int* warp_tot) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int c[4], run = 0;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int b = threadIdx.x * 4 + q;
+    c[q] = b < bins ? v[b] : 0;
+    run += c[q];
+  }
+  int inc = run;
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += up;
+  }
+  if (lane == 31) warp_tot[warp] = inc;
+  __syncthreads();
+  int at = inc - run;
+  for (int w = 0; w < warp; ++w) at += warp_tot[w];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int b = threadIdx.x * 4 + q;
+    if (b < bins) v[b] = at;
+    at += c[q];
+  }
+  __syncthreads();
+}
+
+// Places entries [lo, hi) in order; off[b] is where the next entry with digit b goes.  A warp
+// takes 32 neighbouring entries per round: those with the same digit are ranked by lane, the
+// rounds and warps of a tile by the counters cnt[warp][digit], tiles by off.
+template <class Key, class Out>
+__device__ inline void sort_place(const Key& key, const int32_t* vals, const Out& out, int64_t lo,
+                                  int64_t hi, int shift, int bins, int* off, int* off_next,
+                                  uint16_t* cnt) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  for (int64_t t0 = lo; t0 < hi; t0 += kSortTile) {
+    uint32_t* z = reinterpret_cast<uint32_t*>(cnt);
+    for (int i = threadIdx.x; i < kSortWarps * bins / 2; i += kSortThreads) z[i] = 0;
+    __syncthreads();
+    uint32_t k[kSortRounds];
+    int rank[kSortRounds];
+    uint16_t* mine = cnt + warp * bins;
+#pragma unroll
+    for (int q = 0; q < kSortRounds; ++q) {
+      const int64_t i = t0 + (warp * kSortRounds + q) * 32 + lane;
+      const bool live = i < hi;
+      k[q] = live ? key(i) : 0;
+      const unsigned d = live ? (k[q] >> shift) & (bins - 1) : 0xffffffffu;
+      const unsigned peers = __match_any_sync(0xffffffffu, d);
+      const int before = __popc(peers & ((1u << lane) - 1u));
+      int prev = 0;
+      if (live) prev = mine[d];
+      __syncwarp();
+      if (live && before == 0) mine[d] = static_cast<uint16_t>(prev + __popc(peers));
+      __syncwarp();
+      rank[q] = prev + before;
+    }
+    __syncthreads();
+    for (int b = threadIdx.x; b < bins; b += kSortThreads) {
+      int run = 0;
+#pragma unroll
+      for (int w = 0; w < kSortWarps; ++w) {
+        const int c = cnt[w * bins + b];
+        cnt[w * bins + b] = static_cast<uint16_t>(run);
+        run += c;
+      }
+      off_next[b] = off[b] + run;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kSortRounds; ++q) {
+      const int64_t i = t0 + (warp * kSortRounds + q) * 32 + lane;
+      if (i < hi) {
+        const int d = (k[q] >> shift) & (bins - 1);
+        out(k[q], vals ? vals[i] : static_cast<int32_t>(i), off[d] + mine[d] + rank[q]);
+      }
+    }
+    int* swap = off;
+    off = off_next;
+    off_next = swap;
+    __syncthreads();
+  }
+}
+
+// shared memory of a pass: off, off_next (int[bins] each), cnt (uint16[warps][bins])
+inline size_t sort_smem(int bins) {
+  return static_cast<size_t>(bins) * (2 * sizeof(int) + kSortWarps * sizeof(uint16_t));
+}
+
+// ---- kernels -------------------------------------------------------------------------------------
+// counts[chunk][digit]; the CTAs also zero `clear` (flags of the caller) and *counter
+template <class Key>
+__global__ void __launch_bounds__(kSortThreads)
+sort_count_kernel(Key key, int64_t n, int64_t chunk, int shift, int bins, int* __restrict__ counts,
+                  uint8_t* __restrict__ clear, int64_t n_clear, int32_t* counter) {
+  extern __shared__ int4 smem4[];
+  int* hist = reinterpret_cast<int*>(smem4);
+  for (int b = threadIdx.x; b < bins; b += kSortThreads) hist[b] = 0;
+  __syncthreads();
+  const int64_t lo = blockIdx.x * chunk, hi = lo + chunk < n ? lo + chunk : n;
+  sort_count(key, lo, hi, shift, bins, hist);
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kSortThreads;
+  for (int64_t i = blockIdx.x * static_cast<int64_t>(kSortThreads) + threadIdx.x;
+       i < (n_clear + 15) / 16; i += stride)
+    reinterpret_cast<uint4*>(clear)[i] = make_uint4(0, 0, 0, 0);
+  if (counter && blockIdx.x == 0 && threadIdx.x == 0) *counter = 0;
+  __syncthreads();
+  for (int b = threadIdx.x; b < bins; b += kSortThreads)
+    counts[blockIdx.x * static_cast<int64_t>(bins) + b] = hist[b];
+}
+
+template <class Key, class Out>
+__global__ void __launch_bounds__(kSortThreads)
+sort_place_kernel(Key key, const int32_t* __restrict__ vals, Out out, int64_t n, int64_t chunk,
+                  int shift, int bins, const int* __restrict__ counts) {
+  extern __shared__ int4 smem4[];
+  __shared__ int warp_tot[kSortWarps];
+  int* off = reinterpret_cast<int*>(smem4);
+  int* before = off + bins;  // off_next until the first tile
+  uint16_t* cnt = reinterpret_cast<uint16_t*>(before + bins);
+  for (int b = threadIdx.x; b < bins; b += kSortThreads) off[b] = before[b] = 0;
+  __syncthreads();
+  // every group of bins / 4 threads sums some of the chunks (integer sums: any order)
+  const int quads = bins / 4, groups = kSortThreads / quads > 0 ? kSortThreads / quads : 1;
+  const int group = threadIdx.x / quads, quad = threadIdx.x - group * quads;
+  if (group < groups) {
+    int4 all = make_int4(0, 0, 0, 0), pre = make_int4(0, 0, 0, 0);
+    const int4* table = reinterpret_cast<const int4*>(counts);
+    const int chunks = gridDim.x, me = blockIdx.x;
+#pragma unroll 8
+    for (int c = group; c < chunks; c += groups) {
+      const int4 v = table[static_cast<int64_t>(c) * quads + quad];
+      all.x += v.x; all.y += v.y; all.z += v.z; all.w += v.w;
+      if (c < me) { pre.x += v.x; pre.y += v.y; pre.z += v.z; pre.w += v.w; }
+    }
+    atomicAdd(off + 4 * quad, all.x); atomicAdd(off + 4 * quad + 1, all.y);
+    atomicAdd(off + 4 * quad + 2, all.z); atomicAdd(off + 4 * quad + 3, all.w);
+    atomicAdd(before + 4 * quad, pre.x); atomicAdd(before + 4 * quad + 1, pre.y);
+    atomicAdd(before + 4 * quad + 2, pre.z); atomicAdd(before + 4 * quad + 3, pre.w);
+  }
+  __syncthreads();
+  sort_scan(off, bins, warp_tot);
+  for (int b = threadIdx.x; b < bins; b += kSortThreads) {
+    if (blockIdx.x == 0) out.first(b, off[b]);
+    off[b] += before[b];
+  }
+  __syncthreads();
+  const int64_t lo = blockIdx.x * chunk, hi = lo + chunk < n ? lo + chunk : n;
+  sort_place(key, vals, out, lo, hi, shift, bins, off, before, cnt);
+}
+
+// a list of one chunk: all passes in one CTA (passes alternate between buf[0] and buf[1])
+template <class Key, class Out>
+__global__ void __launch_bounds__(kSortThreads)
+sort_one_kernel(Key key, Out out, int64_t n, int bits, int passes, BufferOut buf0, BufferOut buf1,
+                uint8_t* __restrict__ clear, int64_t n_clear, int32_t* counter) {
+  extern __shared__ int4 smem4[];
+  __shared__ int warp_tot[kSortWarps];
+  const int bins = 1 << bits;
+  int* off = reinterpret_cast<int*>(smem4);
+  int* next = off + bins;
+  uint16_t* cnt = reinterpret_cast<uint16_t*>(next + bins);
+  for (int64_t i = threadIdx.x; i < (n_clear + 15) / 16; i += kSortThreads)
+    reinterpret_cast<uint4*>(clear)[i] = make_uint4(0, 0, 0, 0);
+  if (counter && threadIdx.x == 0) *counter = 0;
+  for (int p = 0; p < passes; ++p) {
+    const BufferOut& from = (p & 1) ? buf0 : buf1;  // pass p reads what pass p - 1 wrote
+    const BufferOut& to = (p & 1) ? buf1 : buf0;
+    const int shift = p * bits;
+    for (int b = threadIdx.x; b < bins; b += kSortThreads) off[b] = 0;
+    __syncthreads();
+    if (p == 0) {
+      sort_count(key, 0, n, shift, bins, off);
+    } else if constexpr (!Out::kOnePass) {
+      sort_count(StoredKeys{from.keys}, 0, n, shift, bins, off);
+    }
+    __syncthreads();
+    sort_scan(off, bins, warp_tot);
+    const bool last = p + 1 == passes;
+    if (last)
+      for (int b = threadIdx.x; b < bins; b += kSortThreads) out.first(b, off[b]);
+    if (p == 0 && last) sort_place(key, nullptr, out, 0, n, shift, bins, off, next, cnt);
+    if constexpr (!Out::kOnePass) {
+      const StoredKeys stored{from.keys};
+      if (p == 0 && !last) sort_place(key, nullptr, to, 0, n, shift, bins, off, next, cnt);
+      if (p > 0 && last) sort_place(stored, from.vals, out, 0, n, shift, bins, off, next, cnt);
+      if (p > 0 && !last) sort_place(stored, from.vals, to, 0, n, shift, bins, off, next, cnt);
+    }
+    __syncthreads();
+  }
+}
+
+// ---- host ----------------------------------------------------------------------------------------
+struct SortShape {
+  int passes, bits, bins;
+  int64_t chunk, chunks;
+};
+inline SortShape sort_shape(int64_t n, int64_t n_keys) {
+  SortShape s;
+  int width = 2;  // bits of the largest key (n_keys: masked); four bins at least
+  while ((n_keys >> width) > 0) ++width;
+  s.passes = (width + kSortMaxBits - 1) / kSortMaxBits;
+  s.bits = (width + s.passes - 1) / s.passes;
+  s.bins = 1 << s.bits;
+  if (n <= kSortOneChunk) {
+    s.chunk = kSortOneChunk;
+    s.chunks = 1;
+  } else {
+    const int64_t tiles = (n + kSortTile - 1) / kSortTile;
+    s.chunk = (tiles + kSortMaxChunks - 1) / kSortMaxChunks * kSortTile;
+    s.chunks = (n + s.chunk - 1) / s.chunk;
+  }
+  return s;
+}
+// scratch: two (key, value) lists between passes, and the table of counts
+inline int64_t sort_bytes(int64_t n, int64_t n_keys) {
+  const SortShape s = sort_shape(n, n_keys);
+  const int lists = s.passes > 2 ? 2 : s.passes - 1;
+  return lists * 2 * align256(n * 4) + align256(s.chunks * s.bins * 4);
+}
+
+// Sorts ids 0 .. n - 1 into `out`; zeroes clear[0 .. n_clear) (padded to 16) and *counter before
+// any entry is placed.
+template <class I, class Out>
+int sort_ids(const IdKeys<I>& ids, int64_t n, const Out& out, uint8_t* clear, int64_t n_clear,
+             int32_t* counter, unsigned char* ws, cudaStream_t st) {
+  const SortShape s = sort_shape(n, ids.n_keys);
+  const int lists = s.passes > 2 ? 2 : s.passes - 1;
+  BufferOut buf[2] = {{nullptr, nullptr}, {nullptr, nullptr}};
+  for (int b = 0; b < lists; ++b) {
+    buf[b].keys = reinterpret_cast<uint32_t*>(ws); ws += align256(n * 4);
+    buf[b].vals = reinterpret_cast<int32_t*>(ws); ws += align256(n * 4);
+  }
+  int* counts = reinterpret_cast<int*>(ws);
+  const size_t smem = sort_smem(s.bins);
+  if (s.chunks == 1) {
+    ensure_dyn_smem(reinterpret_cast<const void*>(&sort_one_kernel<IdKeys<I>, Out>),
+                    sort_smem(kSortMaxBins));
+    sort_one_kernel<IdKeys<I>, Out><<<1, kSortThreads, smem, st>>>(
+        ids, out, n, s.bits, s.passes, buf[0], buf[1], clear, n_clear, counter);
+    return launch_status();
+  }
+  const unsigned grid = static_cast<unsigned>(s.chunks);
+  auto place = [&](const auto& key, const int32_t* vals, const auto& to, int shift) {
+    auto kernel = &sort_place_kernel<std::decay_t<decltype(key)>, std::decay_t<decltype(to)>>;
+    ensure_dyn_smem(reinterpret_cast<const void*>(kernel), sort_smem(kSortMaxBins));
+    kernel<<<grid, kSortThreads, smem, st>>>(key, vals, to, n, s.chunk, shift, s.bins, counts);
+  };
+  sort_count_kernel<<<grid, kSortThreads, s.bins * sizeof(int), st>>>(
+      ids, n, s.chunk, 0, s.bins, counts, clear, n_clear, counter);
+  if constexpr (Out::kOnePass) {
+    place(ids, nullptr, out, 0);
+  } else {
+    if (s.passes == 1) place(ids, nullptr, out, 0);
+    else place(ids, nullptr, buf[0], 0);
+    for (int p = 1; p < s.passes; ++p) {
+      const BufferOut& from = (p & 1) ? buf[0] : buf[1];
+      const StoredKeys stored{from.keys};
+      sort_count_kernel<<<grid, kSortThreads, s.bins * sizeof(int), st>>>(
+          stored, n, s.chunk, p * s.bits, s.bins, counts, static_cast<uint8_t*>(nullptr),
+          int64_t(0), static_cast<int32_t*>(nullptr));
+      if (p + 1 == s.passes) place(stored, from.vals, out, p * s.bits);
+      else place(stored, from.vals, (p & 1) ? buf[1] : buf[0], p * s.bits);
+    }
+  }
+  return launch_status();
+}
+
+}  // namespace b2s

@@ -1,0 +1,583 @@
+"""Products with a selection matrix: the embedding lookup and its gradient, and tokens sorted by
+expert and back.
+
+The sparse matrices of a language model select rows.  ``tokens`` stands for the matrix S with
+S[i, tokens[i]] = 1; ``experts`` (n_tokens x k) for the matrix R that has a one for every
+assignment of a token to an expert.  The calls here are the products that ``flagsparse_spmm_csr``
+computes when such a matrix is written out as CSR, without writing it out, checking it or keeping
+a plan of it, together with the gradients that training needs:
+
+    flagsparse_embedding        alpha * S @ table + beta * out
+    flagsparse_embedding_grad   alpha * S.T @ grad + beta * out
+    prepare_token_route         the rows of R sorted by expert: slots, indptr, indices
+    flagsparse_token_dispatch   the tokens' rows in that order (and flagsparse_token_dispatch_grad)
+    flagsparse_token_combine    the weighted sum of a token's rows (and ..._combine_grad)
+
+FlagSparse has no counterpart (its gather / scatter take one vector, gather_scatter.py:22-81).
+
+The lookup, the dispatch and the combine are differentiable: when an input requires a gradient
+and gradients are enabled they record themselves for ``torch.autograd``.  Inside a CUDA graph
+capture that is refused (autograd may run a leaf's accumulation on a stream outside the capture);
+captured training steps call the ``*_grad`` functions.
+
+Nothing synchronises.  Ids are checked by the kernels: one outside its range selects nothing, and
+IndexError is raised by the next call on that device, or by ``check_selection_ids()``, which waits
+for the device.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import threading
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._contract import SUPPORTED_INDEX_DTYPES, check_scalar
+from .spmm import _row_major_ok
+
+SUPPORTED_SELECTION_VALUE_DTYPES = (torch.float16, torch.bfloat16, torch.float32, torch.float64)
+MAX_EXPERTS = 2047               # the plan sorts by one digit of 11 bits
+MAX_ENTRIES = 2**31 - 1 - 2**25  # positions are int32
+MAX_ROWS = 2**31 - 2
+MAX_DIM = 1 << 22
+
+_WORDS = {}
+_WORDS_LOCK = threading.Lock()
+
+
+# -------------------------------------------------------------------------------------------------
+# errors that kernels report
+# -------------------------------------------------------------------------------------------------
+class _StatusWord:
+    """One int32 in pinned host memory per device; the kernels set it when they meet an id
+    outside its range, and the host reads it without a copy or a synchronisation."""
+
+    def __init__(self):
+        self.memory = torch.zeros(1, dtype=torch.int32).pin_memory()
+        self.address = self.memory.data_ptr()
+        self.value = ctypes.c_int32.from_address(self.address)
+
+    def check(self):
+        if self.value.value:
+            self.value.value = 0
+            raise IndexError("a token or expert id given to an earlier call on this device lies "
+                             "outside its range")
+
+
+def _status_word(index):
+    word = _WORDS.get(index)
+    if word is None:
+        with _WORDS_LOCK:
+            word = _WORDS.get(index)
+            if word is None:
+                word = _WORDS[index] = _StatusWord()
+    word.check()
+    return word.address
+
+
+def check_selection_ids(device=None):
+    """Wait for `device` (default: the current one) and raise IndexError if a kernel of this
+    module met an id outside its range since the last check."""
+    index = torch.device("cuda" if device is None else device).index
+    if index is None:
+        index = torch.cuda.current_device()
+    torch.cuda.synchronize(index)
+    word = _WORDS.get(index)
+    if word is not None:
+        word.check()
+
+
+# -------------------------------------------------------------------------------------------------
+# arguments
+# -------------------------------------------------------------------------------------------------
+def _check_ids(t, name):
+    if not torch.is_tensor(t):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype not in SUPPORTED_INDEX_DTYPES:
+        raise TypeError(f"{name} dtype must be torch.int32 or torch.int64")
+
+
+def _check_values(t, name):
+    if not torch.is_tensor(t):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype not in SUPPORTED_SELECTION_VALUE_DTYPES:
+        raise TypeError(f"{name} dtype must be one of: float16, bfloat16, float32, float64")
+
+
+def _check_device(named):
+    first = None
+    for name, t in named:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor")
+        if first is None:
+            first = (name, t.device)
+        elif t.device != first[1]:
+            raise ValueError(f"{name} must be on the same CUDA device as {first[0]}")
+    return first[1]
+
+
+def _check_size(name, value, limit):
+    if value > limit:
+        raise ValueError(f"{name} must be at most {limit}, got {value}")
+
+
+def _as_int(value, name):
+    if isinstance(value, bool) or not hasattr(value, "__index__"):
+        raise TypeError(f"{name} must be an integer")
+    return value.__index__()
+
+
+def _wants_grad(*tensors):
+    if not torch.is_grad_enabled():
+        return False
+    return any(t is not None and t.requires_grad for t in tensors)
+
+
+def _refuse_capture():
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(
+            "differentiable calls are not recorded inside a CUDA graph capture: call them under "
+            "torch.no_grad() and take the gradients with the *_grad functions")
+
+
+def _refuse_out(out, tensors):
+    if out is not None and _wants_grad(out, *tensors):
+        raise RuntimeError("out= does not support automatic differentiation, but one of the "
+                           "arguments requires grad")
+
+
+def _rows(t):
+    """`t` (2-D) with unit stride inside a row and rows that do not overlap; copied if need be."""
+    return t if _row_major_ok(t) else t.contiguous()
+
+
+def _pitch(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+class _Result:
+    """Where a call writes: a new tensor, `out` itself, or (when the kernels cannot write its
+    layout) a contiguous stand-in that is copied into `out` afterwards."""
+
+    __slots__ = ("out", "flat", "stand_in")
+
+    def __init__(self, out, shape, dtype, device, beta, what="out"):
+        rows = 1
+        for n in shape[:-1]:
+            rows *= n
+        self.out, self.stand_in = out, False
+        if out is None:
+            if beta != 0:
+                raise ValueError("beta != 0 requires out= holding the rows to scale")
+            self.out = torch.empty(shape, dtype=dtype, device=device)
+            self.flat = self.out if len(shape) == 2 else self.out.view(rows, shape[-1])
+            return
+        if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
+            raise ValueError("out shape/dtype must match result")
+        if len(shape) == 2:
+            flat = out
+        else:
+            try:
+                flat = out.view(rows, shape[-1])
+            except RuntimeError:
+                flat = None
+        if flat is None or not _row_major_ok(flat):
+            flat = out.reshape(rows, shape[-1]).contiguous() if beta != 0 else torch.empty(
+                (rows, shape[-1]), dtype=dtype, device=device)
+            self.stand_in = True
+        self.flat = flat
+
+    def done(self, given):
+        if self.stand_in:
+            self.out.copy_(self.flat.view(self.out.shape))
+        elif given is not None:
+            # written by a kernel: tell autograd (and everything else that watches the counter)
+            torch.autograd.graph.increment_version(given)
+        return self.out
+
+
+def _call(device, fn, *args):
+    """fn(*args, stream of `device`) with `device` current; raise on a non-zero status."""
+    index = device.index
+    if torch.cuda.current_device() == index:
+        st = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    else:
+        with torch.cuda.device(index):
+            st = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+    if st:
+        _lib.check(st, fn.__name__)
+
+
+# -------------------------------------------------------------------------------------------------
+# embedding
+# -------------------------------------------------------------------------------------------------
+def _ignored(ignore_index):
+    if ignore_index is None:
+        return 0, 0
+    value = _as_int(ignore_index, "ignore_index")
+    if not -2**63 <= value < 2**63:
+        raise ValueError("ignore_index must fit int64")
+    return 1, value
+
+
+def flagsparse_embedding(tokens, table, alpha=1.0, ignore_index=None, out=None, beta=0.0):
+    """alpha * table[tokens] + beta * out: the rows of `table` that `tokens` names, scaled.
+
+    tokens: integer tensor of any shape; table: (n_rows, dim), float16 / bfloat16 / float32 /
+    float64.  The result has the shape tokens.shape + (dim,) and the table's dtype; the product is
+    formed in float32 (float64) and rounded once.  Where a token equals `ignore_index` (any
+    integer, inside the table or not) nothing is selected: the row is beta * out, zero for beta = 0.
+    alpha, beta are numbers; beta != 0 needs `out`.
+    Differentiable in `table` (a dense gradient, see flagsparse_embedding_grad).
+    """
+    _check_ids(tokens, "tokens")
+    _check_values(table, "table")
+    if table.ndim != 2:
+        raise ValueError("table must be a 2D tensor: (n_rows, dim)")
+    alpha = check_scalar(alpha, table.dtype, "alpha")
+    beta = check_scalar(beta, table.dtype, "beta")
+    has_ignore, ignore = _ignored(ignore_index)
+    _refuse_out(out, (table,))
+    device = _check_device((("table", table), ("tokens", tokens), ("out", out)))
+    if _wants_grad(table):
+        _refuse_capture()
+        return _Embedding.apply(tokens, table, alpha, has_ignore, ignore)
+    return _embedding(tokens, table, alpha, has_ignore, ignore, out, beta, device)
+
+
+def _embedding(tokens, table, alpha, has_ignore, ignore, out, beta, device):
+    n_rows, dim = table.shape
+    n = tokens.numel()
+    _check_size("the number of tokens", n, MAX_ENTRIES)
+    _check_size("the number of rows of table", n_rows, MAX_ROWS)
+    _check_size("dim", dim, MAX_DIM)
+    result = _Result(out, (*tokens.shape, dim), table.dtype, device, beta)
+    if not tokens.is_contiguous():
+        tokens = tokens.contiguous()
+    table, flat = _rows(table), result.flat
+    lib = _lib.load()
+    _call(device, lib.b2s_select_rows, _lib.VALUE_CODE[table.dtype],
+          _lib.INDEX_CODE[tokens.dtype], tokens.data_ptr(), n, has_ignore, ignore,
+          table.data_ptr(), n_rows, _pitch(table), dim, flat.data_ptr(), _pitch(flat), alpha, beta,
+          _status_word(device.index))
+    return result.done(out)
+
+
+def flagsparse_embedding_grad(tokens, grad, n_rows, alpha=1.0, ignore_index=None, out=None,
+                              beta=0.0, out_dtype=None):
+    """alpha * (sum of grad over equal tokens) + beta * out: the gradient of an embedding table
+    of `n_rows` rows from the gradient of its looked-up rows.
+
+    grad: tokens.shape + (dim,).  The result is (n_rows, dim), of grad's dtype or, for float16 and
+    bfloat16, of float32 (`out_dtype`, or the dtype of `out`).  beta = 0 writes every row (zero
+    where no token names it); beta = 1 adds to `out` and touches the named rows only.
+    The tokens are sorted, and the rows of one token are summed in float32 (float64) in a fixed
+    order: the result is the same from run to run.
+    """
+    _check_ids(tokens, "tokens")
+    _check_values(grad, "grad")
+    n_rows = _as_int(n_rows, "n_rows")
+    if n_rows < 0:
+        raise ValueError("n_rows must be non-negative")
+    if grad.ndim != tokens.ndim + 1 or grad.shape[:-1] != tokens.shape:
+        raise ValueError(f"grad shape must be tokens.shape + (dim,), got {tuple(grad.shape)} for "
+                         f"tokens of shape {tuple(tokens.shape)}")
+    if out_dtype is None:
+        out_dtype = grad.dtype if out is None else out.dtype
+    if out_dtype != grad.dtype and not (out_dtype == torch.float32 and grad.element_size() == 2):
+        raise TypeError("out dtype must be the dtype of grad, or float32 for float16 / bfloat16")
+    alpha = check_scalar(alpha, grad.dtype, "alpha")
+    beta = check_scalar(beta, grad.dtype, "beta")
+    has_ignore, ignore = _ignored(ignore_index)
+    _refuse_out(out, (grad,))
+    device = _check_device((("grad", grad), ("tokens", tokens), ("out", out)))
+    dim = grad.shape[-1]
+    n = tokens.numel()
+    _check_size("the number of tokens", n, MAX_ENTRIES)
+    _check_size("n_rows", n_rows, MAX_ROWS)
+    _check_size("dim", dim, MAX_DIM)
+    result = _Result(out, (n_rows, dim), out_dtype, device, beta)
+    if not tokens.is_contiguous():
+        tokens = tokens.contiguous()
+    grad, flat = _rows(grad if grad.ndim == 2 else grad.reshape(n, dim)), result.flat
+    lib = _lib.load()
+    vcode = _lib.VALUE_CODE[grad.dtype]
+    nbytes = lib.b2s_select_grad_bytes(vcode, n, n_rows, dim)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    _call(device, lib.b2s_select_grad, vcode, _lib.VALUE_CODE[out_dtype],
+          _lib.INDEX_CODE[tokens.dtype], tokens.data_ptr(), n, has_ignore, ignore,
+          grad.data_ptr(), _pitch(grad), n_rows, dim, flat.data_ptr(), _pitch(flat), alpha, beta,
+          ws.data_ptr(), nbytes, _status_word(device.index))
+    return result.done(out)
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, tokens, table, alpha, has_ignore, ignore):
+        ctx.save_for_backward(tokens)
+        ctx.args = (table.shape[0], alpha, ignore if has_ignore else None)
+        return _embedding(tokens, table, alpha, has_ignore, ignore, None, 0.0, table.device)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        _refuse_capture()
+        n_rows, alpha, ignore = ctx.args
+        grad_table = flagsparse_embedding_grad(ctx.saved_tensors[0], grad, n_rows, alpha=alpha,
+                                               ignore_index=ignore)
+        return None, grad_table, None, None, None
+
+
+# -------------------------------------------------------------------------------------------------
+# tokens to experts and back
+# -------------------------------------------------------------------------------------------------
+class TokenRoute:
+    """Where every assignment of a token to an expert stands when they are sorted by expert.
+
+    slots    int32 (n_tokens, k): the row of assignment (t, j) among the sorted rows, -1 if masked
+    indptr   int32 (n_experts + 1,): the rows of expert e are indptr[e] .. indptr[e + 1] - 1
+    indices  int32 (n_tokens * k,): the token of each row (of the first indptr[-1] rows)
+
+    (indptr, indices) is the experts x tokens matrix of the route in CSR form.  Masked assignments
+    have no row: the rows from indptr[-1] on belong to nobody and are kept zero.
+    """
+
+    __slots__ = ("slots", "indptr", "indices", "n_tokens", "k", "n_experts", "device", "_stream")
+
+    def __init__(self, slots, indptr, indices, n_experts, stream):
+        self.slots, self.indptr, self.indices = slots, indptr, indices
+        self.n_tokens, self.k = slots.shape
+        self.n_experts = n_experts
+        self.device = slots.device
+        self._stream = stream
+
+    @property
+    def n_rows(self):
+        """Rows of the sorted array: n_tokens * k, whatever is masked."""
+        return self.n_tokens * self.k
+
+    def _use(self):
+        """Called before a launch: keeps the arrays from being reused while a stream other than
+        the one they were made on still reads them."""
+        stream = torch.cuda.current_stream(self.device)
+        if stream.cuda_stream != self._stream and not torch.cuda.is_current_stream_capturing():
+            for t in (self.slots, self.indptr, self.indices):
+                t.record_stream(stream)
+
+    def __repr__(self):
+        return (f"TokenRoute(n_tokens={self.n_tokens}, k={self.k}, n_experts={self.n_experts}, "
+                f"device={self.device})")
+
+
+def prepare_token_route(experts, n_experts):
+    """Sort the assignments experts[t, j] (int32 / int64, -1: masked) by expert, keeping their
+    order within an expert, and return the TokenRoute.  Nothing is read back to the host."""
+    _check_ids(experts, "experts")
+    if experts.ndim != 2:
+        raise ValueError("experts must be a 2D tensor: (n_tokens, k)")
+    n_experts = _as_int(n_experts, "n_experts")
+    if not 0 <= n_experts <= MAX_EXPERTS:
+        raise ValueError(f"n_experts must be between 0 and {MAX_EXPERTS}, got {n_experts}")
+    n_tokens, k = experts.shape
+    _check_size("n_tokens * k", n_tokens * k, MAX_ENTRIES)
+    device = _check_device((("experts", experts),))
+    if not experts.is_contiguous():
+        experts = experts.contiguous()
+    slots = torch.empty((n_tokens, k), dtype=torch.int32, device=device)
+    indptr = torch.empty(n_experts + 1, dtype=torch.int32, device=device)
+    indices = torch.empty(n_tokens * k, dtype=torch.int32, device=device)
+    lib = _lib.load()
+    nbytes = lib.b2s_route_plan_bytes(n_tokens, k, n_experts)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    _call(device, lib.b2s_route_plan, _lib.INDEX_CODE[experts.dtype], experts.data_ptr(), n_tokens,
+          k, n_experts, slots.data_ptr(), indptr.data_ptr(), indices.data_ptr(), ws.data_ptr(),
+          nbytes, _status_word(device.index))
+    return TokenRoute(slots, indptr, indices, n_experts,
+                      torch.cuda.current_stream(device).cuda_stream)
+
+
+def _check_route(route):
+    if not isinstance(route, TokenRoute):
+        raise TypeError("route must be a TokenRoute (prepare_token_route)")
+
+
+def _check_matrix(t, name, rows, what):
+    _check_values(t, name)
+    if t.ndim != 2:
+        raise ValueError(f"{name} must be a 2D tensor: ({what}, dim)")
+    if t.shape[0] != rows:
+        raise ValueError(f"{name}.shape[0] must be {what}={rows}, got {t.shape[0]}")
+    _check_size("dim", t.shape[1], MAX_DIM)
+
+
+def _check_weights(weights, route, dtype):
+    if weights is None:
+        return
+    _check_values(weights, "weights")
+    if weights.dtype != dtype and weights.dtype != torch.float32:
+        raise TypeError("weights dtype must be the dtype of the rows, or float32")
+    if tuple(weights.shape) != (route.n_tokens, route.k):
+        raise ValueError(f"weights shape must be {(route.n_tokens, route.k)}, got "
+                         f"{tuple(weights.shape)}")
+
+
+def flagsparse_token_dispatch(x, route, out=None):
+    """The tokens' rows sorted by expert: row route.slots[t, j] of the result is x[t].
+
+    x: (n_tokens, dim); the result is (n_tokens * k, dim) of x's dtype, its rows from
+    route.indptr[-1] on (left by masked assignments) zero.  Differentiable in x.
+    """
+    _check_route(route)
+    _check_matrix(x, "x", route.n_tokens, "n_tokens")
+    _refuse_out(out, (x,))
+    _check_device((("route", route.slots), ("x", x), ("out", out)))
+    if _wants_grad(x):
+        _refuse_capture()
+        return _Dispatch.apply(x, route)
+    return _dispatch(x, route, out)
+
+
+def _dispatch(x, route, out):
+    dim = x.shape[1]
+    result = _Result(out, (route.n_rows, dim), x.dtype, route.device, 0.0)
+    x, flat = _rows(x), result.flat
+    route._use()
+    _call(route.device, _lib.load().b2s_route_dispatch, _lib.VALUE_CODE[x.dtype], x.data_ptr(),
+          _pitch(x), route.n_tokens, route.k, dim, route.slots.data_ptr(),
+          route.indptr.data_ptr() + 4 * route.n_experts, flat.data_ptr(), _pitch(flat))
+    return result.done(out)
+
+
+def flagsparse_token_dispatch_grad(grad, route, out=None, beta=0.0):
+    """The gradient of flagsparse_token_dispatch: row t is the sum of grad[route.slots[t, j]] over
+    the j that are not masked (float32 / float64 sums, one rounding), plus beta * out.
+
+    grad: (n_tokens * k, dim); its rows from route.indptr[-1] on are not read.
+    """
+    _check_route(route)
+    _check_matrix(grad, "grad", route.n_rows, "n_tokens * k")
+    beta = check_scalar(beta, grad.dtype, "beta")
+    _refuse_out(out, (grad,))
+    _check_device((("route", route.slots), ("grad", grad), ("out", out)))
+    return _combine(grad, route, None, 1.0, out, beta)
+
+
+def flagsparse_token_combine(y, route, weights=None, alpha=1.0, out=None, beta=0.0):
+    """The rows of each token brought back and summed with their weights:
+    alpha * sum_j weights[t, j] * y[route.slots[t, j]] + beta * out[t], without the masked j.
+
+    y: (n_tokens * k, dim); weights: (n_tokens, k) of y's dtype or float32, None for ones.  The
+    result is (n_tokens, dim) of y's dtype: float32 (float64) sums, one rounding; a token whose
+    assignments are all masked gets beta * out.  Differentiable in y and weights.
+    """
+    _check_route(route)
+    _check_matrix(y, "y", route.n_rows, "n_tokens * k")
+    _check_weights(weights, route, y.dtype)
+    alpha = check_scalar(alpha, y.dtype, "alpha")
+    beta = check_scalar(beta, y.dtype, "beta")
+    _refuse_out(out, (y, weights))
+    _check_device((("route", route.slots), ("y", y), ("weights", weights), ("out", out)))
+    if _wants_grad(y, weights):
+        _refuse_capture()
+        return _Combine.apply(y, weights, route, alpha)
+    return _combine(y, route, weights, alpha, out, beta)
+
+
+def _combine(y, route, weights, alpha, out, beta):
+    dim = y.shape[1]
+    result = _Result(out, (route.n_tokens, dim), y.dtype, route.device, beta)
+    y, flat = _rows(y), result.flat
+    wcode = 0
+    if weights is not None:
+        if not weights.is_contiguous():
+            weights = weights.contiguous()
+        wcode = _lib.VALUE_CODE[weights.dtype]
+    route._use()
+    _call(route.device, _lib.load().b2s_route_combine, _lib.VALUE_CODE[y.dtype], y.data_ptr(),
+          _pitch(y), route.slots.data_ptr(), wcode,
+          None if weights is None else weights.data_ptr(), route.n_tokens, route.k, dim,
+          flat.data_ptr(), _pitch(flat), alpha, beta)
+    return result.done(out)
+
+
+def flagsparse_token_combine_grad(grad, y, route, weights=None, alpha=1.0):
+    """The gradients of flagsparse_token_combine: (grad_y, grad_weights).
+
+    grad: (n_tokens, dim).  grad_y[route.slots[t, j]] = alpha * weights[t, j] * grad[t] (rows that
+    belong to nobody are zero); grad_weights[t, j] = alpha * <grad[t], y[route.slots[t, j]]> in the
+    dtype of weights, zero where masked.  Without weights, y may be None and grad_weights is None.
+    """
+    _check_route(route)
+    _check_matrix(grad, "grad", route.n_tokens, "n_tokens")
+    _check_weights(weights, route, grad.dtype)
+    if weights is not None:
+        if y is None:
+            raise ValueError("y is needed for the gradient of weights")
+    if y is not None:
+        _check_matrix(y, "y", route.n_rows, "n_tokens * k")
+        if y.dtype != grad.dtype:
+            raise TypeError("y dtype must match grad dtype")
+        if y.shape[1] != grad.shape[1]:
+            raise ValueError("y and grad must have the same number of columns")
+    alpha = check_scalar(alpha, grad.dtype, "alpha")
+    _check_device((("route", route.slots), ("grad", grad), ("y", y), ("weights", weights)))
+    return _combine_grad(grad, y, route, weights, alpha, weights is not None)
+
+
+def _combine_grad(grad, y, route, weights, alpha, want_weights):
+    dim = grad.shape[1]
+    grad = _rows(grad)
+    grad_y = torch.empty((route.n_rows, dim), dtype=grad.dtype, device=route.device)
+    grad_w, wcode = None, 0
+    if weights is not None:
+        if not weights.is_contiguous():
+            weights = weights.contiguous()
+        wcode = _lib.VALUE_CODE[weights.dtype]
+        if want_weights:
+            y = _rows(y)
+            grad_w = torch.empty((route.n_tokens, route.k), dtype=weights.dtype,
+                                 device=route.device)
+    route._use()
+    _call(route.device, _lib.load().b2s_route_combine_grad, _lib.VALUE_CODE[grad.dtype],
+          grad.data_ptr(), _pitch(grad), None if grad_w is None else y.data_ptr(),
+          0 if grad_w is None else _pitch(y), route.slots.data_ptr(),
+          route.indptr.data_ptr() + 4 * route.n_experts, wcode,
+          None if weights is None else weights.data_ptr(), route.n_tokens, route.k, dim, alpha,
+          grad_y.data_ptr(), dim, None if grad_w is None else grad_w.data_ptr())
+    return grad_y, grad_w
+
+
+class _Dispatch(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, route):
+        ctx.route = route
+        return _dispatch(x, route, None)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        _refuse_capture()
+        return flagsparse_token_dispatch_grad(grad, ctx.route), None
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, weights, route, alpha):
+        ctx.route, ctx.alpha = route, alpha
+        wants_weights = ctx.needs_input_grad[1]
+        ctx.wants_weights = wants_weights
+        # y is read by the gradient of the weights only
+        ctx.save_for_backward(y if wants_weights else None, weights)
+        return _combine(y, route, weights, alpha, None, 0.0)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        _refuse_capture()
+        y, weights = ctx.saved_tensors
+        grad_y, grad_w = _combine_grad(grad, y, ctx.route, weights, ctx.alpha, ctx.wants_weights)
+        return grad_y, grad_w, None, None

@@ -36,9 +36,10 @@ typedef enum {
   B2S_ERR_WORKSPACE = 6,  /* scratch buffer smaller than *_bytes() asked for      */
   B2S_ERR_RANGE = 7,      /* a size does not fit the requested index dtype        */
   B2S_ERR_TOO_LARGE = 8,  /* problem exceeds the fixed scratch of b2s_spmv_csr_fixed */
-  B2S_ERR_BOUNDS = 9      /* (device status word, bounds-checked build only) a column index or
-                             row pointer read from the matrix points outside its array; the
-                             access was skipped                                       */
+  B2S_ERR_BOUNDS = 9      /* (device status word) an id given to b2s_select_* / b2s_route_plan
+                             lies outside the table or the experts; in the bounds-checked build
+                             also: a column index or row pointer read from the matrix points
+                             outside its array.  The access was skipped               */
 } b2s_status;
 
 /* value dtypes (FlagSparse's SUPPORTED_VALUE_DTYPES, _common.py:21-29).  B2S_F16 / B2S_BF16:
@@ -374,6 +375,67 @@ int b2s_csr2csc(int val_type, int idx_type, int ptr_type,
                 int64_t n_rows, int64_t n_cols, int64_t nnz, int conj,
                 void* t_data_dev, void* t_indices_dev, void* t_indptr_dev,
                 void* scratch_dev, int64_t scratch_bytes, b2s_stream stream);
+
+/* ---- products with a selection matrix ----------------------------------------------------------
+ * No counterpart in the reference, whose SpMM needs the matrix written out.  S is given by ids and
+ * never formed.  val_type is B2S_F16, B2S_BF16, B2S_F32 or B2S_F64; sums and scalars are float32
+ * for the 16-bit types and every result is rounded once.  Rows are row-major with a pitch of ld
+ * elements (ld >= dim).  alpha and beta are passed by value.  Results do not depend on scheduling:
+ * no floating-point atomics.
+ *   status  may be NULL; one int32 the device can write (pinned host memory will do) that is SET
+ *           to 1 << B2S_ERR_BOUNDS when an id lies outside its range.  Such an id is then treated
+ *           as a masked one.  It is not shared with calls that OR other bits into theirs.
+ *
+ * b2s_select_rows: out[i] = alpha * table[idx[i]] + beta * out[i] for i < n (out is not read when
+ * beta is 0).  Where has_ignore != 0 and idx[i] == ignore, the row of S is empty: beta * out[i].
+ *
+ * b2s_select_grad: out[v] = alpha * (sum of grad[i] over the i with idx[i] == v) + beta * out[v]
+ * for every v < n_rows; the sum runs over ascending i in pieces of at most 63 rows.  out_type is
+ * val_type, or B2S_F32 for the 16-bit types.  beta = 1 touches the rows that idx names only.
+ * ws: b2s_select_grad_bytes() bytes, 256-byte aligned. */
+int b2s_select_rows(int val_type, int idx_type, const void* idx_dev, int64_t n, int has_ignore,
+                    int64_t ignore, const void* table_dev, int64_t n_rows, int64_t ld_table,
+                    int64_t dim, void* out_dev, int64_t ld_out, double alpha, double beta,
+                    int32_t* status, b2s_stream stream);
+int64_t b2s_select_grad_bytes(int val_type, int64_t n, int64_t n_rows, int64_t dim);
+int b2s_select_grad(int val_type, int out_type, int idx_type, const void* idx_dev, int64_t n,
+                    int has_ignore, int64_t ignore, const void* grad_dev, int64_t ld_grad,
+                    int64_t n_rows, int64_t dim, void* out_dev, int64_t ld_out, double alpha,
+                    double beta, void* ws_dev, int64_t ws_bytes, int32_t* status,
+                    b2s_stream stream);
+
+/* Routing: assignment a = t * k + j sends token t to expert experts[a] (-1: to none).
+ * b2s_route_plan sorts the assignments by expert, keeping their order within an expert:
+ *   slots[a]     place of a among the sorted rows, -1 for a masked one
+ *   indptr[e]    first place of expert e; indptr[n_experts] = number of places held
+ *   indices[p]   token of place p; (indptr, indices) is the experts x tokens matrix in CSR form
+ * All int32; n_experts <= 2047.  ws: b2s_route_plan_bytes() bytes, 256-byte aligned.
+ *
+ * b2s_route_dispatch: rows[slots[a]] = x[a / k]; the rows from *held_dev (= indptr[n_experts]) to
+ * n_tokens * k are zeroed.
+ * b2s_route_combine: out[t] = alpha * sum_j w[t, j] * y[slots[t, j]] + beta * out[t], without the
+ * masked j.  weights NULL: all one (with beta = 0 that is the gradient of the dispatch).
+ * w_type: val_type or B2S_F32.
+ * b2s_route_combine_grad: grad_y[slots[a]] = alpha * w[a] * g[a / k], the rows behind the held
+ * ones zeroed; grad_w[a] (w_type; may be NULL, y is then not read) = alpha * <g[a / k],
+ * y[slots[a]]>, 0 for a masked a. */
+int64_t b2s_route_plan_bytes(int64_t n_tokens, int64_t k, int64_t n_experts);
+int b2s_route_plan(int idx_type, const void* experts_dev, int64_t n_tokens, int64_t k,
+                   int64_t n_experts, int32_t* slots_dev, int32_t* indptr_dev,
+                   int32_t* indices_dev, void* ws_dev, int64_t ws_bytes, int32_t* status,
+                   b2s_stream stream);
+int b2s_route_dispatch(int val_type, const void* x_dev, int64_t ld_x, int64_t n_tokens, int64_t k,
+                       int64_t dim, const int32_t* slots_dev, const int32_t* held_dev,
+                       void* rows_dev, int64_t ld_rows, b2s_stream stream);
+int b2s_route_combine(int val_type, const void* y_dev, int64_t ld_y, const int32_t* slots_dev,
+                      int w_type, const void* weights_dev, int64_t n_tokens, int64_t k,
+                      int64_t dim, void* out_dev, int64_t ld_out, double alpha, double beta,
+                      b2s_stream stream);
+int b2s_route_combine_grad(int val_type, const void* g_dev, int64_t ld_g, const void* y_dev,
+                           int64_t ld_y, const int32_t* slots_dev, const int32_t* held_dev,
+                           int w_type, const void* weights_dev, int64_t n_tokens, int64_t k,
+                           int64_t dim, double alpha, void* grad_y_dev, int64_t ld_gy,
+                           void* grad_w_dev, b2s_stream stream);
 
 #ifdef __cplusplus
 }

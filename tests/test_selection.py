@@ -1,0 +1,241 @@
+"""Selection products (embedding, token route) on the CPU: what they refuse before anything
+touches a device, the status codes of the C entry points, and the work split of the gradient
+kernel restated in Python."""
+
+import ctypes
+import random
+
+import pytest
+import torch
+
+import flagsparse_b200 as fs
+from flagsparse_b200 import _lib, selection
+
+TOK = torch.zeros(3, dtype=torch.int64)
+TABLE = torch.zeros(5, 4)
+
+
+def test_public_names():
+    for name in ("flagsparse_embedding", "flagsparse_embedding_grad", "prepare_token_route",
+                 "TokenRoute", "flagsparse_token_dispatch", "flagsparse_token_dispatch_grad",
+                 "flagsparse_token_combine", "flagsparse_token_combine_grad",
+                 "check_selection_ids"):
+        assert name in fs.__all__ and callable(getattr(fs, name))
+
+
+@pytest.mark.parametrize("args, kwargs, error, message", [
+    ((TOK.float(), TABLE), {}, TypeError, "tokens dtype must be torch.int32 or torch.int64"),
+    (([0, 1], TABLE), {}, TypeError, "tokens must be a torch.Tensor"),
+    ((TOK, TABLE.to(torch.complex64)), {}, TypeError, "table dtype must be one of"),
+    ((TOK, TABLE.long()), {}, TypeError, "table dtype must be one of"),
+    ((TOK, TABLE[0]), {}, ValueError, "table must be a 2D tensor"),
+    ((TOK, TABLE), {"alpha": 1j}, TypeError, "alpha is complex"),
+    ((TOK, TABLE), {"alpha": torch.ones(2)}, ValueError, "alpha must be a scalar"),
+    ((TOK, TABLE), {"ignore_index": 1.0}, TypeError, "ignore_index must be an integer"),
+    ((TOK, TABLE), {"ignore_index": True}, TypeError, "ignore_index must be an integer"),
+    ((TOK, TABLE), {"ignore_index": 2**63}, ValueError, "ignore_index must fit int64"),
+    ((TOK, TABLE), {}, ValueError, "table must be a CUDA tensor"),
+    ((TOK, TABLE.clone().requires_grad_()), {"out": torch.zeros(3, 4)}, RuntimeError,
+     "does not support automatic differentiation"),
+])
+def test_embedding_refuses(args, kwargs, error, message):
+    with pytest.raises(error, match=message):
+        fs.flagsparse_embedding(*args, **kwargs)
+
+
+@pytest.mark.parametrize("args, kwargs, error, message", [
+    ((TOK, torch.zeros(3, 4), -1), {}, ValueError, "n_rows must be non-negative"),
+    ((TOK, torch.zeros(3, 4), 2.0), {}, TypeError, "n_rows must be an integer"),
+    ((TOK, torch.zeros(4, 4), 5), {}, ValueError, "grad shape must be tokens.shape"),
+    ((TOK, torch.zeros(3), 5), {}, ValueError, "grad shape must be tokens.shape"),
+    ((TOK, torch.zeros(3, 4), 5), {"out_dtype": torch.bfloat16}, TypeError, "out dtype must be"),
+    ((TOK, torch.zeros(3, 4, dtype=torch.float64), 5), {"out_dtype": torch.float32}, TypeError,
+     "out dtype must be"),
+    ((TOK, torch.zeros(3, 4, dtype=torch.half), 5), {"out": torch.zeros(5, 4).bfloat16()},
+     TypeError, "out dtype must be"),
+    ((TOK, torch.zeros(3, 4), 5), {}, ValueError, "grad must be a CUDA tensor"),
+])
+def test_embedding_grad_refuses(args, kwargs, error, message):
+    with pytest.raises(error, match=message):
+        fs.flagsparse_embedding_grad(*args, **kwargs)
+
+
+@pytest.mark.parametrize("args, error, message", [
+    ((TOK, 4), ValueError, "experts must be a 2D tensor"),
+    ((TOK[None].float(), 4), TypeError, "experts dtype must be"),
+    ((TOK[None], 4.0), TypeError, "n_experts must be an integer"),
+    ((TOK[None], -1), ValueError, "n_experts must be between 0 and 2047"),
+    ((TOK[None], 2048), ValueError, "n_experts must be between 0 and 2047"),
+    ((TOK[None], 4), ValueError, "experts must be a CUDA tensor"),
+])
+def test_route_refuses(args, error, message):
+    with pytest.raises(error, match=message):
+        fs.prepare_token_route(*args)
+
+
+def _route(n_tokens=3, k=2, n_experts=4):
+    """A route on the CPU: enough for the checks in front of a launch."""
+    return fs.TokenRoute(torch.zeros(n_tokens, k, dtype=torch.int32),
+                         torch.zeros(n_experts + 1, dtype=torch.int32),
+                         torch.zeros(n_tokens * k, dtype=torch.int32), n_experts, 0)
+
+
+def test_route_operators_refuse():
+    r, x, y = _route(), torch.zeros(3, 4), torch.zeros(6, 4)
+    with pytest.raises(TypeError, match="route must be a TokenRoute"):
+        fs.flagsparse_token_dispatch(x, (1, 2))
+    with pytest.raises(ValueError, match=r"x.shape\[0\] must be n_tokens=3"):
+        fs.flagsparse_token_dispatch(y, r)
+    with pytest.raises(ValueError, match="x must be a 2D tensor"):
+        fs.flagsparse_token_dispatch(x[None], r)
+    with pytest.raises(TypeError, match="x dtype must be one of"):
+        fs.flagsparse_token_dispatch(x.int(), r)
+    with pytest.raises(ValueError, match=r"y.shape\[0\] must be n_tokens \* k=6"):
+        fs.flagsparse_token_combine(x, r)
+    with pytest.raises(ValueError, match="weights shape must be"):
+        fs.flagsparse_token_combine(y, r, torch.zeros(2, 3))
+    with pytest.raises(TypeError, match="weights dtype must be the dtype of the rows"):
+        fs.flagsparse_token_combine(y, r, torch.zeros(3, 2).half())
+    with pytest.raises(ValueError, match=r"grad.shape\[0\] must be n_tokens \* k=6"):
+        fs.flagsparse_token_dispatch_grad(x, r)
+    with pytest.raises(ValueError, match="y is needed"):
+        fs.flagsparse_token_combine_grad(x, None, r, torch.zeros(3, 2))
+    with pytest.raises(TypeError, match="y dtype must match"):
+        fs.flagsparse_token_combine_grad(x, y.half(), r)
+    with pytest.raises(ValueError, match="same number of columns"):
+        fs.flagsparse_token_combine_grad(x, torch.zeros(6, 5), r)
+    with pytest.raises(ValueError, match="route must be a CUDA tensor"):
+        fs.flagsparse_token_dispatch(x, r)
+    with pytest.raises(RuntimeError, match="does not support automatic differentiation"):
+        fs.flagsparse_token_combine(y.requires_grad_(), r, out=torch.zeros(3, 4))
+
+
+def test_result_places():
+    """out that the kernels can write is written in place; another layout gets a stand-in."""
+    f32, cpu = torch.float32, torch.device("cpu")
+    with pytest.raises(ValueError, match="beta != 0 requires out="):
+        selection._Result(None, (3, 4), f32, cpu, 1.0)
+    for bad in (torch.zeros(4, 3), torch.zeros(3, 4).half()):
+        with pytest.raises(ValueError, match="out shape/dtype must match result"):
+            selection._Result(bad, (3, 4), f32, cpu, 0.0)
+    wide = torch.zeros(3, 9)
+    r = selection._Result(wide[:, :4], (3, 4), f32, cpu, 0.0)
+    assert not r.stand_in and r.flat.data_ptr() == wide.data_ptr() and r.flat.stride(0) == 9
+    cols = torch.arange(12.0).reshape(4, 3).t()
+    r = selection._Result(cols, (3, 4), f32, cpu, 1.0)
+    assert r.stand_in and torch.equal(r.flat, cols)      # beta reads what is there
+    r.flat.zero_()
+    assert r.done(cols) is cols and not cols.any()
+    deep = torch.zeros(2, 3, 9)[:, :, :4]                # rows of one pitch: a view will do
+    r = selection._Result(deep, (2, 3, 4), f32, cpu, 0.0)
+    assert not r.stand_in and r.flat.shape == (6, 4) and r.flat.stride(0) == 9
+    deep = torch.zeros(3, 2, 4).transpose(0, 1)
+    assert selection._Result(deep, (2, 3, 4), f32, cpu, 0.0).stand_in
+
+
+def test_c_entry_points_answer_before_any_launch():
+    lib, d = _lib.load(), ctypes.c_void_p(4096)          # never read: every call below is refused
+    odd = ctypes.c_void_p(4097)
+    ok, dtype, arg, align, ws, rng = 0, 1, 2, 3, 6, 7
+    rows = lambda v=0, i=0, idx=d, n=4, t=d, r=5, ld=8, dim=8, o=d, ldo=8: lib.b2s_select_rows(  # noqa: E731
+        v, i, idx, n, 0, 0, t, r, ld, dim, o, ldo, 1.0, 0.0, None, None)
+    assert rows(v=2) == dtype and rows(v=9) == dtype and rows(i=7) == dtype
+    assert rows(n=-1) == arg and rows(idx=None) == arg and rows(t=None) == arg
+    assert rows(o=None) == arg and rows(ld=7) == arg and rows(ldo=7) == arg
+    assert rows(n=2**31) == rng and rows(r=2**31) == rng and rows(dim=2**23) == rng
+    assert rows(idx=odd) == align and rows(t=odd) == align and rows(o=odd) == align
+    assert rows(n=0) == ok and rows(dim=0) == ok
+    grad = lambda v=5, o=5, n=4, r=5, b=1 << 30, w=d, ld=8: lib.b2s_select_grad(  # noqa: E731
+        v, o, 0, d, n, 0, 0, d, ld, r, 8, d, 8, 1.0, 0.0, w, b, None, None)
+    assert grad(v=3) == dtype and grad(v=0, o=5) == dtype and grad(v=1, o=0) == dtype
+    assert grad(o=4) == dtype and grad(n=-1) == arg and grad(ld=4) == arg
+    assert grad(b=16) == ws and grad(w=None) == ws and grad(w=odd) == align
+    assert grad(r=0) == ok
+    assert lib.b2s_select_grad_bytes(2, 4, 4, 4) == 0 and lib.b2s_select_grad_bytes(0, -1, 4, 4) == 0
+    plan = lambda i=1, e=d, t=4, k=2, n=8, b=1 << 30: lib.b2s_route_plan(  # noqa: E731
+        i, e, t, k, n, d, d, d, d, b, None, None)
+    assert plan(i=2) == dtype and plan(e=None) == arg and plan(n=-1) == arg
+    assert plan(n=2048) == rng and plan(t=2**31, k=2) == rng and plan(b=0) == ws
+    assert plan(e=ctypes.c_void_p(4100)) == align
+    disp = lambda v=0, x=d, s=d, h=d, t=4, ld=8: lib.b2s_route_dispatch(  # noqa: E731
+        v, x, ld, t, 2, 8, s, h, d, 8, None)
+    assert disp(v=3) == dtype and disp(x=None) == arg and disp(s=None) == arg
+    assert disp(h=None) == arg and disp(ld=1) == arg and disp(t=0) == ok
+    comb = lambda v=0, w=0, p=d, y=d: lib.b2s_route_combine(  # noqa: E731
+        v, y, 8, d, w, p, 4, 2, 8, d, 8, 1.0, 0.0, None)
+    assert comb(v=2) == dtype and comb(w=4) == dtype and comb(y=None) == arg
+    assert comb(p=ctypes.c_void_p(4098)) == align
+    back = lambda w=d, gw=d, y=d, wt=0: lib.b2s_route_combine_grad(  # noqa: E731
+        0, d, 8, y, 8, d, d, wt, w, 4, 2, 8, 1.0, d, 8, gw, None)
+    assert back(w=None) == arg and back(y=None) == arg and back(wt=5) == dtype
+
+
+# ---- the tiles of the gradient: every entry is summed once, by one owner ---------------------------
+P = 32
+
+
+def _tiles(keys, none):
+    """The decisions of one warp per tile of 32 sorted entries (b2s_select.cu, grad_tile), and of
+    the kernel that joins long runs, on a list of sorted keys (`none`: masked)."""
+    n, rows, head, tail, runs = len(keys), {}, {}, {}, []
+
+    def key(i):
+        return keys[i] if 0 <= i < n else (0xffffffff if i < 0 else none)
+
+    tiles = -(-n // P)
+    for t in range(tiles):
+        at = t * P
+        cur, nxt, prv = ([key(at + d + i) for i in range(P)] for d in (0, P, -P))
+        valid = sum(c < none for c in cur)
+        if not valid:
+            continue
+        before, last, after = prv[-1], cur[valid - 1], nxt[0]
+        in_head, in_prev = cur.count(before), prv.count(before)
+        in_tail, in_next = cur.count(last), nxt.count(last)
+        head_ends = in_head < P or after != before
+        head_began = in_prev < P or key(at - P - 1) != before
+        goes_on = valid == P and after == last
+        tail_begins = in_tail < P or before != last
+        tail_ends = in_next < P or key(at + 2 * P) != last
+        own_head = in_head > 0 and not (head_ends and head_began)
+        lo = in_head if in_head > 0 and not own_head else 0
+        long_tail = goes_on and tail_begins and not tail_ends
+        hi = valid + (in_next if goes_on and tail_begins and tail_ends else 0)
+        if lo < hi and long_tail:
+            runs.append(t)
+        acc = []
+        for i in range(lo, hi):
+            k = cur[i] if i < P else last
+            acc.append(at + i)
+            if i + 1 >= hi or (cur[i + 1] if i + 1 < P else last) != k:
+                part = head if own_head and i < in_head else tail if long_tail and i + 1 == hi else None
+                where = (rows, k) if part is None else (part, t)
+                assert where[1] not in where[0]
+                where[0][where[1]], acc = acc, []
+    for first in runs:
+        k, lo, hi = keys[first * P + P - 1], first + 1, tiles - 1
+        while lo < hi:
+            mid = (lo + hi + 1) // 2
+            lo, hi = (mid, hi) if keys[mid * P] <= k else (lo, mid - 1)
+        assert k not in rows
+        rows[k] = sum((tail.pop(t) if t == first else head.pop(t) for t in range(first, lo + 1)), [])
+    assert not head and not tail
+    return rows, len(runs)
+
+
+def test_gradient_tiles_cover_every_entry_once():
+    rng = random.Random(3)
+    long_runs = 0
+    for _ in range(3000):
+        none, n = rng.choice([1, 2, 5, 50]), rng.choice([1, 31, 32, 33, 64, 65, 97, 130, 300])
+        hot = rng.choice([0.1, 0.9])
+        keys = sorted(min(none, int(rng.expovariate(1.0))) if rng.random() < hot
+                      else rng.randrange(none + 1) for _ in range(n))
+        rows, runs = _tiles(keys, none)
+        long_runs += runs
+        want = {}
+        for i, k in enumerate(keys):
+            if k < none:
+                want.setdefault(k, []).append(i)
+        assert rows == want
+    assert long_runs > 100
