@@ -21,87 +21,194 @@ template <> struct raw_of<4> { using type = uint32_t; };
 template <> struct raw_of<8> { using type = unsigned long long; };
 template <> struct raw_of<16> { using type = uint4; };
 
-// The lane's eight columns of a 256-column slab of one row, as U vectors of VE elements: vector u
-// begins at column (u * 32 + lane) * VE of the slab.  VB = 16 when base, pitch and width allow
-// it, else one element per access (the accesses of a warp still cover one contiguous piece).
-template <class T, int VB> struct RowPart {
-  using Raw = typename raw_of<VB>::type;
-  static constexpr int VE = VB / static_cast<int>(sizeof(T));
-  static constexpr int U = 8 / VE;
-  Raw r[U];
+// A lane's E columns of a slab of 32 E columns of one row, as U groups of VE neighbouring elements:
+// group u begins at column (u * 32 + lane) * VE of the slab.  VE is 16 bytes of the value type
+// when bases, pitches and width allow it (a float row beside 16-bit values is then taken in two
+// pieces of 16 bytes), else one element; either way the accesses of a warp cover one contiguous
+// piece of the row.
+template <class O, int VE, int E = 8> struct Part {
+  static constexpr int U = E / VE;
+  static constexpr int OB = VE == 1 ? static_cast<int>(sizeof(O)) : 16;
+  static constexpr int OE = OB / static_cast<int>(sizeof(O));
+  static constexpr int N = VE / OE;
+  using Raw = typename raw_of<OB>::type;
+  Raw r[U * N];
 
   __device__ static int column(int col0, int u) {
     return col0 + (u * 32 + static_cast<int>(threadIdx.x & 31)) * VE;
   }
-  __device__ void clear() { memset(r, 0, sizeof(r)); }
-  __device__ void load(const T* row, int col0, int dim) {
+  __device__ void load(const O* row, int col0, int dim) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int c = column(col0, u);
-      if (c < dim)
-        r[u] = *reinterpret_cast<const Raw*>(row + c);
-      else
-        memset(&r[u], 0, sizeof(Raw));
+#pragma unroll
+      for (int p = 0; p < N; ++p)
+        if (c < dim) r[u * N + p] = *reinterpret_cast<const Raw*>(row + c + p * OE);
     }
   }
-  __device__ void store(T* row, int col0, int dim) const {
+  __device__ void store(O* row, int col0, int dim) const {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int c = column(col0, u);
-      if (c < dim) *reinterpret_cast<Raw*>(row + c) = r[u];
+#pragma unroll
+      for (int p = 0; p < N; ++p)
+        if (c < dim) *reinterpret_cast<Raw*>(row + c + p * OE) = r[u * N + p];
     }
   }
-  __device__ typename acc_of<T>::type get(int i) const {
-    T v;
-    memcpy(&v, reinterpret_cast<const char*>(r) + i * sizeof(T), sizeof(T));
+  __device__ typename acc_of<O>::type get(int i) const {
+    O v;
+    memcpy(&v, reinterpret_cast<const char*>(r) + i * sizeof(O), sizeof(O));
     return to_acc(v);
   }
-  __device__ void set(int i, typename acc_of<T>::type a) {
-    const T v = storage_of<T>::from_acc(a);
-    memcpy(reinterpret_cast<char*>(r) + i * sizeof(T), &v, sizeof(T));
+  // elements 2 i and 2 i + 1, for sums in pairs
+  __device__ float2 pair(int i) const {
+    if constexpr (VE > 1 && sizeof(O) == 2) {
+      uint32_t w;
+      memcpy(&w, reinterpret_cast<const char*>(r) + 4 * i, 4);
+      if constexpr (std::is_same_v<O, bf16>)
+        return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+      __half2 h;
+      memcpy(&h, &w, 4);
+      return __half22float2(h);
+    } else {
+      return make_float2(get(2 * i), get(2 * i + 1));
+    }
+  }
+  __device__ void set(int i, typename acc_of<O>::type a) {
+    const O v = storage_of<O>::from_acc(a);
+    memcpy(reinterpret_cast<char*>(r) + i * sizeof(O), &v, sizeof(O));
   }
 };
 
-// eight accumulators laid out like a RowPart<T, VB>, stored as O (T or float): alpha * acc, and
-// beta * (what is there) added when has_beta
+// E sums beside a Part: float32 ones are kept and added in pairs (one instruction for two)
+template <class A, int E> struct Sums {
+  A v[E];
+  __device__ void clear() {
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = A(0);
+  }
+  template <class P> __device__ void add(const P& p) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = v[e] + p.get(e);
+  }
+  template <class P> __device__ void fma(A w, const P& p) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) fma_acc(v[e], w, p.get(e));
+  }
+};
+template <int E> struct Sums<float, E> {
+  float2 v2[E / 2];
+  __device__ void clear() {
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) v2[e] = make_float2(0.f, 0.f);
+  }
+  template <class P> __device__ void add(const P& p) {
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) v2[e] = __fadd2_rn(v2[e], p.pair(e));
+  }
+  template <class P> __device__ void fma(float w, const P& p) {
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) v2[e] = __ffma2_rn(make_float2(w, w), p.pair(e), v2[e]);
+  }
+};
+template <class A, int E> __device__ inline A sum_of(const Sums<A, E>& s, int e) {
+  if constexpr (std::is_same_v<A, float>)
+    return e & 1 ? s.v2[e / 2].y : s.v2[e / 2].x;
+  else
+    return s.v[e];
+}
+
+// sums as they are, stored as O
+template <class O, int VE, class A, int E>
+__device__ inline void store_sums(O* row, int col0, int dim, const Sums<A, E>& s) {
+  Part<O, VE, E> v;
+#pragma unroll
+  for (int e = 0; e < E; ++e) v.set(e, sum_of(s, e));
+  v.store(row, col0, dim);
+}
+// alpha * sums (+ beta * old)
+template <class O, int VE, class A, int E>
+__device__ inline void store_axpby(O* row, int col0, int dim, const Sums<A, E>& s, A alpha,
+                                   bool has_beta, A beta, const Part<O, VE, E>& old) {
+  Part<O, VE, E> v;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    A x = alpha * sum_of(s, e);
+    if (has_beta) x = x + beta * old.get(e);
+    v.set(e, x);
+  }
+  v.store(row, col0, dim);
+}
+template <class O, int VE, class A, int E>
+__device__ inline void store_axpby(O* row, int col0, int dim, const Sums<A, E>& s, A alpha,
+                                   bool has_beta, A beta) {
+  Part<O, VE, E> old;
+  if (has_beta) old.load(row, col0, dim);
+  store_axpby<O, VE, A, E>(row, col0, dim, s, alpha, has_beta, beta, old);
+}
+// a row of zeros, or beta times what is there
 template <class O, int VE, class A>
-__device__ inline void store_acc(O* row, int col0, int dim, const A* acc, A alpha, bool has_beta,
-                                 A beta) {
-  constexpr int U = 8 / VE;
-  constexpr int OB = VE == 1 ? static_cast<int>(sizeof(O)) : 16;
-  constexpr int OE = OB / static_cast<int>(sizeof(O));
-  using Raw = typename raw_of<OB>::type;
+__device__ inline void scale_row(O* row, int dim, bool has_beta, A beta) {
+  Sums<A, 8> zero;
+  zero.clear();
+  for (int c = 0; c < dim; c += kSelCols)
+    store_axpby<O, VE, A, 8>(row, c, dim, zero, A(1), has_beta, beta);
+}
+
+// A warp's queue of row parts on their way from global to shared memory.  Every lane copies and
+// later reads its own 16-byte pieces, so that no barrier is needed, and the bytes in flight do
+// not cost registers.  Parts are asked for in batches: kStages batches of kBatch parts.
+template <class P, int kBatch, int kStages> struct PartQueue {
+  static constexpr int kPieces = P::U * P::N;
+  static constexpr int kWarpBytes = kBatch * kStages * static_cast<int>(sizeof(P)) * 32;
+  using Raw = typename P::Raw;
+  Raw* base;      // this lane's first piece in stage 0; pieces of a lane are 32 apart
+  int put, take;  // stages
+
+  __device__ explicit PartQueue(unsigned char* warp_smem)
+      : base(reinterpret_cast<Raw*>(warp_smem) + (threadIdx.x & 31)), put(0), take(0) {}
+  // asks for part q of the batch being put together; a dead part becomes zeros
+  template <class T> __device__ void push(int q, const T* row, bool live, int col0, int dim) {
+    Raw* at = base + (put * kBatch + q) * (kPieces * 32);
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int c = col0 + (u * 32 + static_cast<int>(threadIdx.x & 31)) * VE;
-    if (c < dim) {
+    for (int u = 0; u < P::U; ++u) {
+      const int c = P::column(col0, u);
 #pragma unroll
-      for (int p = 0; p < VE / OE; ++p) {
-        Raw* at = reinterpret_cast<Raw*>(row + c + p * OE);
-        Raw old;
-        if (has_beta) old = *at;
-        O v[OE];
-#pragma unroll
-        for (int e = 0; e < OE; ++e) {
-          A x = alpha * acc[u * VE + p * OE + e];
-          if (has_beta) {
-            O o;
-            memcpy(&o, reinterpret_cast<const char*>(&old) + e * sizeof(O), sizeof(O));
-            x = x + beta * static_cast<A>(to_acc(o));
-          }
-          v[e] = storage_of<O>::from_acc(x);
-        }
-        Raw neu;
-        memcpy(&neu, v, sizeof(Raw));
-        *at = neu;
-      }
+      for (int p = 0; p < P::N; ++p)
+        if (c < dim)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                           smem_addr(at + (u * P::N + p) * 32)),
+                       "l"(row + c + p * P::OE), "r"(live ? 16 : 0)
+                       : "memory");
     }
   }
-}
+  __device__ void send() {
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    put = put + 1 == kStages ? 0 : put + 1;
+  }
+  // waits for the oldest batch (kStages - 1 younger ones may still be under way)
+  __device__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory"); }
+  __device__ P part(int q) const {
+    const Raw* at = base + (take * kBatch + q) * (kPieces * 32);
+    P v;
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) v.r[i] = at[i * 32];
+    return v;
+  }
+  // nothing may be under way when the warp ends
+  __device__ void drain() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+  __device__ void done() { take = take + 1 == kStages ? 0 : take + 1; }
+};
+// Four CTAs of eight warps share an SM, with 48 KB of queues each: 6 KB a warp, in batches of two
+// parts of 1 KB (32 bytes a lane).
+constexpr int kQueueCtas = 4;
+constexpr int kQueueBatch = 2;
+constexpr int kQueueStages = 3;
+template <class T> constexpr int kQueueCols = 32 / static_cast<int>(sizeof(T));  // of a lane
 
 // ---- embedding lookup ------------------------------------------------------------------------
 // One warp per (token, group of G slabs).
-template <class T, class I, int VB, int G>
+template <class T, class I, int VE, int G>
 __global__ void __launch_bounds__(kSelThreads)
 select_rows_kernel(IdKeys<I> ids, int64_t n, const T* __restrict__ table, int64_t ld_table,
                    int dim, T* __restrict__ out, int64_t ld_out,
@@ -114,29 +221,20 @@ select_rows_kernel(IdKeys<I> ids, int64_t n, const T* __restrict__ table, int64_
   const uint32_t id = ids(i);
   const bool live = id < ids.n_keys;
   const int col0 = static_cast<int>(g) * (G * kSelCols);
-  RowPart<T, VB> r[G];
+  Part<T, VE> r[G];
+  if (live) {
 #pragma unroll
-  for (int s = 0; s < G; ++s) {
-    if (live)
+    for (int s = 0; s < G; ++s)
       r[s].load(table + static_cast<int64_t>(id) * ld_table, col0 + s * kSelCols, dim);
-    else
-      r[s].clear();
   }
   T* o = out + i * ld_out;
 #pragma unroll
   for (int s = 0; s < G; ++s) {
-    A acc[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = r[s].get(e);
-    if (!live && !has_beta) {
-      // alpha may be infinite: a masked row is zero, not alpha * 0
-#pragma unroll
-      for (int e = 0; e < 8; ++e) acc[e] = A(0);
-      store_acc<T, RowPart<T, VB>::VE, A>(o, col0 + s * kSelCols, dim, acc, A(1), false, A(0));
-    } else {
-      store_acc<T, RowPart<T, VB>::VE, A>(o, col0 + s * kSelCols, dim, acc, live ? alpha : A(1),
-                                          has_beta, beta);
-    }
+    Sums<A, 8> v;
+    v.clear();
+    if (live) v.add(r[s]);
+    // (a masked row is zero whatever alpha is)
+    store_axpby<T, VE, A, 8>(o, col0 + s * kSelCols, dim, v, live ? alpha : A(1), has_beta, beta);
   }
 }
 
@@ -160,8 +258,8 @@ __device__ inline uint32_t run_key(const GradRuns& g, int64_t i) {
   return (i >= 0 && i < g.n) ? g.keys[i] : (i < 0 ? 0xffffffffu : g.n_keys);
 }
 
-template <class T, class O, int VB>
-__device__ inline void grad_tile(const GradRuns& runs, int64_t tile, int64_t n_tiles, int slab,
+template <class T, class O, int VE>
+__device__ inline void grad_tile(const GradRuns& runs, int64_t tile, int slab,
                                  const T* __restrict__ grad, int64_t ld_grad, int dim,
                                  O* __restrict__ out, int64_t ld_out,
                                  typename acc_of<T>::type alpha, typename acc_of<T>::type beta,
@@ -169,7 +267,7 @@ __device__ inline void grad_tile(const GradRuns& runs, int64_t tile, int64_t n_t
                                  typename acc_of<T>::type* __restrict__ tail,
                                  int32_t* __restrict__ long_list, int32_t* long_count) {
   using A = typename acc_of<T>::type;
-  using RP = RowPart<T, VB>;
+  using RP = Part<T, VE>;
   constexpr int P = kGradTile;
   const int lane = threadIdx.x & 31;
   const int64_t at = tile * P;
@@ -204,50 +302,57 @@ __device__ inline void grad_tile(const GradRuns& runs, int64_t tile, int64_t n_t
   const int pos_nxt = at + P + lane < runs.n ? runs.vals[at + P + lane] : 0;
   const int col0 = slab * kSelCols;
 
-  A acc[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) acc[e] = A(0);
-  constexpr int kAhead = 8;
+  Sums<A, 8> acc;
+  acc.clear();
+  // The rows of a group, and the rows of `out` that its ends are added to, are all asked for
+  // before the first is used: a run of one token (most are) would otherwise wait for its old
+  // row by itself.
+  constexpr int kAhead = 4;
   for (int i0 = lo; i0 < hi; i0 += kAhead) {
     RP r[kAhead];
+    Part<O, VE> old[kAhead];
+    uint32_t key[kAhead];
+    bool ends[kAhead];
 #pragma unroll
     for (int q = 0; q < kAhead; ++q) {
       const int i = i0 + q;
       const int a = __shfl_sync(0xffffffffu, pos_cur, i & 31);
       const int b = __shfl_sync(0xffffffffu, pos_nxt, i & 31);
+      const uint32_t ka = __shfl_sync(0xffffffffu, cur, i & 31);
+      const uint32_t kb = __shfl_sync(0xffffffffu, cur, (i + 1) & 31);
+      key[q] = i < P ? ka : last;
+      ends[q] = i < hi && (i + 1 >= hi || (i + 1 < P ? kb : last) != key[q]);
       if (i < hi) r[q].load(grad + static_cast<int64_t>(i < P ? a : b) * ld_grad, col0, dim);
+      const bool part = (own_head && i < in_head) || (long_tail && i + 1 == hi);
+      if (has_beta && ends[q] && !part)
+        old[q].load(out + static_cast<int64_t>(key[q]) * ld_out, col0, dim);
     }
 #pragma unroll
     for (int q = 0; q < kAhead; ++q) {
       const int i = i0 + q;
-      const uint32_t ka = __shfl_sync(0xffffffffu, cur, i & 31);
-      const uint32_t kc = i < P ? ka : last;
-      const uint32_t kb = __shfl_sync(0xffffffffu, cur, (i + 1) & 31);
-      const bool ends = i + 1 >= hi || (i + 1 < P ? kb : last) != kc;
       if (i < hi) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] = acc[e] + r[q].get(e);
-        if (ends) {
+        acc.add(r[q]);
+        if (ends[q]) {
           const bool is_head = own_head && i < in_head;
-          const bool is_tail = long_tail && i + 1 == hi;
-          if (is_head || is_tail) {
+          if (is_head || (long_tail && i + 1 == hi)) {
             A* part = (is_head ? head : tail) + tile * dim;
-            store_acc<A, RP::VE, A>(part, col0, dim, acc, A(1), false, A(0));
+            store_sums<A, VE>(part, col0, dim, acc);
           } else {
-            store_acc<O, RP::VE, A>(out + static_cast<int64_t>(kc) * ld_out, col0, dim, acc,
-                                    alpha, has_beta, beta);
+            store_axpby<O, VE, A, 8>(out + static_cast<int64_t>(key[q]) * ld_out, col0, dim, acc,
+                                     alpha, has_beta, beta, old[q]);
           }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) acc[e] = A(0);
+          acc.clear();
         }
       }
     }
   }
 }
 
-// The first sum_blocks CTAs sum tiles; the others write the rows no token names: zero, or
-// beta times what is there (none are launched when beta = 1 leaves those rows as they are).
-template <class T, class O, int VB>
+// CTAs that sum tiles and CTAs that write the rows no token names (zero, or beta times what is
+// there; none when beta = 1 leaves them as they are) alternate from the first on, until one kind
+// is used up: the waits of the first overlap the writes of the second, and no long CTA starts
+// late.
+template <class T, class O, int VE>
 __global__ void __launch_bounds__(kSelThreads)
 select_grad_kernel(GradRuns runs, int64_t n_tiles, unsigned sum_blocks, unsigned slabs,
                    const T* __restrict__ grad, int64_t ld_grad, int dim, O* __restrict__ out,
@@ -255,30 +360,27 @@ select_grad_kernel(GradRuns runs, int64_t n_tiles, unsigned sum_blocks, unsigned
                    bool has_beta, typename acc_of<T>::type* __restrict__ head,
                    typename acc_of<T>::type* __restrict__ tail, int32_t* __restrict__ long_list,
                    int32_t* long_count, const uint8_t* __restrict__ named) {
-  using A = typename acc_of<T>::type;
   const int warp = threadIdx.x >> 5;
-  if (blockIdx.x < sum_blocks) {
-    const unsigned tb = blockIdx.x / slabs, slab = blockIdx.x - tb * slabs;
+  const unsigned b = blockIdx.x, rest = gridDim.x - sum_blocks;
+  const unsigned both = 2 * (sum_blocks < rest ? sum_blocks : rest);
+  const bool sums = b < both ? (b & 1) == 0 : sum_blocks > rest;
+  const unsigned at = b < both ? b / 2 : b - both / 2;  // among the CTAs of its kind
+  if (sums) {
+    const unsigned tb = at / slabs, slab = at - tb * slabs;
     const int64_t tile = static_cast<int64_t>(tb) * kSelWarps + warp;
     if (tile < n_tiles)
-      grad_tile<T, O, VB>(runs, tile, n_tiles, static_cast<int>(slab), grad, ld_grad, dim, out,
-                          ld_out, alpha, beta, has_beta, head, tail, long_list, long_count);
+      grad_tile<T, O, VE>(runs, tile, static_cast<int>(slab), grad, ld_grad, dim, out, ld_out,
+                          alpha, beta, has_beta, head, tail, long_list, long_count);
     return;
   }
-  const int64_t row = static_cast<int64_t>(blockIdx.x - sum_blocks) * kSelWarps + warp;
-  if (row >= runs.n_keys || named[row]) return;
-  O* o = out + row * ld_out;
-  A acc[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) acc[e] = A(0);
-  for (int c = 0; c < dim; c += kSelCols)
-    store_acc<O, RowPart<T, VB>::VE, A>(o, c, dim, acc, A(1), has_beta, beta);
+  const int64_t row = static_cast<int64_t>(at) * kSelWarps + warp;
+  if (row < runs.n_keys && !named[row]) scale_row<O, VE>(out + row * ld_out, dim, has_beta, beta);
 }
 
 // A run that spans two tile borders or more: the piece of its first tile, then the pieces of the
 // tiles behind it.  One CTA per (run, 128 columns): its warps take the pieces in turn and the
 // warps' sums are added in warp order.
-constexpr int kLongWarps = 16;
+constexpr int kLongWarps = 8;
 constexpr int kLongCols = 128;
 
 template <class A, class O>
@@ -295,13 +397,19 @@ select_grad_long_kernel(GradRuns runs, int64_t n_tiles, int dim, O* __restrict__
   for (int item = blockIdx.x; item < count; item += gridDim.x) {
     const int64_t first = long_list[item];
     const uint32_t key = runs.keys[first * kGradTile + kGradTile - 1];
-    // the last tile whose first entry has this key
-    int64_t lo = first + 1, hi = n_tiles - 1;
-    while (lo < hi) {
-      const int64_t mid = (lo + hi + 1) >> 1;
-      if (runs.keys[mid * kGradTile] <= key) lo = mid; else hi = mid - 1;
+    // the last tile whose first entry has this key, 32 places at a time
+    int64_t lo = first + 1, len = n_tiles - lo;
+    while (len > 1) {
+      const int64_t step = (len + 31) / 32;
+      const int64_t at = lo + lane * step;
+      const bool mine = at < lo + len && runs.keys[at * kGradTile] <= key;
+      const int hits = __popc(__ballot_sync(0xffffffffu, mine));  // lane 0 always hits
+      const int64_t end = lo + len;
+      lo += (hits - 1) * step;
+      len = end - lo < step ? end - lo : step;
     }
     A acc[4] = {A(0), A(0), A(0), A(0)};
+#pragma unroll 4
     for (int64_t t = first + warp; t <= lo; t += kLongWarps) {
       const A* part = (t == first ? tail : head) + t * dim;
 #pragma unroll
@@ -311,11 +419,11 @@ select_grad_long_kernel(GradRuns runs, int64_t n_tiles, int dim, O* __restrict__
 #pragma unroll
     for (int e = 0; e < 4; ++e) sums[warp][lane + 32 * e] = acc[e];
     __syncthreads();
-    if (warp < 4) {
-      const int c = warp * 32 + lane;
+    if (threadIdx.x < kLongCols) {
       A s = A(0);
-      for (int w = 0; w < kLongWarps; ++w) s = s + sums[w][c];
-      const int64_t col = static_cast<int64_t>(blockIdx.y) * kLongCols + c;
+#pragma unroll
+      for (int w = 0; w < kLongWarps; ++w) s = s + sums[w][threadIdx.x];
+      const int col = static_cast<int>(blockIdx.y) * kLongCols + threadIdx.x;
       if (col < dim) {
         O* o = out + static_cast<int64_t>(key) * ld_out + col;
         A x = alpha * s;
@@ -333,17 +441,17 @@ __device__ inline bool is_row(int32_t s, int64_t rows) {
   return static_cast<uint32_t>(s) < static_cast<uint64_t>(rows);
 }
 
-// Rows are only moved: units of VB bytes, whatever the value type.  One warp per (token, slab);
+// Rows are only moved: units of UB bytes, whatever the value type.  One warp per (token, slab);
 // the token's row is read once and written to its slots.  The rows behind the last expert's are
 // zeroed by the same warps.
-template <int VB>
+template <int UB>
 __global__ void __launch_bounds__(kSelThreads)
 route_dispatch_kernel(const unsigned char* __restrict__ x, int64_t ld_x, int64_t n, int k,
                       int units, const int32_t* __restrict__ slots,
                       const int32_t* __restrict__ held_at, unsigned char* __restrict__ rows,
                       int64_t ld_rows, unsigned slabs) {
-  using Raw = typename raw_of<VB>::type;
-  constexpr int U = VB == 16 ? 4 : 8;
+  using Raw = typename raw_of<UB>::type;
+  constexpr int U = UB == 16 ? 4 : 8;
   const unsigned tb = blockIdx.x / slabs, slab = blockIdx.x - tb * slabs;
   const int64_t t = static_cast<int64_t>(tb) * kSelWarps + (threadIdx.x >> 5);
   if (t >= n) return;
@@ -352,21 +460,21 @@ route_dispatch_kernel(const unsigned char* __restrict__ x, int64_t ld_x, int64_t
 #pragma unroll
   for (int u = 0; u < U; ++u)
     if (u0 + 32 * u < units)
-      r[u] = *reinterpret_cast<const Raw*>(x + t * ld_x + static_cast<int64_t>(u0 + 32 * u) * VB);
+      r[u] = *reinterpret_cast<const Raw*>(x + t * ld_x + static_cast<int64_t>(u0 + 32 * u) * UB);
   for (int j = 0; j < k; ++j) {
     const int32_t s = slots[t * k + j];
     if (!is_row(s, n * k)) continue;
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (u0 + 32 * u < units)
-        *reinterpret_cast<Raw*>(rows + s * ld_rows + static_cast<int64_t>(u0 + 32 * u) * VB) = r[u];
+        *reinterpret_cast<Raw*>(rows + s * ld_rows + static_cast<int64_t>(u0 + 32 * u) * UB) = r[u];
   }
   memset(r, 0, sizeof(r));
   for (int64_t z = *held_at + t; z < n * k; z += n) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (u0 + 32 * u < units)
-        *reinterpret_cast<Raw*>(rows + z * ld_rows + static_cast<int64_t>(u0 + 32 * u) * VB) = r[u];
+        *reinterpret_cast<Raw*>(rows + z * ld_rows + static_cast<int64_t>(u0 + 32 * u) * UB) = r[u];
   }
 }
 
@@ -379,48 +487,136 @@ __device__ inline typename acc_of<T>::type route_weight(const void* w, bool w_is
   return to_acc(static_cast<const T*>(w)[a]);
 }
 
-// out[t] = alpha * sum_j w[t, j] * y[slots[t, j]] + beta * out[t]: one warp per (token, slab)
-template <class T, int VB>
-__global__ void __launch_bounds__(kSelThreads)
+// out[t] = alpha * sum_j w[t, j] * y[slots[t, j]] + beta * out[t].  A warp takes a range of tokens
+// and one slab of columns; the assignments of its tokens are one stretch of `slots`, read 32 at a
+// time and a stretch ahead, and their rows stream through the warp's queue without a pause
+// between tokens.  A masked assignment is a part of zeros with weight zero.
+template <class T, int VE>
+__global__ void __launch_bounds__(kSelThreads, kQueueCtas)
 route_combine_kernel(const T* __restrict__ y, int64_t ld_y, const int32_t* __restrict__ slots,
                      const void* __restrict__ weights, bool w_is_f32, int64_t n, int k, int dim,
                      T* __restrict__ out, int64_t ld_out, typename acc_of<T>::type alpha,
-                     typename acc_of<T>::type beta, bool has_beta, unsigned slabs) {
+                     typename acc_of<T>::type beta, bool has_beta, unsigned slabs,
+                     unsigned ranges) {
   using A = typename acc_of<T>::type;
-  using RP = RowPart<T, VB>;
+  constexpr int E = kQueueCols<T>, B = kQueueBatch;
+  using Queue = PartQueue<Part<T, VE, E>, B, kQueueStages>;
+  extern __shared__ int4 smem4[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const unsigned w = blockIdx.x * kSelWarps + warp;
+  const unsigned range = w / slabs, slab = w - range * slabs;
+  if (range >= ranges) return;
+  Queue queue(reinterpret_cast<unsigned char*>(smem4) + warp * Queue::kWarpBytes);
+  const int col0 = static_cast<int>(slab) * (32 * E);
+  int64_t t = n * range / ranges;
+  const int64_t t1 = n * (range + 1) / ranges;
+  const int32_t* my_slots = slots + t * k;
+  const int64_t w0 = t * k;
+  const int count = static_cast<int>((t1 - t) * k);  // the warp's assignments: 0 .. count - 1
+  const uint32_t rows = static_cast<uint32_t>(n * k);
+
+  // stretches of 32 assignments: the one that rows are asked for from, the one behind it; the
+  // weights of the one that is summed from, and of the one behind it
+  auto slot_of = [&](int a) {  // a valid slot, or -1
+    const int32_t s = a < count ? my_slots[a] : -1;
+    return static_cast<uint32_t>(s) < rows ? s : -1;
+  };
+  auto weight_of = [&](int a) {
+    return slot_of(a) >= 0 ? route_weight<T>(weights, w_is_f32, w0 + a) : A(0);
+  };
+  int32_t ask_slot = slot_of(lane), next_slot = slot_of(32 + lane);
+  A weight = weight_of(lane), next_weight = weight_of(32 + lane);
+  int ask = 0;
+  auto send = [&] {
+#pragma unroll
+    for (int q = 0; q < B; ++q) {
+      const int32_t s = __shfl_sync(0xffffffffu, ask_slot, (ask + q) & 31);
+      queue.push(q, y + static_cast<int64_t>(s < 0 ? 0 : s) * ld_y, s >= 0, col0, dim);
+    }
+    queue.send();
+    ask += B;
+    if ((ask & 31) == 0) {
+      ask_slot = next_slot;
+      next_slot = slot_of(ask + 32 + lane);
+    }
+  };
+  for (int q = 0; q < kQueueStages - 1; ++q) send();
+  Sums<A, E> acc;
+  acc.clear();
+  int j = 0;
+  for (int a = 0; a < count; a += B) {
+    send();
+    if ((a & 31) == 0 && a > 0) {
+      weight = next_weight;
+      next_weight = weight_of(a + 32 + lane);
+    }
+    queue.wait();
+#pragma unroll
+    for (int q = 0; q < B; ++q) {
+      acc.fma(__shfl_sync(0xffffffffu, weight, (a + q) & 31), queue.part(q));
+      if (++j == k) {
+        if (a + q < count)
+          store_axpby<T, VE, A, E>(out + t * ld_out, col0, dim, acc, alpha, has_beta, beta);
+        acc.clear();
+        j = 0;
+        ++t;
+      }
+    }
+    queue.done();
+  }
+  queue.drain();
+}
+
+// The same for rows that cannot be taken 16 bytes at a time: one warp per (token, slab), up to 32
+// slots and weights read at once, four rows in flight in registers.
+template <class T>
+__global__ void __launch_bounds__(kSelThreads)
+route_combine_plain_kernel(const T* __restrict__ y, int64_t ld_y,
+                           const int32_t* __restrict__ slots, const void* __restrict__ weights,
+                           bool w_is_f32, int64_t n, int k, int dim, T* __restrict__ out,
+                           int64_t ld_out, typename acc_of<T>::type alpha,
+                           typename acc_of<T>::type beta, bool has_beta, unsigned slabs) {
+  using A = typename acc_of<T>::type;
+  constexpr int kAhead = 4;
   const unsigned tb = blockIdx.x / slabs, slab = blockIdx.x - tb * slabs;
   const int64_t t = static_cast<int64_t>(tb) * kSelWarps + (threadIdx.x >> 5);
   if (t >= n) return;
+  const int lane = threadIdx.x & 31;
   const int col0 = static_cast<int>(slab) * kSelCols;
-  A acc[8];
+  Sums<A, 8> acc;
+  acc.clear();
+  for (int c = 0; c < k; c += 32) {
+    int32_t my_slot = -1;
+    A my_weight = A(0);
+    if (c + lane < k) {
+      my_slot = slots[t * k + c + lane];
+      my_weight = route_weight<T>(weights, w_is_f32, t * k + c + lane);
+    }
+    const int m = k - c < 32 ? k - c : 32;
+    for (int j0 = 0; j0 < m; j0 += kAhead) {
+      Part<T, 1> r[kAhead];
+      int32_t s[kAhead];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) acc[e] = A(0);
-  constexpr int kAhead = 4;
-  for (int j0 = 0; j0 < k; j0 += kAhead) {
-    RP r[kAhead];
-    int32_t s[kAhead];
+      for (int q = 0; q < kAhead; ++q) {
+        s[q] = __shfl_sync(0xffffffffu, my_slot, (j0 + q) & 31);
+        if (j0 + q >= m) s[q] = -1;
+        if (is_row(s[q], n * k)) r[q].load(y + static_cast<int64_t>(s[q]) * ld_y, col0, dim);
+      }
 #pragma unroll
-    for (int q = 0; q < kAhead; ++q) s[q] = j0 + q < k ? slots[t * k + j0 + q] : -1;
-#pragma unroll
-    for (int q = 0; q < kAhead; ++q)
-      if (is_row(s[q], n * k)) r[q].load(y + static_cast<int64_t>(s[q]) * ld_y, col0, dim);
-#pragma unroll
-    for (int q = 0; q < kAhead; ++q) {
-      if (is_row(s[q], n * k)) {
-        const A w = route_weight<T>(weights, w_is_f32, t * k + j0 + q);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) fma_acc(acc[e], w, r[q].get(e));
+      for (int q = 0; q < kAhead; ++q) {
+        const A w = __shfl_sync(0xffffffffu, my_weight, (j0 + q) & 31);
+        if (is_row(s[q], n * k)) acc.fma(w, r[q]);
       }
     }
   }
-  store_acc<T, RP::VE, A>(out + t * ld_out, col0, dim, acc, alpha, has_beta, beta);
+  store_axpby<T, 1, A, 8>(out + t * ld_out, col0, dim, acc, alpha, has_beta, beta);
 }
 
 // grad_y[slots[a]] = alpha * w[a] * g[a / k], grad_w[a] = alpha * <g[a / k], y[slots[a]]>: one
 // warp per assignment a, over the whole row (the dot product ends in the warp); the warps of one
 // token share its row of g through the caches.  Rows behind the last expert's are zeroed.
-template <class T, int VB>
-__global__ void __launch_bounds__(kSelThreads)
+template <class T, int VE>
+__global__ void __launch_bounds__(kSelThreads, sizeof(T) < 8 ? 8 : 4)
 route_combine_grad_kernel(const T* __restrict__ g, int64_t ld_g, const T* __restrict__ y,
                           int64_t ld_y, const int32_t* __restrict__ slots,
                           const int32_t* __restrict__ held_at,
@@ -428,7 +624,6 @@ route_combine_grad_kernel(const T* __restrict__ g, int64_t ld_g, const T* __rest
                           int dim, typename acc_of<T>::type alpha, T* __restrict__ grad_y,
                           int64_t ld_gy, void* __restrict__ grad_w) {
   using A = typename acc_of<T>::type;
-  using RP = RowPart<T, VB>;
   const int64_t a = blockIdx.x * static_cast<int64_t>(kSelWarps) + (threadIdx.x >> 5);
   if (a >= n * k) return;
   const int lane = threadIdx.x & 31;
@@ -440,16 +635,20 @@ route_combine_grad_kernel(const T* __restrict__ g, int64_t ld_g, const T* __rest
     T* o = grad_y + static_cast<int64_t>(s) * ld_gy;
     const A w = alpha * route_weight<T>(weights, w_is_f32, a);
     for (int c = 0; c < dim; c += kSelCols) {
-      RP rg, ry;
+      Part<T, VE> rg, ry;
       rg.load(gr, c, dim);
       if (grad_w) ry.load(yr, c, dim);
-      A acc[8];
+      if (grad_w) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        acc[e] = rg.get(e);
-        if (grad_w) fma_acc(dot, acc[e], ry.get(e));
+        for (int u = 0; u < 8 / VE; ++u)
+          if (Part<T, VE>::column(c, u) < dim) {
+#pragma unroll
+            for (int e = u * VE; e < u * VE + VE; ++e) fma_acc(dot, rg.get(e), ry.get(e));
+          }
       }
-      store_acc<T, RP::VE, A>(o, c, dim, acc, w, false, A(0));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ry.set(e, w * rg.get(e));
+      ry.store(o, c, dim);
     }
   }
   if (grad_w) {
@@ -462,13 +661,7 @@ route_combine_grad_kernel(const T* __restrict__ g, int64_t ld_g, const T* __rest
     }
   }
   const int64_t z = *held_at + a;
-  if (z < n * k) {
-    A acc[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = A(0);
-    for (int c = 0; c < dim; c += kSelCols)
-      store_acc<T, RP::VE, A>(grad_y + z * ld_gy, c, dim, acc, A(1), false, A(0));
-  }
+  if (z < n * k) scale_row<T, VE, A>(grad_y + z * ld_gy, dim, false, A(0));
 }
 
 // ---- host ----------------------------------------------------------------------------------------
@@ -536,14 +729,14 @@ int select_rows_run(const IdKeys<I>& ids, int64_t n, const void* table, int64_t 
   const T* tp = static_cast<const T*>(table);
   T* op = static_cast<T*>(out);
   const A a = static_cast<A>(alpha), b = static_cast<A>(beta);
-#define B2S_GO(VB, GG)                                                                          \
-  select_rows_kernel<T, I, VB, GG><<<static_cast<unsigned>(blocks), kSelThreads, 0, s>>>(       \
+#define B2S_GO(VE, GG)                                                                          \
+  select_rows_kernel<T, I, VE, GG><<<static_cast<unsigned>(blocks), kSelThreads, 0, s>>>(       \
       ids, n, tp, ld_table, static_cast<int>(dim), op, ld_out, a, b, b != A(0),                 \
       static_cast<unsigned>(groups))
   if (wide) {
-    if (G == 1) B2S_GO(16, 1); else B2S_GO(16, 4);
+    if (G == 1) B2S_GO(16 / sizeof(T), 1); else B2S_GO(16 / sizeof(T), 4);
   } else {
-    if (G == 1) B2S_GO(sizeof(T), 1); else B2S_GO(sizeof(T), 4);
+    if (G == 1) B2S_GO(1, 1); else B2S_GO(1, 4);
   }
 #undef B2S_GO
   return launch_status();
@@ -566,12 +759,12 @@ int select_grad_run(const GradRuns& runs, const void* grad, int64_t ld_grad, int
   A* tail = reinterpret_cast<A*>(ws + l.tail);
   int32_t* list = reinterpret_cast<int32_t*>(ws + l.list);
   const unsigned grid = static_cast<unsigned>(sums + rest);
-#define B2S_GO(VB)                                                                             \
-  select_grad_kernel<T, O, VB><<<grid, kSelThreads, 0, s>>>(                                   \
+#define B2S_GO(VE)                                                                             \
+  select_grad_kernel<T, O, VE><<<grid, kSelThreads, 0, s>>>(                                   \
       runs, tiles, static_cast<unsigned>(sums), static_cast<unsigned>(slabs),                  \
       static_cast<const T*>(grad), ld_grad, static_cast<int>(dim), static_cast<O*>(out), ld_out, \
       a, b, b != A(0), head, tail, list + 1, list, ws + l.named)
-  if (wide) B2S_GO(16); else B2S_GO(sizeof(T));
+  if (wide) B2S_GO(16 / sizeof(T)); else B2S_GO(1);
 #undef B2S_GO
   if (tiles > 2) {  // a long run touches three tiles at least
     const dim3 lg(static_cast<unsigned>(tiles < 256 ? tiles : 256),
@@ -707,24 +900,51 @@ inline int check_weights(int val_type, int w_type, const void* weights, bool* is
   *is_f32 = w_type == B2S_F32;
   return B2S_OK;
 }
+template <class T, int VE>
+int route_combine_go(const T* y, int64_t ld_y, const int32_t* slots, const void* weights,
+                     bool w_f32, int64_t n, int64_t k, int64_t dim, T* out, int64_t ld_out,
+                     double alpha, double beta, cudaStream_t s) {
+  using A = typename acc_of<T>::type;
+  auto kernel = &route_combine_kernel<T, VE>;
+  constexpr int E = kQueueCols<T>;
+  constexpr size_t smem =
+      kSelWarps * PartQueue<Part<T, VE, E>, kQueueBatch, kQueueStages>::kWarpBytes;
+  ensure_dyn_smem(reinterpret_cast<const void*>(kernel), smem);
+  const int64_t slabs = ceil_div(dim, 32 * E);
+  // every warp that fits the GPU at once gets one range
+  constexpr int64_t kResident = 148 * kQueueCtas * kSelWarps;
+  int64_t ranges = kResident / slabs;
+  ranges = ranges < 1 ? 1 : ranges > n ? n : ranges;
+  // a warp counts its assignments in 32 bits (with two stretches to spare)
+  while (ceil_div(n, ranges) * k > 0x7fff0000) ++ranges;
+  const int64_t blocks = ceil_div(ranges * slabs, kSelWarps);
+  const A b = static_cast<A>(beta);
+  kernel<<<static_cast<unsigned>(blocks), kSelThreads, smem, s>>>(
+      y, ld_y, slots, weights, w_f32, n, static_cast<int>(k), static_cast<int>(dim), out, ld_out,
+      static_cast<A>(alpha), b, b != A(0), static_cast<unsigned>(slabs),
+      static_cast<unsigned>(ranges));
+  return launch_status();
+}
+
 template <class T>
 int route_combine_run(const void* y, int64_t ld_y, const int32_t* slots, const void* weights,
                       bool w_f32, int64_t n, int64_t k, int64_t dim, void* out, int64_t ld_out,
                       double alpha, double beta, cudaStream_t s) {
+  const bool wide = k > 0 && wide_rows(y, ld_y, dim, sizeof(T)) &&
+                    wide_rows(out, ld_out, dim, sizeof(T));
+  const T* yp = static_cast<const T*>(y);
+  T* op = static_cast<T*>(out);
+  if (wide)
+    return route_combine_go<T, 16 / sizeof(T)>(
+        yp, ld_y, slots, weights, w_f32, n, k, dim, op, ld_out, alpha, beta, s);
   using A = typename acc_of<T>::type;
   const int64_t slabs = ceil_div(dim, kSelCols), blocks = ceil_div(n, kSelWarps) * slabs;
   if (blocks > kMaxGrid) return B2S_ERR_RANGE;
-  const bool wide = (k == 0 || wide_rows(y, ld_y, dim, sizeof(T))) &&
-                    wide_rows(out, ld_out, dim, sizeof(T));
   const A b = static_cast<A>(beta);
-  auto go = [&](auto kernel) {
-    kernel<<<static_cast<unsigned>(blocks), kSelThreads, 0, s>>>(
-        static_cast<const T*>(y), ld_y, slots, weights, w_f32, n, static_cast<int>(k),
-        static_cast<int>(dim), static_cast<T*>(out), ld_out, static_cast<A>(alpha), b, b != A(0),
-        static_cast<unsigned>(slabs));
-    return launch_status();
-  };
-  return wide ? go(&route_combine_kernel<T, 16>) : go(&route_combine_kernel<T, sizeof(T)>);
+  route_combine_plain_kernel<T><<<static_cast<unsigned>(blocks), kSelThreads, 0, s>>>(
+      yp, ld_y, slots, weights, w_f32, n, static_cast<int>(k), static_cast<int>(dim), op, ld_out,
+      static_cast<A>(alpha), b, b != A(0), static_cast<unsigned>(slabs));
+  return launch_status();
 }
 
 template <class T>
@@ -745,8 +965,8 @@ int route_combine_grad_run(const void* g, int64_t ld_g, const void* y, int64_t l
         static_cast<T*>(grad_y), ld_gy, grad_w);
     return launch_status();
   };
-  return wide ? go(&route_combine_grad_kernel<T, 16>)
-              : go(&route_combine_grad_kernel<T, sizeof(T)>);
+  return wide ? go(&route_combine_grad_kernel<T, 16 / sizeof(T)>)
+              : go(&route_combine_grad_kernel<T, 1>);
 }
 }  // namespace b2s
 
