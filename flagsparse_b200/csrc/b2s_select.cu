@@ -3,6 +3,8 @@
 // (dW = alpha S^T G + beta dW), and the routing of tokens to experts and back (S has k entries a
 // row).  All of them move rows of `dim` values; a warp owns 256 columns of a row at a time, eight
 // per lane, so that every load and store of a warp is one contiguous piece of a row.
+#include <algorithm>
+
 #include "b2s_sort.cuh"
 
 namespace b2s {
@@ -16,6 +18,7 @@ template <class T> struct acc_of { using type = float; };
 template <> struct acc_of<double> { using type = double; };
 
 template <int VB> struct raw_of;
+template <> struct raw_of<1> { using type = uint8_t; };
 template <> struct raw_of<2> { using type = uint16_t; };
 template <> struct raw_of<4> { using type = uint32_t; };
 template <> struct raw_of<8> { using type = unsigned long long; };
@@ -146,18 +149,34 @@ __device__ inline void store_axpby(O* row, int col0, int dim, const Sums<A, E>& 
   if (has_beta) old.load(row, col0, dim);
   store_axpby<O, VE, A, E>(row, col0, dim, s, alpha, has_beta, beta, old);
 }
-// a row of zeros, or beta times what is there
+// a row of zeros: 16 bytes at a time between the first and the last 16-byte border in it
+template <class O> __device__ inline void zero_row(O* row, int dim) {
+  constexpr int V = 16 / static_cast<int>(sizeof(O));
+  const int lane = threadIdx.x & 31;
+  O zero;
+  memset(&zero, 0, sizeof(O));
+  int head = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) /
+             static_cast<int>(sizeof(O));
+  head = head < dim ? head : dim;
+  if (lane < head) row[lane] = zero;
+  uint4* body = reinterpret_cast<uint4*>(row + head);
+  const int full = (dim - head) / V;
+  for (int i = lane; i < full; i += 32) body[i] = make_uint4(0, 0, 0, 0);
+  const int tail = head + full * V + lane;
+  if (tail < dim) row[tail] = zero;
+}
+// beta times what is there
 template <class O, int VE, class A>
-__device__ inline void scale_row(O* row, int dim, bool has_beta, A beta) {
+__device__ inline void scale_row(O* row, int dim, A beta) {
   Sums<A, 8> zero;
   zero.clear();
   for (int c = 0; c < dim; c += kSelCols)
-    store_axpby<O, VE, A, 8>(row, c, dim, zero, A(1), has_beta, beta);
+    store_axpby<O, VE, A, 8>(row, c, dim, zero, A(1), true, beta);
 }
 
 // A warp's queue of row parts on their way from global to shared memory.  Every lane copies and
-// later reads its own 16-byte pieces, so that no barrier is needed, and the bytes in flight do
-// not cost registers.  Parts are asked for in batches: kStages batches of kBatch parts.
+// later reads its own pieces (of 16 bytes, or single elements of 4 or 8), so that no barrier is
+// needed, and the bytes in flight do not cost registers.  Parts are asked for in batches: kStages batches of kBatch parts.
 template <class P, int kBatch, int kStages> struct PartQueue {
   static constexpr int kPieces = P::U * P::N;
   static constexpr int kWarpBytes = kBatch * kStages * static_cast<int>(sizeof(P)) * 32;
@@ -167,6 +186,17 @@ template <class P, int kBatch, int kStages> struct PartQueue {
 
   __device__ explicit PartQueue(unsigned char* warp_smem)
       : base(reinterpret_cast<Raw*>(warp_smem) + (threadIdx.x & 31)), put(0), take(0) {}
+  __device__ static void copy(Raw* to, const void* from, bool live) {
+    constexpr int kSize = static_cast<int>(sizeof(Raw));
+    if constexpr (kSize == 16)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(to)), "l"(from),
+                   "r"(live ? 16 : 0)
+                   : "memory");
+    else
+      asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(smem_addr(to)), "l"(from),
+                   "n"(kSize), "r"(live ? kSize : 0)
+                   : "memory");
+  }
   // asks for part q of the batch being put together; a dead part becomes zeros
   template <class T> __device__ void push(int q, const T* row, bool live, int col0, int dim) {
     Raw* at = base + (put * kBatch + q) * (kPieces * 32);
@@ -175,11 +205,7 @@ template <class P, int kBatch, int kStages> struct PartQueue {
       const int c = P::column(col0, u);
 #pragma unroll
       for (int p = 0; p < P::N; ++p)
-        if (c < dim)
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                           smem_addr(at + (u * P::N + p) * 32)),
-                       "l"(row + c + p * P::OE), "r"(live ? 16 : 0)
-                       : "memory");
+        if (c < dim) copy(at + (u * P::N + p) * 32, row + c + p * P::OE, live);
     }
   }
   __device__ void send() {
@@ -196,6 +222,7 @@ template <class P, int kBatch, int kStages> struct PartQueue {
     return v;
   }
   // nothing may be under way when the warp ends
+  __device__ void skip() { put = put + 1 == kStages ? 0 : put + 1; }  // shares another's groups
   __device__ void drain() { asm volatile("cp.async.wait_all;" ::: "memory"); }
   __device__ void done() { take = take + 1 == kStages ? 0 : take + 1; }
 };
@@ -204,7 +231,10 @@ template <class P, int kBatch, int kStages> struct PartQueue {
 constexpr int kQueueCtas = 4;
 constexpr int kQueueBatch = 2;
 constexpr int kQueueStages = 3;
-template <class T> constexpr int kQueueCols = 32 / static_cast<int>(sizeof(T));  // of a lane
+template <class T, int VE>
+constexpr int kQueueCols = VE == 1 ? 8 : 32 / static_cast<int>(sizeof(T));  // of a lane
+// whether parts can be queued: single 16-bit elements are too small for an asynchronous copy
+template <class T, int VE> constexpr bool kQueued = VE * sizeof(T) >= 4;
 
 // ---- embedding lookup ------------------------------------------------------------------------
 // One warp per (token, group of G slabs).
@@ -239,197 +269,361 @@ select_rows_kernel(IdKeys<I> ids, int64_t n, const T* __restrict__ table, int64_
 }
 
 // ---- embedding gradient ----------------------------------------------------------------------
-// The sorted (token, position) list is cut into tiles of 32 entries; a warp sums the rows of one
-// tile over one slab of columns and writes each token's row when its run of equal tokens ends.
-// A run that begins in one tile and ends in the next belongs to the first (it reads on); only a
-// run that spans two borders or more is written as one partial row per tile, which
-// select_grad_long_kernel adds in tile order.  No floating-point atomics: the sums have one
-// order whatever the scheduling.
-constexpr int kGradTile = 32;
-
+// The sorted (token, position) list is cut into as many ranges as the GPU holds warps for one slab
+// of columns; a warp sums the rows of its range and writes each token's row when its run of equal
+// tokens ends.  A run that crosses a border and ends within 31 entries behind it is read to its
+// end by the warp in front of the border.  A longer one is cut there: each range writes its piece
+// as a partial row, and select_grad_long_kernel adds the pieces in order.  No floating-point
+// atomics: the sums have one order whatever the scheduling.
 struct GradRuns {
-  const uint32_t* keys;  // sorted tokens; n_keys: masked, at the end
+  const uint32_t* keys;  // sorted tokens; the masked ones at the end
   const int32_t* vals;   // their positions
   int64_t n;
   uint32_t n_keys;
 };
+// how many entries are not masked (made by whole warps)
+__device__ inline int64_t grad_held(const GradRuns& runs) {
+  if (runs.keys[runs.n - 1] < runs.n_keys) return runs.n;
+  int64_t lo = 0, len = runs.n;  // the answer is in [lo, lo + len)
+  while (len > 0) {
+    const int64_t step = (len + 31) / 32, end = lo + len;
+    const int64_t at = lo + (threadIdx.x & 31) * step;
+    const int hits = __popc(__ballot_sync(0xffffffffu, at < end && runs.keys[at] < runs.n_keys));
+    if (hits == 0) break;
+    lo += (hits - 1) * step + 1;  // the entry in front of lo is held
+    len = end - lo < step - 1 ? end - lo : step - 1;
+  }
+  return lo;
+}
+struct GradRange {
+  int64_t range, size;  // its number, entries between two borders
+  int64_t lo, hi;       // the entries it sums
+  bool head, tail;      // its first run began before it; its last run goes on behind it
+};
 
-__device__ inline uint32_t run_key(const GradRuns& g, int64_t i) {
-  return (i >= 0 && i < g.n) ? g.keys[i] : (i < 0 ? 0xffffffffu : g.n_keys);
+// The ranges of m entries: `most` of them, or fewer (of eight entries at least).
+struct GradRanges {
+  int64_t m, size, count;
+  __device__ GradRanges(int64_t held, int64_t most) : m(held) {
+    const int64_t even = (held + most - 1) / most;
+    size = even > 8 ? even : 8;
+    count = (held + size - 1) / size;
+  }
+  __device__ int64_t border(int64_t r) const { return r * size < m ? r * size : m; }
+};
+// entries from border x on that continue the run in front of it, kCross for that many or more
+constexpr int kCross = 32;
+__device__ inline int grad_crossing(const GradRuns& runs, int64_t m, int64_t x) {
+  if (x <= 0 || x >= m) return 0;
+  const uint32_t key = runs.keys[x - 1];
+  int n = 0;
+#pragma unroll
+  for (int q = 0; q < kCross / 32; ++q) {
+    const int64_t i = x + 32 * q + (threadIdx.x & 31);
+    n += __popc(__ballot_sync(0xffffffffu, i < m && runs.keys[i] == key));
+  }
+  return n;
+}
+__device__ inline GradRange grad_range(const GradRuns& runs, const GradRanges& all, int64_t r) {
+  const int64_t a = all.border(r), b = all.border(r + 1);
+  const int in = grad_crossing(runs, all.m, a), out = grad_crossing(runs, all.m, b);
+  GradRange g;
+  g.range = r;
+  g.size = all.size;
+  g.head = in == kCross;
+  g.tail = out == kCross;
+  g.lo = a + (g.head ? 0 : in);
+  g.hi = b + (g.tail ? 0 : out);
+  return g;
 }
 
-template <class T, class O, int VE>
-__device__ inline void grad_tile(const GradRuns& runs, int64_t tile, int slab,
-                                 const T* __restrict__ grad, int64_t ld_grad, int dim,
-                                 O* __restrict__ out, int64_t ld_out,
-                                 typename acc_of<T>::type alpha, typename acc_of<T>::type beta,
-                                 bool has_beta, typename acc_of<T>::type* __restrict__ head,
-                                 typename acc_of<T>::type* __restrict__ tail,
-                                 int32_t* __restrict__ long_list, int32_t* long_count) {
+// Where the sums of a run go: its row of `out`, or a partial row of the range.
+template <class T, class O> struct GradOut {
   using A = typename acc_of<T>::type;
-  using RP = Part<T, VE>;
-  constexpr int P = kGradTile;
-  const int lane = threadIdx.x & 31;
-  const int64_t at = tile * P;
-  const uint32_t none = runs.n_keys;
-  const uint32_t cur = run_key(runs, at + lane);
-  const uint32_t nxt = run_key(runs, at + P + lane);
-  const uint32_t prv = run_key(runs, at - P + lane);
-  const int valid = __popc(__ballot_sync(0xffffffffu, cur < none));
-  if (valid == 0) return;
-  const uint32_t before = __shfl_sync(0xffffffffu, prv, 31);  // key of the entry before the tile
-  const uint32_t last = __shfl_sync(0xffffffffu, cur, valid - 1);
-  const uint32_t after = __shfl_sync(0xffffffffu, nxt, 0);
-  const int in_head = __popc(__ballot_sync(0xffffffffu, cur == before));
-  const int in_prev = __popc(__ballot_sync(0xffffffffu, prv == before));
-  const int in_tail = __popc(__ballot_sync(0xffffffffu, cur == last));
-  const int in_next = __popc(__ballot_sync(0xffffffffu, nxt == last));
-  const bool head_ends = in_head < P || after != before;
-  const bool head_began = in_prev < P || run_key(runs, at - P - 1) != before;
-  const bool goes_on = valid == P && after == last;
-  const bool tail_begins = in_tail < P || before != last;
-  const bool tail_ends = in_next < P || run_key(runs, at + 2 * P) != last;
-  const bool own_head = in_head > 0 && !(head_ends && head_began);  // a piece of a long run
-  const int lo = (in_head > 0 && !own_head) ? in_head : 0;
-  const bool long_tail = goes_on && tail_begins && !tail_ends;
-  const int hi = valid + (goes_on && tail_begins && tail_ends ? in_next : 0);
-  if (lo >= hi) return;
-  if (long_tail && slab == 0 && lane == 0) {
-    // (the order of the list does not reach any result: every entry is finished by itself)
-    long_list[atomicAdd(long_count, 1)] = static_cast<int32_t>(tile);
-  }
-  const int pos_cur = at + lane < runs.n ? runs.vals[at + lane] : 0;
-  const int pos_nxt = at + P + lane < runs.n ? runs.vals[at + P + lane] : 0;
-  const int col0 = slab * kSelCols;
+  O* out;
+  int64_t ld_out;
+  A alpha, beta;
+  A *head, *tail;  // partial rows of `dim` values, one per range
+  int4* long_list;  // of each cut run: the ranges it begins and ends in, its token
+  int32_t* long_count;
+  int dim;
 
-  Sums<A, 8> acc;
-  acc.clear();
-  // The rows of a group, and the rows of `out` that its ends are added to, are all asked for
-  // before the first is used: a run of one token (most are) would otherwise wait for its old
-  // row by itself.
-  constexpr int kAhead = 4;
-  for (int i0 = lo; i0 < hi; i0 += kAhead) {
-    RP r[kAhead];
-    Part<O, VE> old[kAhead];
-    uint32_t key[kAhead];
-    bool ends[kAhead];
-#pragma unroll
-    for (int q = 0; q < kAhead; ++q) {
-      const int i = i0 + q;
-      const int a = __shfl_sync(0xffffffffu, pos_cur, i & 31);
-      const int b = __shfl_sync(0xffffffffu, pos_nxt, i & 31);
-      const uint32_t ka = __shfl_sync(0xffffffffu, cur, i & 31);
-      const uint32_t kb = __shfl_sync(0xffffffffu, cur, (i + 1) & 31);
-      key[q] = i < P ? ka : last;
-      ends[q] = i < hi && (i + 1 >= hi || (i + 1 < P ? kb : last) != key[q]);
-      if (i < hi) r[q].load(grad + static_cast<int64_t>(i < P ? a : b) * ld_grad, col0, dim);
-      const bool part = (own_head && i < in_head) || (long_tail && i + 1 == hi);
-      if (has_beta && ends[q] && !part)
-        old[q].load(out + static_cast<int64_t>(key[q]) * ld_out, col0, dim);
+  // head: the run began before the range; tail: it goes on behind it
+  template <int VE, int E, bool kBeta>
+  __device__ void flush(const Sums<A, E>& acc, const Part<O, VE, E>& old, uint32_t key, int col0,
+                        const GradRuns& runs, const GradRange& g, bool is_head,
+                        bool is_tail) const {
+    if (is_head)
+      store_sums<A, VE>(head + g.range * dim, col0, dim, acc);
+    else if (is_tail)
+      store_sums<A, VE>(tail + g.range * dim, col0, dim, acc);
+    else
+      store_axpby<O, VE, A, E>(out + static_cast<int64_t>(key) * ld_out, col0, dim, acc, alpha,
+                               kBeta, beta, old);
+    if (is_head && !is_tail && col0 == 0) list(runs, g, key);
+  }
+  // a cut run ends in this range: where it begins (made by whole warps)
+  __device__ void list(const GradRuns& runs, const GradRange& g, uint32_t key) const {
+    const int lane = threadIdx.x & 31;
+    int64_t lo = 0, len = g.lo;  // its first entry is in [lo, lo + len)
+    while (len > 1) {
+      const int64_t step = (len + 31) / 32, end = lo + len, at = lo + lane * step;
+      const int below = __popc(__ballot_sync(0xffffffffu, at < end && runs.keys[at] < key));
+      if (below == 0) break;  // it is the entry at lo
+      lo += (below - 1) * step + 1;
+      len = end - lo < step ? end - lo : step;
     }
+    // (the order of the list does not reach any result: every entry is finished by itself)
+    if (lane == 0)
+      long_list[atomicAdd(long_count, 1)] =
+          make_int4(static_cast<int>(lo / g.size), static_cast<int>(g.range),
+                    static_cast<int>(key), 0);
+  }
+};
+
+// bit i: a run ends with entry i of the stretch whose keys the lanes hold
+__device__ inline uint32_t run_ends(uint32_t keys, uint32_t next_keys) {
+  const uint32_t first = __shfl_sync(0xffffffffu, next_keys, 0);
+  uint32_t right = __shfl_down_sync(0xffffffffu, keys, 1);
+  if ((threadIdx.x & 31) == 31) right = first;
+  return __ballot_sync(0xffffffffu, right != keys);
+}
+
+// The rows of the range stream through the warp's queue; where `out` is added to, the row that a
+// run ends in comes along with the run's last row (a run of one token, as most are, would
+// otherwise wait for it by itself).  Keys and positions are read 32 at a time, a stretch ahead.
+template <bool kBeta> constexpr int kGradStages = kBeta ? 4 : 6;
+template <class T, class O, int VE, bool kBeta>
+constexpr int kGradCols = kBeta && sizeof(O) > sizeof(T) ? 8 : kQueueCols<T, VE>;
+template <class T, class O, int VE, bool kBeta>
+__device__ inline void grad_sum(const GradRuns& runs, const GradRange& g,
+                                const GradOut<T, O>& to, unsigned char* warp_smem, int col0,
+                                const T* __restrict__ grad, int64_t ld_grad) {
+  constexpr int E = kGradCols<T, O, VE, kBeta>, S = kGradStages<kBeta>;
+  using Rows = PartQueue<Part<T, VE, E>, 1, S>;
+  using Olds = PartQueue<Part<O, VE, E>, 1, S>;
+  Rows rows(warp_smem);
+  Olds olds(warp_smem + Rows::kWarpBytes);  // not touched unless kBeta
+  const int lane = threadIdx.x & 31, dim = to.dim;
+  const uint32_t* keys = runs.keys + g.lo;
+  const int32_t* vals = runs.vals + g.lo;
+  const int count = static_cast<int>(g.hi - g.lo);
+  auto key_of = [&](int i) { return i < count ? keys[i] : 0xffffffffu; };
+  auto pos_of = [&](int i) { return i < count ? vals[i] : 0; };
+
+  int ask = 0, ask_pos = pos_of(lane), next_pos = pos_of(32 + lane);
+  uint32_t sum_keys = key_of(lane), next_keys = key_of(32 + lane);
+  uint32_t sum_ends = run_ends(sum_keys, next_keys);
+  uint32_t ask_keys = sum_keys, ask_next = next_keys, ask_ends = sum_ends;
+  bool ask_head = g.head, sum_head = g.head;
+  auto send = [&] {
+    const int at = ask & 31;
+    const int64_t pos = __shfl_sync(0xffffffffu, ask_pos, at);
+    if (ask < count) rows.push(0, grad + pos * ld_grad, true, col0, dim);
+    if constexpr (kBeta) {
+      const uint32_t key = __shfl_sync(0xffffffffu, ask_keys, at);
+      if (ask < count && ((ask_ends >> at) & 1)) {
+        if (!ask_head && !(g.tail && ask + 1 == count))
+          olds.push(0, to.out + static_cast<int64_t>(key) * to.ld_out, true, col0, dim);
+        ask_head = false;
+      }
+    }
+    rows.send();
+    if constexpr (kBeta) olds.skip();
+    ++ask;
+    if ((ask & 31) == 0) {
+      ask_pos = next_pos;
+      next_pos = pos_of(ask + 32 + lane);
+      if constexpr (kBeta) {
+        ask_keys = ask_next;
+        ask_next = key_of(ask + 32 + lane);
+        ask_ends = run_ends(ask_keys, ask_next);
+      }
+    }
+  };
+  for (int q = 0; q < S - 1; ++q) send();
+  Sums<typename acc_of<T>::type, E> acc;
+  acc.clear();
+  for (int i = 0; i < count; ++i) {
+    send();
+    rows.wait();
+    acc.add(rows.part(0));
+    const int at = i & 31;
+    if ((sum_ends >> at) & 1) {
+      Part<O, VE, E> old;
+      if constexpr (kBeta) old = olds.part(0);
+      to.template flush<VE, E, kBeta>(acc, old, __shfl_sync(0xffffffffu, sum_keys, at), col0,
+                                      runs, g, sum_head, g.tail && i + 1 == count);
+      acc.clear();
+      sum_head = false;
+    }
+    rows.done();
+    if constexpr (kBeta) olds.done();
+    if (at == 31) {
+      sum_keys = next_keys;
+      next_keys = key_of(i + 33 + lane);
+      sum_ends = run_ends(sum_keys, next_keys);
+    }
+  }
+  rows.drain();
+}
+// shared memory of one warp
+template <class T, class O, int VE, bool kBeta>
+constexpr int kGradWarpBytes =
+    PartQueue<Part<T, VE, kGradCols<T, O, VE, kBeta>>, 1, kGradStages<kBeta>>::kWarpBytes +
+    (kBeta ? PartQueue<Part<O, VE, kGradCols<T, O, VE, kBeta>>, 1, kGradStages<kBeta>>::kWarpBytes
+           : 0);
+
+// The same for rows that cannot be taken 16 bytes at a time: groups of rows in registers.
+template <class T, class O, bool kBeta>
+__device__ inline void grad_sum_plain(const GradRuns& runs, const GradRange& g,
+                                      const GradOut<T, O>& to, int col0,
+                                      const T* __restrict__ grad, int64_t ld_grad) {
+  constexpr int kAhead = sizeof(T) == 8 ? 2 : 4;
+  const int lane = threadIdx.x & 31;
+  Sums<typename acc_of<T>::type, 8> acc;
+  acc.clear();
+  bool head = g.head;
+  for (int64_t c = g.lo; c < g.hi; c += 32) {
+    const uint32_t keys = c + lane < g.hi ? runs.keys[c + lane] : 0xffffffffu;
+    const uint32_t next = c + 32 + lane < g.hi ? runs.keys[c + 32 + lane] : 0xffffffffu;
+    const int pos = c + lane < g.hi ? runs.vals[c + lane] : 0;
+    const uint32_t ends = run_ends(keys, next);
+    const int m = g.hi - c < 32 ? static_cast<int>(g.hi - c) : 32;
+    for (int i0 = 0; i0 < m; i0 += kAhead) {
+      Part<T, 1> r[kAhead];
+      Part<O, 1> old[kAhead];
 #pragma unroll
-    for (int q = 0; q < kAhead; ++q) {
-      const int i = i0 + q;
-      if (i < hi) {
-        acc.add(r[q]);
-        if (ends[q]) {
-          const bool is_head = own_head && i < in_head;
-          if (is_head || (long_tail && i + 1 == hi)) {
-            A* part = (is_head ? head : tail) + tile * dim;
-            store_sums<A, VE>(part, col0, dim, acc);
-          } else {
-            store_axpby<O, VE, A, 8>(out + static_cast<int64_t>(key[q]) * ld_out, col0, dim, acc,
-                                     alpha, has_beta, beta, old[q]);
+      for (int q = 0; q < kAhead; ++q) {
+        const int i = i0 + q;
+        const int64_t p = __shfl_sync(0xffffffffu, pos, i & 31);
+        const uint32_t key = __shfl_sync(0xffffffffu, keys, i & 31);
+        if (i < m) {
+          r[q].load(grad + p * ld_grad, col0, to.dim);
+          if (kBeta && ((ends >> i) & 1))
+            old[q].load(to.out + static_cast<int64_t>(key) * to.ld_out, col0, to.dim);
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < kAhead; ++q) {
+        const int i = i0 + q;
+        const uint32_t key = __shfl_sync(0xffffffffu, keys, i & 31);
+        if (i < m) {
+          acc.add(r[q]);
+          if ((ends >> i) & 1) {
+            to.template flush<1, 8, kBeta>(acc, old[q], key, col0, runs, g, head,
+                                           g.tail && c + i + 1 == g.hi);
+            acc.clear();
+            head = false;
           }
-          acc.clear();
         }
       }
     }
   }
 }
 
-// CTAs that sum tiles and CTAs that write the rows no token names (zero, or beta times what is
-// there; none when beta = 1 leaves them as they are) alternate from the first on, until one kind
-// is used up: the waits of the first overlap the writes of the second, and no long CTA starts
-// late.
-template <class T, class O, int VE>
-__global__ void __launch_bounds__(kSelThreads)
-select_grad_kernel(GradRuns runs, int64_t n_tiles, unsigned sum_blocks, unsigned slabs,
-                   const T* __restrict__ grad, int64_t ld_grad, int dim, O* __restrict__ out,
-                   int64_t ld_out, typename acc_of<T>::type alpha, typename acc_of<T>::type beta,
-                   bool has_beta, typename acc_of<T>::type* __restrict__ head,
-                   typename acc_of<T>::type* __restrict__ tail, int32_t* __restrict__ long_list,
-                   int32_t* long_count, const uint8_t* __restrict__ named) {
+// CTAs that share an SM: as many as their queues allow.
+template <class T, class O, int VE, bool kBeta>
+constexpr int kGradCtas = !kQueued<T, VE> || (VE == 1 && sizeof(T) == 8) ? 2
+                          : !kBeta || sizeof(O) > sizeof(T)               ? kQueueCtas
+                                                                          : 3;
+
+// CTAs that sum and CTAs that write the rows no token names (zero, or beta times what is there;
+// none when beta = 1 leaves them as they are) alternate from the first on, until one kind is used
+// up: the waits of the first overlap the writes of the second, and no long CTA starts late.
+// Rows per warp of the second kind.  Narrow accesses leave room for two CTAs on an SM, not four:
+// their warps take four rows, whose flags are one load.
+template <class T, int VE> constexpr int kRestRows = kQueued<T, VE> ? 1 : 4;
+template <class T, class O, int VE, bool kBeta>
+__global__ void __launch_bounds__(kSelThreads, kGradCtas<T, O, VE, kBeta>)
+select_grad_kernel(GradRuns runs, int64_t ranges, unsigned sum_blocks, unsigned slabs,
+                   const T* __restrict__ grad, int64_t ld_grad, GradOut<T, O> to,
+                   const uint8_t* __restrict__ named) {
+  extern __shared__ int4 smem4[];
   const int warp = threadIdx.x >> 5;
   const unsigned b = blockIdx.x, rest = gridDim.x - sum_blocks;
   const unsigned both = 2 * (sum_blocks < rest ? sum_blocks : rest);
   const bool sums = b < both ? (b & 1) == 0 : sum_blocks > rest;
   const unsigned at = b < both ? b / 2 : b - both / 2;  // among the CTAs of its kind
-  if (sums) {
-    const unsigned tb = at / slabs, slab = at - tb * slabs;
-    const int64_t tile = static_cast<int64_t>(tb) * kSelWarps + warp;
-    if (tile < n_tiles)
-      grad_tile<T, O, VE>(runs, tile, static_cast<int>(slab), grad, ld_grad, dim, out, ld_out,
-                          alpha, beta, has_beta, head, tail, long_list, long_count);
+  const int64_t w = static_cast<int64_t>(at) * kSelWarps + warp;
+  if (!sums) {
+    const int64_t row0 = w * kRestRows<T, VE>;
+    if (row0 >= runs.n_keys) return;
+    using Flags = typename raw_of<kRestRows<T, VE>>::type;
+    const uint32_t flags = *reinterpret_cast<const Flags*>(named + row0);  // (padded)
+    for (int q = 0; q < kRestRows<T, VE>; ++q) {
+      if (((flags >> (8 * q)) & 1) || row0 + q >= runs.n_keys) continue;
+      O* row = to.out + (row0 + q) * to.ld_out;
+      if constexpr (kBeta) scale_row<O, VE>(row, to.dim, to.beta);
+      else zero_row(row, to.dim);
+    }
     return;
   }
-  const int64_t row = static_cast<int64_t>(at) * kSelWarps + warp;
-  if (row < runs.n_keys && !named[row]) scale_row<O, VE>(out + row * ld_out, dim, has_beta, beta);
+  const int64_t range = w / slabs;
+  const int slab = static_cast<int>(w - range * slabs);
+  if (range >= ranges) return;
+  const GradRanges all(grad_held(runs), ranges);
+  if (range >= all.count) return;
+  const GradRange g = grad_range(runs, all, range);
+  if (g.lo >= g.hi) return;
+  if constexpr (!kQueued<T, VE>)
+    grad_sum_plain<T, O, kBeta>(runs, g, to, slab * kSelCols, grad, ld_grad);
+  else
+    grad_sum<T, O, VE, kBeta>(runs, g, to,
+                              reinterpret_cast<unsigned char*>(smem4) +
+                                  warp * kGradWarpBytes<T, O, VE, kBeta>,
+                              slab * (32 * kGradCols<T, O, VE, kBeta>), grad, ld_grad);
 }
 
-// A run that spans two tile borders or more: the piece of its first tile, then the pieces of the
-// tiles behind it.  One CTA per (run, 128 columns): its warps take the pieces in turn and the
-// warps' sums are added in warp order.
+// A run that was cut: the piece of the range it begins in, then the pieces of those behind.  One
+// CTA per (run, slab of 32 E columns): its warps take the pieces in turn and the warps' sums are
+// added in warp order.
 constexpr int kLongWarps = 8;
-constexpr int kLongCols = 128;
 
-template <class A, class O>
-__global__ void __launch_bounds__(32 * kLongWarps)
-select_grad_long_kernel(GradRuns runs, int64_t n_tiles, int dim, O* __restrict__ out,
-                        int64_t ld_out, A alpha, A beta, bool has_beta,
-                        const A* __restrict__ head, const A* __restrict__ tail,
-                        const int32_t* __restrict__ long_list,
-                        const int32_t* __restrict__ long_count) {
-  __shared__ A sums[kLongWarps][kLongCols];
+template <class T, class O, int VE, int E>
+__global__ void __launch_bounds__(32 * kLongWarps, sizeof(T) == 8 ? 2 : 3)
+select_grad_long_kernel(GradOut<T, O> to, bool has_beta) {
+  using A = typename acc_of<T>::type;
+  __shared__ A sums[kLongWarps][E][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int count = *long_count;
-  const int col0 = static_cast<int>(blockIdx.y) * kLongCols + lane;
+  const int count = *to.long_count;
+  int4 run = to.long_list[blockIdx.x];  // (there is room for gridDim.x entries)
+  const int col0 = static_cast<int>(blockIdx.y) * (32 * E);
   for (int item = blockIdx.x; item < count; item += gridDim.x) {
-    const int64_t first = long_list[item];
-    const uint32_t key = runs.keys[first * kGradTile + kGradTile - 1];
-    // the last tile whose first entry has this key, 32 places at a time
-    int64_t lo = first + 1, len = n_tiles - lo;
-    while (len > 1) {
-      const int64_t step = (len + 31) / 32;
-      const int64_t at = lo + lane * step;
-      const bool mine = at < lo + len && runs.keys[at * kGradTile] <= key;
-      const int hits = __popc(__ballot_sync(0xffffffffu, mine));  // lane 0 always hits
-      const int64_t end = lo + len;
-      lo += (hits - 1) * step;
-      len = end - lo < step ? end - lo : step;
-    }
-    A acc[4] = {A(0), A(0), A(0), A(0)};
-#pragma unroll 4
-    for (int64_t t = first + warp; t <= lo; t += kLongWarps) {
-      const A* part = (t == first ? tail : head) + t * dim;
+    if (item != static_cast<int>(blockIdx.x)) run = to.long_list[item];
+    const int first = run.x, last = run.y;
+    const uint32_t key = static_cast<uint32_t>(run.z);
+    Sums<A, E> acc;
+    acc.clear();
+    constexpr int kAhead = 4;
+    for (int r0 = first + warp; r0 <= last; r0 += kAhead * kLongWarps) {
+      Part<A, VE, E> part[kAhead];
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (col0 + 32 * e < dim) acc[e] = acc[e] + part[col0 + 32 * e];
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) sums[warp][lane + 32 * e] = acc[e];
-    __syncthreads();
-    if (threadIdx.x < kLongCols) {
-      A s = A(0);
-#pragma unroll
-      for (int w = 0; w < kLongWarps; ++w) s = s + sums[w][threadIdx.x];
-      const int col = static_cast<int>(blockIdx.y) * kLongCols + threadIdx.x;
-      if (col < dim) {
-        O* o = out + static_cast<int64_t>(key) * ld_out + col;
-        A x = alpha * s;
-        if (has_beta) x = x + beta * static_cast<A>(to_acc(*o));
-        *o = storage_of<O>::from_acc(x);
+      for (int q = 0; q < kAhead; ++q) {
+        const int r = r0 + q * kLongWarps;
+        if (r <= last)
+          part[q].load((r == first ? to.tail : to.head) + static_cast<int64_t>(r) * to.dim, col0,
+                       to.dim);
       }
+#pragma unroll
+      for (int q = 0; q < kAhead; ++q)
+        if (r0 + q * kLongWarps <= last) acc.add(part[q]);
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) sums[warp][e][lane] = sum_of(acc, e);
+    __syncthreads();
+    if (warp == 0) {
+      Sums<A, E> total;
+      total.clear();
+#pragma unroll
+      for (int w = 0; w < kLongWarps; ++w) {
+        Part<A, 1, E> part;
+#pragma unroll
+        for (int e = 0; e < E; ++e) part.set(e, sums[w][e][lane]);
+        total.add(part);
+      }
+      store_axpby<O, VE, A, E>(to.out + static_cast<int64_t>(key) * to.ld_out, col0, to.dim, total,
+                               to.alpha, has_beta, to.beta);
     }
     __syncthreads();
   }
@@ -492,14 +686,16 @@ __device__ inline typename acc_of<T>::type route_weight(const void* w, bool w_is
 // time and a stretch ahead, and their rows stream through the warp's queue without a pause
 // between tokens.  A masked assignment is a part of zeros with weight zero.
 template <class T, int VE>
-__global__ void __launch_bounds__(kSelThreads, kQueueCtas)
+constexpr int kCombineCtas = VE == 1 && sizeof(T) == 8 ? 2 : kQueueCtas;
+template <class T, int VE>
+__global__ void __launch_bounds__(kSelThreads, kCombineCtas<T, VE>)
 route_combine_kernel(const T* __restrict__ y, int64_t ld_y, const int32_t* __restrict__ slots,
                      const void* __restrict__ weights, bool w_is_f32, int64_t n, int k, int dim,
                      T* __restrict__ out, int64_t ld_out, typename acc_of<T>::type alpha,
                      typename acc_of<T>::type beta, bool has_beta, unsigned slabs,
                      unsigned ranges) {
   using A = typename acc_of<T>::type;
-  constexpr int E = kQueueCols<T>, B = kQueueBatch;
+  constexpr int E = kQueueCols<T, VE>, B = kQueueBatch;
   using Queue = PartQueue<Part<T, VE, E>, B, kQueueStages>;
   extern __shared__ int4 smem4[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -531,7 +727,7 @@ route_combine_kernel(const T* __restrict__ y, int64_t ld_y, const int32_t* __res
 #pragma unroll
     for (int q = 0; q < B; ++q) {
       const int32_t s = __shfl_sync(0xffffffffu, ask_slot, (ask + q) & 31);
-      queue.push(q, y + static_cast<int64_t>(s < 0 ? 0 : s) * ld_y, s >= 0, col0, dim);
+      if (y) queue.push(q, y + static_cast<int64_t>(s < 0 ? 0 : s) * ld_y, s >= 0, col0, dim);
     }
     queue.send();
     ask += B;
@@ -543,6 +739,9 @@ route_combine_kernel(const T* __restrict__ y, int64_t ld_y, const int32_t* __res
   for (int q = 0; q < kQueueStages - 1; ++q) send();
   Sums<A, E> acc;
   acc.clear();
+  if (k == 0)
+    for (; t < t1; ++t)
+      store_axpby<T, VE, A, E>(out + t * ld_out, col0, dim, acc, alpha, has_beta, beta);
   int j = 0;
   for (int a = 0; a < count; a += B) {
     send();
@@ -661,7 +860,7 @@ route_combine_grad_kernel(const T* __restrict__ g, int64_t ld_g, const T* __rest
     }
   }
   const int64_t z = *held_at + a;
-  if (z < n * k) scale_row<T, VE, A>(grad_y + z * ld_gy, dim, false, A(0));
+  if (z < n * k) zero_row(grad_y + z * ld_gy, dim);
 }
 
 // ---- host ----------------------------------------------------------------------------------------
@@ -698,18 +897,32 @@ constexpr int64_t kMaxGrid = 0x7fffffff;
     if (st_ != B2S_OK) return st_;       \
   } while (0)
 
+// How the sorted list is cut: ranges of 24 entries (rows that are also read and written take
+// longer than others: the more ranges a warp slot gets, the more even the work), longer ones where
+// every slot has eight ranges already, and down to 8 entries where half the slots would have none.
+inline int64_t grad_ranges(int64_t n, int64_t slabs, int64_t ctas_per_sm) {
+  const int64_t slots = 148 * ctas_per_sm * kSelWarps;
+  const int64_t most = std::min(8 * slots / slabs, ceil_div(n, 24));
+  const int64_t least = std::min(slots / (2 * slabs), ceil_div(n, 8));
+  return std::max<int64_t>(std::max(most, least), 1);
+}
 struct GradLayout {
-  int64_t keys, vals, list, head, tail, named, end;
+  int64_t keys, vals, words, head, tail, named, end;
+  int64_t ranges;  // partial rows there is room for
 };
+// words: the number of cut runs, the list of them
 inline GradLayout grad_layout(int vtype, int64_t n, int64_t n_rows, int64_t dim) {
   GradLayout l;
-  const int64_t tiles = ceil_div(n, kGradTile);
+  // (the most ranges any of the kernels uses: slabs of at most 1 KB, kQueueCtas CTAs)
+  const int64_t slabs = ceil_div(dim * static_cast<int64_t>(vsize(vtype)), 1024);
+  l.ranges = grad_ranges(n, slabs > 0 ? slabs : 1, kQueueCtas);
+  const int64_t part = align256(l.ranges * dim * static_cast<int64_t>(acc_size(vtype)));
   int64_t at = sort_bytes(n, n_rows);
   l.keys = at; at += align256(n * 4);
   l.vals = at; at += align256(n * 4);
-  l.list = at; at += align256((tiles + 1) * 4);
-  l.head = at; at += align256(tiles * dim * static_cast<int64_t>(acc_size(vtype)));
-  l.tail = at; at += align256(tiles * dim * static_cast<int64_t>(acc_size(vtype)));
+  l.words = at; at += align256((l.ranges + 1) * 16);
+  l.head = at; at += part;
+  l.tail = at; at += part;
   l.named = at; at += align256(n_rows);
   l.end = at;
   return l;
@@ -742,38 +955,53 @@ int select_rows_run(const IdKeys<I>& ids, int64_t n, const void* table, int64_t 
   return launch_status();
 }
 
+template <class T, class O, int VE, bool kBeta>
+int select_grad_go(const GradRuns& runs, const T* grad, int64_t ld_grad,
+                   const GradOut<T, O>& to, const uint8_t* named, int64_t most_ranges,
+                   cudaStream_t s) {
+  using A = typename acc_of<T>::type;
+  constexpr int E = kGradCols<T, O, VE, kBeta>;
+  constexpr size_t smem = kQueued<T, VE> ? kSelWarps * kGradWarpBytes<T, O, VE, kBeta> : 0;
+  const int64_t slabs = ceil_div(to.dim, 32 * E);
+  const int64_t ranges =
+      runs.n == 0 ? 0 : std::min(grad_ranges(runs.n, slabs, kGradCtas<T, O, VE, kBeta>), most_ranges);
+  const int64_t sums = ceil_div(ranges * slabs, kSelWarps);
+  const int64_t rest = to.beta == A(1) ? 0 : ceil_div(static_cast<int64_t>(runs.n_keys),
+                                                        kRestRows<T, VE> * kSelWarps);
+  if (sums + rest > kMaxGrid) return B2S_ERR_RANGE;
+  if (sums + rest == 0) return B2S_OK;
+  auto kernel = &select_grad_kernel<T, O, VE, kBeta>;
+  if (smem > 0) ensure_dyn_smem(reinterpret_cast<const void*>(kernel), smem);
+  kernel<<<static_cast<unsigned>(sums + rest), kSelThreads, smem, s>>>(
+      runs, ranges, static_cast<unsigned>(sums), static_cast<unsigned>(slabs), grad, ld_grad, to,
+      named);
+  if (runs.n > kCross) {  // a run that is cut goes on for kCross entries behind a border
+    constexpr int kCols = VE > 1 && sizeof(T) == 8 ? 4 : 8;
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>(ranges, 128)),
+                    static_cast<unsigned>(ceil_div(to.dim, 32 * kCols)));
+    select_grad_long_kernel<T, O, VE, kCols><<<grid, 32 * kLongWarps, 0, s>>>(to, kBeta);
+  }
+  return launch_status();
+}
+
 template <class T, class O>
-int select_grad_run(const GradRuns& runs, const void* grad, int64_t ld_grad, int64_t dim,
-                    void* out, int64_t ld_out, double alpha, double beta, unsigned char* ws,
+int select_grad_run(const GradRuns& runs, const void* grad, int64_t ld_grad, int64_t dim, void* out,
+                    int64_t ld_out, double alpha, double beta, unsigned char* ws,
                     const GradLayout& l, cudaStream_t s) {
   using A = typename acc_of<T>::type;
   const bool wide = wide_rows(grad, ld_grad, dim, sizeof(T)) &&
                     wide_rows(out, ld_out, dim, sizeof(O)) && (dim * sizeof(T)) % 16 == 0;
-  const int64_t tiles = ceil_div(runs.n, kGradTile), slabs = ceil_div(dim, kSelCols);
-  const A a = static_cast<A>(alpha), b = static_cast<A>(beta);
-  const int64_t sums = ceil_div(tiles, kSelWarps) * slabs;
-  const int64_t rest = b == A(1) ? 0 : ceil_div(static_cast<int64_t>(runs.n_keys), kSelWarps);
-  if (sums + rest > kMaxGrid) return B2S_ERR_RANGE;
-  if (sums + rest == 0) return B2S_OK;
-  A* head = reinterpret_cast<A*>(ws + l.head);
-  A* tail = reinterpret_cast<A*>(ws + l.tail);
-  int32_t* list = reinterpret_cast<int32_t*>(ws + l.list);
-  const unsigned grid = static_cast<unsigned>(sums + rest);
-#define B2S_GO(VE)                                                                             \
-  select_grad_kernel<T, O, VE><<<grid, kSelThreads, 0, s>>>(                                   \
-      runs, tiles, static_cast<unsigned>(sums), static_cast<unsigned>(slabs),                  \
-      static_cast<const T*>(grad), ld_grad, static_cast<int>(dim), static_cast<O*>(out), ld_out, \
-      a, b, b != A(0), head, tail, list + 1, list, ws + l.named)
-  if (wide) B2S_GO(16 / sizeof(T)); else B2S_GO(1);
-#undef B2S_GO
-  if (tiles > 2) {  // a long run touches three tiles at least
-    const dim3 lg(static_cast<unsigned>(tiles < 256 ? tiles : 256),
-                  static_cast<unsigned>(ceil_div(dim, kLongCols)));
-    select_grad_long_kernel<A, O><<<lg, 32 * kLongWarps, 0, s>>>(
-        runs, tiles, static_cast<int>(dim), static_cast<O*>(out), ld_out, a, b, b != A(0), head,
-        tail, list + 1, list);
-  }
-  return launch_status();
+  int32_t* words = reinterpret_cast<int32_t*>(ws + l.words);
+  const GradOut<T, O> to{static_cast<O*>(out), ld_out, static_cast<A>(alpha), static_cast<A>(beta),
+                         reinterpret_cast<A*>(ws + l.head), reinterpret_cast<A*>(ws + l.tail),
+                         reinterpret_cast<int4*>(words + 4), words, static_cast<int>(dim)};
+  auto go = [&](auto run) {
+    return run(runs, static_cast<const T*>(grad), ld_grad, to, ws + l.named, l.ranges, s);
+  };
+  constexpr int VE = 16 / sizeof(T);
+  if (wide) return to.beta != A(0) ? go(&select_grad_go<T, O, VE, true>)
+                                   : go(&select_grad_go<T, O, VE, false>);
+  return to.beta != A(0) ? go(&select_grad_go<T, O, 1, true>) : go(&select_grad_go<T, O, 1, false>);
 }
 
 }  // namespace b2s
@@ -831,12 +1059,12 @@ extern "C" int b2s_select_grad(int val_type, int out_type, int idx_type, const v
   unsigned char* ws = static_cast<unsigned char*>(ws_dev);
   uint32_t* keys = reinterpret_cast<uint32_t*>(ws + l.keys);
   int32_t* vals = reinterpret_cast<int32_t*>(ws + l.vals);
+  int32_t* words = reinterpret_cast<int32_t*>(ws + l.words);
   B2S_DISPATCH_I(idx_type, I, {
     const IdKeys<I> ids{static_cast<const I*>(idx_dev), static_cast<uint32_t>(n_rows),
                         has_ignore != 0, ignore, status};
     const RunsOut sink{keys, vals, ws + l.named, static_cast<uint32_t>(n_rows)};
-    B2S_TRY(sort_ids(ids, n, sink, ws + l.named, n_rows,
-                     reinterpret_cast<int32_t*>(ws + l.list), ws, s));
+    B2S_TRY(sort_ids(ids, n, sink, ws + l.named, n_rows, words, ws, s));
   });
   const GradRuns runs{keys, vals, n, static_cast<uint32_t>(n_rows)};
   if (out_type == val_type) {
@@ -844,8 +1072,8 @@ extern "C" int b2s_select_grad(int val_type, int out_type, int idx_type, const v
                                                               out_dev, ld_out, alpha, beta, ws,
                                                               l, s)));
   } else if (val_type == B2S_F16) {
-    return select_grad_run<f16, float>(runs, grad_dev, ld_grad, dim, out_dev, ld_out, alpha, beta,
-                                       ws, l, s);
+    return select_grad_run<f16, float>(runs, grad_dev, ld_grad, dim, out_dev, ld_out, alpha,
+                                       beta, ws, l, s);
   } else {
     return select_grad_run<bf16, float>(runs, grad_dev, ld_grad, dim, out_dev, ld_out, alpha,
                                         beta, ws, l, s);
@@ -906,13 +1134,13 @@ int route_combine_go(const T* y, int64_t ld_y, const int32_t* slots, const void*
                      double alpha, double beta, cudaStream_t s) {
   using A = typename acc_of<T>::type;
   auto kernel = &route_combine_kernel<T, VE>;
-  constexpr int E = kQueueCols<T>;
+  constexpr int E = kQueueCols<T, VE>;
   constexpr size_t smem =
       kSelWarps * PartQueue<Part<T, VE, E>, kQueueBatch, kQueueStages>::kWarpBytes;
   ensure_dyn_smem(reinterpret_cast<const void*>(kernel), smem);
   const int64_t slabs = ceil_div(dim, 32 * E);
   // every warp that fits the GPU at once gets one range
-  constexpr int64_t kResident = 148 * kQueueCtas * kSelWarps;
+  constexpr int64_t kResident = 148 * kCombineCtas<T, VE> * kSelWarps;
   int64_t ranges = kResident / slabs;
   ranges = ranges < 1 ? 1 : ranges > n ? n : ranges;
   // a warp counts its assignments in 32 bits (with two stretches to spare)
@@ -930,21 +1158,25 @@ template <class T>
 int route_combine_run(const void* y, int64_t ld_y, const int32_t* slots, const void* weights,
                       bool w_f32, int64_t n, int64_t k, int64_t dim, void* out, int64_t ld_out,
                       double alpha, double beta, cudaStream_t s) {
-  const bool wide = k > 0 && wide_rows(y, ld_y, dim, sizeof(T)) &&
-                    wide_rows(out, ld_out, dim, sizeof(T));
+  const bool wide = wide_rows(out, ld_out, dim, sizeof(T)) &&
+                    (k == 0 || wide_rows(y, ld_y, dim, sizeof(T)));
   const T* yp = static_cast<const T*>(y);
   T* op = static_cast<T*>(out);
   if (wide)
-    return route_combine_go<T, 16 / sizeof(T)>(
-        yp, ld_y, slots, weights, w_f32, n, k, dim, op, ld_out, alpha, beta, s);
-  using A = typename acc_of<T>::type;
-  const int64_t slabs = ceil_div(dim, kSelCols), blocks = ceil_div(n, kSelWarps) * slabs;
-  if (blocks > kMaxGrid) return B2S_ERR_RANGE;
-  const A b = static_cast<A>(beta);
-  route_combine_plain_kernel<T><<<static_cast<unsigned>(blocks), kSelThreads, 0, s>>>(
-      yp, ld_y, slots, weights, w_f32, n, static_cast<int>(k), static_cast<int>(dim), op, ld_out,
-      static_cast<A>(alpha), b, b != A(0), static_cast<unsigned>(slabs));
-  return launch_status();
+    return route_combine_go<T, 16 / sizeof(T)>(yp, ld_y, slots, weights, w_f32, n, k, dim, op,
+                                               ld_out, alpha, beta, s);
+  if constexpr (kQueued<T, 1>)
+    return route_combine_go<T, 1>(yp, ld_y, slots, weights, w_f32, n, k, dim, op, ld_out, alpha,
+                                  beta, s);
+  if constexpr (!kQueued<T, 1>) {
+    const int64_t slabs = ceil_div(dim, kSelCols), blocks = ceil_div(n, kSelWarps) * slabs;
+    if (blocks > kMaxGrid) return B2S_ERR_RANGE;
+    const float b = static_cast<float>(beta);
+    route_combine_plain_kernel<T><<<static_cast<unsigned>(blocks), kSelThreads, 0, s>>>(
+        yp, ld_y, slots, weights, w_f32, n, static_cast<int>(k), static_cast<int>(dim), op, ld_out,
+        static_cast<float>(alpha), b, b != 0, static_cast<unsigned>(slabs));
+    return launch_status();
+  }
 }
 
 template <class T>

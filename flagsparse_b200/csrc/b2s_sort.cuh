@@ -323,7 +323,7 @@ inline SortShape sort_shape(int64_t n, int64_t n_keys) {
 inline int64_t sort_bytes(int64_t n, int64_t n_keys) {
   const SortShape s = sort_shape(n, n_keys);
   const int lists = s.passes > 2 ? 2 : s.passes - 1;
-  return lists * 2 * align256(n * 4) + align256(s.chunks * s.bins * 4);
+  return lists * 2 * align256(n * 4) + (s.chunks > 1 ? align256(s.chunks * s.bins * 4) : 0);
 }
 
 // Sorts ids 0 .. n - 1 into `out`; zeroes clear[0 .. n_clear) (padded to 16) and *counter before

@@ -90,34 +90,40 @@ def check_selection_ids(device=None):
 
 
 # -------------------------------------------------------------------------------------------------
-# arguments
+# arguments.  A decoding step makes these calls on a few rows, where the host's time is all there
+# is: what every call checks is spelled out instead of looped over.
 # -------------------------------------------------------------------------------------------------
+_Tensor = torch.Tensor
+# the stream's handle without a Stream object around it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _check_ids(t, name):
-    if not torch.is_tensor(t):
+    if not isinstance(t, _Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if t.dtype not in SUPPORTED_INDEX_DTYPES:
         raise TypeError(f"{name} dtype must be torch.int32 or torch.int64")
 
 
 def _check_values(t, name):
-    if not torch.is_tensor(t):
+    if not isinstance(t, _Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
     if t.dtype not in SUPPORTED_SELECTION_VALUE_DTYPES:
         raise TypeError(f"{name} dtype must be one of: float16, bfloat16, float32, float64")
 
 
-def _check_device(named):
-    first = None
-    for name, t in named:
-        if t is None:
-            continue
+def _check_first_device(t, name):
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    return t.get_device()
+
+
+def _check_same_device(t, name, index, first):
+    if t is not None and t.get_device() != index:
         if not t.is_cuda:
             raise ValueError(f"{name} must be a CUDA tensor")
-        if first is None:
-            first = (name, t.device)
-        elif t.device != first[1]:
-            raise ValueError(f"{name} must be on the same CUDA device as {first[0]}")
-    return first[1]
+        raise ValueError(f"{name} must be on the same CUDA device as {first}")
 
 
 def _check_size(name, value, limit):
@@ -131,10 +137,13 @@ def _as_int(value, name):
     return value.__index__()
 
 
-def _wants_grad(*tensors):
-    if not torch.is_grad_enabled():
-        return False
-    return any(t is not None and t.requires_grad for t in tensors)
+def _scalar(value, dtype, name):
+    return value if type(value) is float else check_scalar(value, dtype, name)
+
+
+def _wants_grad(t, other=None):
+    return ((t.requires_grad or (other is not None and other.requires_grad))
+            and torch.is_grad_enabled())
 
 
 def _refuse_capture():
@@ -144,70 +153,64 @@ def _refuse_capture():
             "torch.no_grad() and take the gradients with the *_grad functions")
 
 
-def _refuse_out(out, tensors):
-    if out is not None and _wants_grad(out, *tensors):
+def _refuse_out(out, t, other=None):
+    if _wants_grad(out, t) or _wants_grad(out, other):
         raise RuntimeError("out= does not support automatic differentiation, but one of the "
                            "arguments requires grad")
 
 
 def _rows(t):
     """`t` (2-D) with unit stride inside a row and rows that do not overlap; copied if need be."""
-    return t if _row_major_ok(t) else t.contiguous()
+    return t if t.is_contiguous() or _row_major_ok(t) else t.contiguous()
 
 
 def _pitch(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-class _Result:
-    """Where a call writes: a new tensor, `out` itself, or (when the kernels cannot write its
-    layout) a contiguous stand-in that is copied into `out` afterwards."""
-
-    __slots__ = ("out", "flat", "stand_in")
-
-    def __init__(self, out, shape, dtype, device, beta, what="out"):
-        rows = 1
-        for n in shape[:-1]:
-            rows *= n
-        self.out, self.stand_in = out, False
-        if out is None:
-            if beta != 0:
-                raise ValueError("beta != 0 requires out= holding the rows to scale")
-            self.out = torch.empty(shape, dtype=dtype, device=device)
-            self.flat = self.out if len(shape) == 2 else self.out.view(rows, shape[-1])
-            return
-        if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
-            raise ValueError("out shape/dtype must match result")
-        if len(shape) == 2:
-            flat = out
-        else:
-            try:
-                flat = out.view(rows, shape[-1])
-            except RuntimeError:
-                flat = None
-        if flat is None or not _row_major_ok(flat):
-            flat = out.reshape(rows, shape[-1]).contiguous() if beta != 0 else torch.empty(
-                (rows, shape[-1]), dtype=dtype, device=device)
-            self.stand_in = True
-        self.flat = flat
-
-    def done(self, given):
-        if self.stand_in:
-            self.out.copy_(self.flat.view(self.out.shape))
-        elif given is not None:
-            # written by a kernel: tell autograd (and everything else that watches the counter)
-            torch.autograd.graph.increment_version(given)
-        return self.out
+def _result(out, shape, like, dtype, beta):
+    """(tensor the kernels write, its address, its pitch) for the result of a call: a new tensor,
+    `out` itself, or (when the kernels cannot write its layout) a contiguous stand-in, which
+    _finish copies into `out`.  `like`: a tensor on the device."""
+    if out is None:
+        if beta != 0:
+            raise ValueError("beta != 0 requires out= holding the rows to scale")
+        out = like.new_empty(shape, dtype=dtype)
+        return out, out.data_ptr(), shape[-1]
+    if tuple(out.shape) != tuple(shape) or out.dtype != dtype:
+        raise ValueError("out shape/dtype must match result")
+    flat = out
+    if len(shape) != 2:
+        try:
+            flat = out.view(-1 if out.numel() else 0, shape[-1])
+        except RuntimeError:
+            flat = None
+    if flat is None or not _row_major_ok(flat):
+        flat = out.clone(memory_format=torch.contiguous_format) if beta != 0 else like.new_empty(
+            shape, dtype=dtype)
+        return flat, flat.data_ptr(), shape[-1]
+    return flat, flat.data_ptr(), _pitch(flat)
 
 
-def _call(device, fn, *args):
-    """fn(*args, stream of `device`) with `device` current; raise on a non-zero status."""
-    index = device.index
+def _finish(out, flat):
+    """What the call returns: `flat` if the caller gave no `out`."""
+    if out is None:
+        return flat
+    if out.numel() and flat.data_ptr() != out.data_ptr():
+        out.copy_(flat)
+    else:  # written by a kernel: tell autograd and whoever else watches the counter
+        torch.autograd.graph.increment_version(out)
+    return out
+
+
+def _call(index, fn, *args):
+    """fn(*args, current stream of device `index`) with that device current; raise on a non-zero
+    status."""
     if torch.cuda.current_device() == index:
-        st = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+        st = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            st = fn(*args, torch.cuda.current_stream(index).cuda_stream)
+            st = fn(*args, _raw_stream(index))
     if st:
         _lib.check(st, fn.__name__)
 
@@ -236,35 +239,40 @@ def flagsparse_embedding(tokens, table, alpha=1.0, ignore_index=None, out=None, 
     """
     _check_ids(tokens, "tokens")
     _check_values(table, "table")
-    if table.ndim != 2:
+    if table.dim() != 2:
         raise ValueError("table must be a 2D tensor: (n_rows, dim)")
-    alpha = check_scalar(alpha, table.dtype, "alpha")
-    beta = check_scalar(beta, table.dtype, "beta")
+    alpha = _scalar(alpha, table.dtype, "alpha")
+    beta = _scalar(beta, table.dtype, "beta")
     has_ignore, ignore = _ignored(ignore_index)
-    _refuse_out(out, (table,))
-    device = _check_device((("table", table), ("tokens", tokens), ("out", out)))
+    if out is not None:
+        _refuse_out(out, table)
+    index = _check_first_device(table, "table")
+    _check_same_device(tokens, "tokens", index, "table")
+    _check_same_device(out, "out", index, "table")
     if _wants_grad(table):
         _refuse_capture()
+        if beta != 0:
+            raise ValueError("beta != 0 requires out= holding the rows to scale")
         return _Embedding.apply(tokens, table, alpha, has_ignore, ignore)
-    return _embedding(tokens, table, alpha, has_ignore, ignore, out, beta, device)
+    return _embedding(tokens, table, alpha, has_ignore, ignore, out, beta, index)
 
 
-def _embedding(tokens, table, alpha, has_ignore, ignore, out, beta, device):
+def _embedding(tokens, table, alpha, has_ignore, ignore, out, beta, index):
     n_rows, dim = table.shape
     n = tokens.numel()
-    _check_size("the number of tokens", n, MAX_ENTRIES)
-    _check_size("the number of rows of table", n_rows, MAX_ROWS)
-    _check_size("dim", dim, MAX_DIM)
-    result = _Result(out, (*tokens.shape, dim), table.dtype, device, beta)
+    if n > MAX_ENTRIES or n_rows > MAX_ROWS or dim > MAX_DIM:
+        _check_size("the number of tokens", n, MAX_ENTRIES)
+        _check_size("the number of rows of table", n_rows, MAX_ROWS)
+        _check_size("dim", dim, MAX_DIM)
+    flat, address, pitch = _result(out, (*tokens.shape, dim), table, table.dtype, beta)
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
-    table, flat = _rows(table), result.flat
-    lib = _lib.load()
-    _call(device, lib.b2s_select_rows, _lib.VALUE_CODE[table.dtype],
+    table = _rows(table)
+    _call(index, _lib.load().b2s_select_rows, _lib.VALUE_CODE[table.dtype],
           _lib.INDEX_CODE[tokens.dtype], tokens.data_ptr(), n, has_ignore, ignore,
-          table.data_ptr(), n_rows, _pitch(table), dim, flat.data_ptr(), _pitch(flat), alpha, beta,
-          _status_word(device.index))
-    return result.done(out)
+          table.data_ptr(), n_rows, _pitch(table), dim, address, pitch, alpha, beta,
+          _status_word(index))
+    return flat if out is None else _finish(out, flat)
 
 
 def flagsparse_embedding_grad(tokens, grad, n_rows, alpha=1.0, ignore_index=None, out=None,
@@ -283,36 +291,41 @@ def flagsparse_embedding_grad(tokens, grad, n_rows, alpha=1.0, ignore_index=None
     n_rows = _as_int(n_rows, "n_rows")
     if n_rows < 0:
         raise ValueError("n_rows must be non-negative")
-    if grad.ndim != tokens.ndim + 1 or grad.shape[:-1] != tokens.shape:
-        raise ValueError(f"grad shape must be tokens.shape + (dim,), got {tuple(grad.shape)} for "
+    shape = grad.shape
+    if len(shape) != tokens.dim() + 1 or shape[:-1] != tokens.shape:
+        raise ValueError(f"grad shape must be tokens.shape + (dim,), got {tuple(shape)} for "
                          f"tokens of shape {tuple(tokens.shape)}")
+    dtype = grad.dtype
     if out_dtype is None:
-        out_dtype = grad.dtype if out is None else out.dtype
-    if out_dtype != grad.dtype and not (out_dtype == torch.float32 and grad.element_size() == 2):
+        out_dtype = dtype if out is None else out.dtype
+    if out_dtype != dtype and not (out_dtype == torch.float32 and grad.element_size() == 2):
         raise TypeError("out dtype must be the dtype of grad, or float32 for float16 / bfloat16")
-    alpha = check_scalar(alpha, grad.dtype, "alpha")
-    beta = check_scalar(beta, grad.dtype, "beta")
+    alpha = _scalar(alpha, dtype, "alpha")
+    beta = _scalar(beta, dtype, "beta")
     has_ignore, ignore = _ignored(ignore_index)
-    _refuse_out(out, (grad,))
-    device = _check_device((("grad", grad), ("tokens", tokens), ("out", out)))
-    dim = grad.shape[-1]
+    if out is not None:
+        _refuse_out(out, grad)
+    index = _check_first_device(grad, "grad")
+    _check_same_device(tokens, "tokens", index, "grad")
+    _check_same_device(out, "out", index, "grad")
+    dim = shape[-1]
     n = tokens.numel()
     _check_size("the number of tokens", n, MAX_ENTRIES)
     _check_size("n_rows", n_rows, MAX_ROWS)
     _check_size("dim", dim, MAX_DIM)
-    result = _Result(out, (n_rows, dim), out_dtype, device, beta)
+    flat, address, pitch = _result(out, (n_rows, dim), grad, out_dtype, beta)
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
-    grad, flat = _rows(grad if grad.ndim == 2 else grad.reshape(n, dim)), result.flat
+    grad = _rows(grad if grad.dim() == 2 else grad.reshape(n, dim))
     lib = _lib.load()
-    vcode = _lib.VALUE_CODE[grad.dtype]
+    vcode = _lib.VALUE_CODE[dtype]
     nbytes = lib.b2s_select_grad_bytes(vcode, n, n_rows, dim)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    _call(device, lib.b2s_select_grad, vcode, _lib.VALUE_CODE[out_dtype],
+    ws = grad.new_empty(nbytes, dtype=torch.uint8)
+    _call(index, lib.b2s_select_grad, vcode, _lib.VALUE_CODE[out_dtype],
           _lib.INDEX_CODE[tokens.dtype], tokens.data_ptr(), n, has_ignore, ignore,
-          grad.data_ptr(), _pitch(grad), n_rows, dim, flat.data_ptr(), _pitch(flat), alpha, beta,
-          ws.data_ptr(), nbytes, _status_word(device.index))
-    return result.done(out)
+          grad.data_ptr(), _pitch(grad), n_rows, dim, address, pitch, alpha, beta,
+          ws.data_ptr(), nbytes, _status_word(index))
+    return flat if out is None else _finish(out, flat)
 
 
 class _Embedding(torch.autograd.Function):
@@ -320,7 +333,7 @@ class _Embedding(torch.autograd.Function):
     def forward(ctx, tokens, table, alpha, has_ignore, ignore):
         ctx.save_for_backward(tokens)
         ctx.args = (table.shape[0], alpha, ignore if has_ignore else None)
-        return _embedding(tokens, table, alpha, has_ignore, ignore, None, 0.0, table.device)
+        return _embedding(tokens, table, alpha, has_ignore, ignore, None, 0.0, table.get_device())
 
     @staticmethod
     @once_differentiable
@@ -346,27 +359,45 @@ class TokenRoute:
     have no row: the rows from indptr[-1] on belong to nobody and are kept zero.
     """
 
-    __slots__ = ("slots", "indptr", "indices", "n_tokens", "k", "n_experts", "device", "_stream")
+    __slots__ = ("n_tokens", "k", "n_experts", "n_rows", "device", "_index", "_buffer", "_address",
+                 "_held", "_stream", "_views")
 
-    def __init__(self, slots, indptr, indices, n_experts, stream):
-        self.slots, self.indptr, self.indices = slots, indptr, indices
-        self.n_tokens, self.k = slots.shape
-        self.n_experts = n_experts
-        self.device = slots.device
+    def __init__(self, buffer, n_tokens, k, n_experts, stream):
+        """`buffer` (int32): slots, indptr and indices one behind the other."""
+        self.n_tokens, self.k, self.n_experts = n_tokens, k, n_experts
+        self.n_rows = n_tokens * k      # of the sorted array, whatever is masked
+        self.device = buffer.device
+        self._index = buffer.get_device()
+        self._buffer = buffer
+        self._address = buffer.data_ptr()                            # of slots
+        self._held = self._address + 4 * (self.n_rows + n_experts)   # of indptr[-1]
         self._stream = stream
+        self._views = [None, None, None]
+
+    def _view(self, which, shape, stride, at):
+        view = self._views[which]
+        if view is None:
+            view = self._views[which] = self._buffer.as_strided(shape, stride, at)
+        return view
 
     @property
-    def n_rows(self):
-        """Rows of the sorted array: n_tokens * k, whatever is masked."""
-        return self.n_tokens * self.k
+    def slots(self):
+        return self._view(0, (self.n_tokens, self.k), (self.k, 1), 0)
+
+    @property
+    def indptr(self):
+        return self._view(1, (self.n_experts + 1,), (1,), self.n_rows)
+
+    @property
+    def indices(self):
+        return self._view(2, (self.n_rows,), (1,), self.n_rows + self.n_experts + 1)
 
     def _use(self):
         """Called before a launch: keeps the arrays from being reused while a stream other than
         the one they were made on still reads them."""
-        stream = torch.cuda.current_stream(self.device)
-        if stream.cuda_stream != self._stream and not torch.cuda.is_current_stream_capturing():
-            for t in (self.slots, self.indptr, self.indices):
-                t.record_stream(stream)
+        if _raw_stream(self._index) != self._stream:
+            if not torch.cuda.is_current_stream_capturing():
+                self._buffer.record_stream(torch.cuda.current_stream(self._index))
 
     def __repr__(self):
         return (f"TokenRoute(n_tokens={self.n_tokens}, k={self.k}, n_experts={self.n_experts}, "
@@ -377,27 +408,28 @@ def prepare_token_route(experts, n_experts):
     """Sort the assignments experts[t, j] (int32 / int64, -1: masked) by expert, keeping their
     order within an expert, and return the TokenRoute.  Nothing is read back to the host."""
     _check_ids(experts, "experts")
-    if experts.ndim != 2:
+    if experts.dim() != 2:
         raise ValueError("experts must be a 2D tensor: (n_tokens, k)")
     n_experts = _as_int(n_experts, "n_experts")
     if not 0 <= n_experts <= MAX_EXPERTS:
         raise ValueError(f"n_experts must be between 0 and {MAX_EXPERTS}, got {n_experts}")
     n_tokens, k = experts.shape
-    _check_size("n_tokens * k", n_tokens * k, MAX_ENTRIES)
-    device = _check_device((("experts", experts),))
+    n = n_tokens * k
+    _check_size("n_tokens * k", n, MAX_ENTRIES)
+    index = _check_first_device(experts, "experts")
     if not experts.is_contiguous():
         experts = experts.contiguous()
-    slots = torch.empty((n_tokens, k), dtype=torch.int32, device=device)
-    indptr = torch.empty(n_experts + 1, dtype=torch.int32, device=device)
-    indices = torch.empty(n_tokens * k, dtype=torch.int32, device=device)
     lib = _lib.load()
     nbytes = lib.b2s_route_plan_bytes(n_tokens, k, n_experts)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    _call(device, lib.b2s_route_plan, _lib.INDEX_CODE[experts.dtype], experts.data_ptr(), n_tokens,
-          k, n_experts, slots.data_ptr(), indptr.data_ptr(), indices.data_ptr(), ws.data_ptr(),
-          nbytes, _status_word(device.index))
-    return TokenRoute(slots, indptr, indices, n_experts,
-                      torch.cuda.current_stream(device).cuda_stream)
+    scratch = -(-(2 * n + n_experts + 1) // 64) * 64     # behind the arrays, 256-byte aligned
+    buffer = experts.new_empty(scratch + nbytes // 4, dtype=torch.int32)
+    stream = _raw_stream(index)
+    route = TokenRoute(buffer, n_tokens, k, n_experts, stream)
+    address = route._address
+    _call(index, lib.b2s_route_plan, _lib.INDEX_CODE[experts.dtype], experts.data_ptr(), n_tokens,
+          k, n_experts, address, address + 4 * n, route._held + 4, address + 4 * scratch, nbytes,
+          _status_word(index))
+    return route
 
 
 def _check_route(route):
@@ -407,7 +439,7 @@ def _check_route(route):
 
 def _check_matrix(t, name, rows, what):
     _check_values(t, name)
-    if t.ndim != 2:
+    if t.dim() != 2:
         raise ValueError(f"{name} must be a 2D tensor: ({what}, dim)")
     if t.shape[0] != rows:
         raise ValueError(f"{name}.shape[0] must be {what}={rows}, got {t.shape[0]}")
@@ -433,8 +465,11 @@ def flagsparse_token_dispatch(x, route, out=None):
     """
     _check_route(route)
     _check_matrix(x, "x", route.n_tokens, "n_tokens")
-    _refuse_out(out, (x,))
-    _check_device((("route", route.slots), ("x", x), ("out", out)))
+    if out is not None:
+        _refuse_out(out, x)
+    index = _check_first_device(route._buffer, "route")
+    _check_same_device(x, "x", index, "route")
+    _check_same_device(out, "out", index, "route")
     if _wants_grad(x):
         _refuse_capture()
         return _Dispatch.apply(x, route)
@@ -443,13 +478,12 @@ def flagsparse_token_dispatch(x, route, out=None):
 
 def _dispatch(x, route, out):
     dim = x.shape[1]
-    result = _Result(out, (route.n_rows, dim), x.dtype, route.device, 0.0)
-    x, flat = _rows(x), result.flat
+    flat, address, pitch = _result(out, (route.n_rows, dim), x, x.dtype, 0.0)
+    x = _rows(x)
     route._use()
-    _call(route.device, _lib.load().b2s_route_dispatch, _lib.VALUE_CODE[x.dtype], x.data_ptr(),
-          _pitch(x), route.n_tokens, route.k, dim, route.slots.data_ptr(),
-          route.indptr.data_ptr() + 4 * route.n_experts, flat.data_ptr(), _pitch(flat))
-    return result.done(out)
+    _call(route._index, _lib.load().b2s_route_dispatch, _lib.VALUE_CODE[x.dtype], x.data_ptr(),
+          _pitch(x), route.n_tokens, route.k, dim, route._address, route._held, address, pitch)
+    return flat if out is None else _finish(out, flat)
 
 
 def flagsparse_token_dispatch_grad(grad, route, out=None, beta=0.0):
@@ -460,9 +494,12 @@ def flagsparse_token_dispatch_grad(grad, route, out=None, beta=0.0):
     """
     _check_route(route)
     _check_matrix(grad, "grad", route.n_rows, "n_tokens * k")
-    beta = check_scalar(beta, grad.dtype, "beta")
-    _refuse_out(out, (grad,))
-    _check_device((("route", route.slots), ("grad", grad), ("out", out)))
+    beta = _scalar(beta, grad.dtype, "beta")
+    if out is not None:
+        _refuse_out(out, grad)
+    index = _check_first_device(route._buffer, "route")
+    _check_same_device(grad, "grad", index, "route")
+    _check_same_device(out, "out", index, "route")
     return _combine(grad, route, None, 1.0, out, beta)
 
 
@@ -477,31 +514,36 @@ def flagsparse_token_combine(y, route, weights=None, alpha=1.0, out=None, beta=0
     _check_route(route)
     _check_matrix(y, "y", route.n_rows, "n_tokens * k")
     _check_weights(weights, route, y.dtype)
-    alpha = check_scalar(alpha, y.dtype, "alpha")
-    beta = check_scalar(beta, y.dtype, "beta")
-    _refuse_out(out, (y, weights))
-    _check_device((("route", route.slots), ("y", y), ("weights", weights), ("out", out)))
+    alpha = _scalar(alpha, y.dtype, "alpha")
+    beta = _scalar(beta, y.dtype, "beta")
+    if out is not None:
+        _refuse_out(out, y, weights)
+    index = _check_first_device(route._buffer, "route")
+    _check_same_device(y, "y", index, "route")
+    _check_same_device(weights, "weights", index, "route")
+    _check_same_device(out, "out", index, "route")
     if _wants_grad(y, weights):
         _refuse_capture()
+        if beta != 0:
+            raise ValueError("beta != 0 requires out= holding the rows to scale")
         return _Combine.apply(y, weights, route, alpha)
     return _combine(y, route, weights, alpha, out, beta)
 
 
 def _combine(y, route, weights, alpha, out, beta):
     dim = y.shape[1]
-    result = _Result(out, (route.n_tokens, dim), y.dtype, route.device, beta)
-    y, flat = _rows(y), result.flat
-    wcode = 0
+    flat, address, pitch = _result(out, (route.n_tokens, dim), y, y.dtype, beta)
+    y = _rows(y)
+    wcode, waddress = 0, None
     if weights is not None:
         if not weights.is_contiguous():
             weights = weights.contiguous()
-        wcode = _lib.VALUE_CODE[weights.dtype]
+        wcode, waddress = _lib.VALUE_CODE[weights.dtype], weights.data_ptr()
     route._use()
-    _call(route.device, _lib.load().b2s_route_combine, _lib.VALUE_CODE[y.dtype], y.data_ptr(),
-          _pitch(y), route.slots.data_ptr(), wcode,
-          None if weights is None else weights.data_ptr(), route.n_tokens, route.k, dim,
-          flat.data_ptr(), _pitch(flat), alpha, beta)
-    return result.done(out)
+    _call(route._index, _lib.load().b2s_route_combine, _lib.VALUE_CODE[y.dtype], y.data_ptr(),
+          _pitch(y), route._address, wcode, waddress, route.n_tokens, route.k, dim, address, pitch,
+          alpha, beta)
+    return flat if out is None else _finish(out, flat)
 
 
 def flagsparse_token_combine_grad(grad, y, route, weights=None, alpha=1.0):
@@ -523,31 +565,33 @@ def flagsparse_token_combine_grad(grad, y, route, weights=None, alpha=1.0):
             raise TypeError("y dtype must match grad dtype")
         if y.shape[1] != grad.shape[1]:
             raise ValueError("y and grad must have the same number of columns")
-    alpha = check_scalar(alpha, grad.dtype, "alpha")
-    _check_device((("route", route.slots), ("grad", grad), ("y", y), ("weights", weights)))
+    alpha = _scalar(alpha, grad.dtype, "alpha")
+    index = _check_first_device(route._buffer, "route")
+    _check_same_device(grad, "grad", index, "route")
+    _check_same_device(y, "y", index, "route")
+    _check_same_device(weights, "weights", index, "route")
     return _combine_grad(grad, y, route, weights, alpha, weights is not None)
 
 
 def _combine_grad(grad, y, route, weights, alpha, want_weights):
     dim = grad.shape[1]
     grad = _rows(grad)
-    grad_y = torch.empty((route.n_rows, dim), dtype=grad.dtype, device=route.device)
-    grad_w, wcode = None, 0
+    grad_y = grad.new_empty((route.n_rows, dim))
+    grad_w, wcode, waddress, gaddress = None, 0, None, None
+    yaddress, ypitch = None, 0
     if weights is not None:
         if not weights.is_contiguous():
             weights = weights.contiguous()
-        wcode = _lib.VALUE_CODE[weights.dtype]
+        wcode, waddress = _lib.VALUE_CODE[weights.dtype], weights.data_ptr()
         if want_weights:
             y = _rows(y)
-            grad_w = torch.empty((route.n_tokens, route.k), dtype=weights.dtype,
-                                 device=route.device)
+            yaddress, ypitch = y.data_ptr(), _pitch(y)
+            grad_w = weights.new_empty((route.n_tokens, route.k))
+            gaddress = grad_w.data_ptr()
     route._use()
-    _call(route.device, _lib.load().b2s_route_combine_grad, _lib.VALUE_CODE[grad.dtype],
-          grad.data_ptr(), _pitch(grad), None if grad_w is None else y.data_ptr(),
-          0 if grad_w is None else _pitch(y), route.slots.data_ptr(),
-          route.indptr.data_ptr() + 4 * route.n_experts, wcode,
-          None if weights is None else weights.data_ptr(), route.n_tokens, route.k, dim, alpha,
-          grad_y.data_ptr(), dim, None if grad_w is None else grad_w.data_ptr())
+    _call(route._index, _lib.load().b2s_route_combine_grad, _lib.VALUE_CODE[grad.dtype],
+          grad.data_ptr(), _pitch(grad), yaddress, ypitch, route._address, route._held, wcode,
+          waddress, route.n_tokens, route.k, dim, alpha, grad_y.data_ptr(), dim, gaddress)
     return grad_y, grad_w
 
 

@@ -75,9 +75,17 @@ def test_route_refuses(args, error, message):
 
 def _route(n_tokens=3, k=2, n_experts=4):
     """A route on the CPU: enough for the checks in front of a launch."""
-    return fs.TokenRoute(torch.zeros(n_tokens, k, dtype=torch.int32),
-                         torch.zeros(n_experts + 1, dtype=torch.int32),
-                         torch.zeros(n_tokens * k, dtype=torch.int32), n_experts, 0)
+    buffer = torch.arange(2 * n_tokens * k + n_experts + 1, dtype=torch.int32)
+    return fs.TokenRoute(buffer, n_tokens, k, n_experts, 0)
+
+
+def test_route_arrays_are_views_of_one_buffer():
+    r = _route()
+    assert r.slots.tolist() == [[0, 1], [2, 3], [4, 5]] and r.slots is r.slots
+    assert r.indptr.tolist() == [6, 7, 8, 9, 10]
+    assert r.indices.tolist() == [11, 12, 13, 14, 15, 16]
+    assert (r.n_rows, r.n_tokens, r.k, r.n_experts) == (6, 3, 2, 4)
+    assert "n_tokens=3, k=2, n_experts=4" in repr(r)
 
 
 def test_route_operators_refuse():
@@ -112,25 +120,33 @@ def test_route_operators_refuse():
 
 def test_result_places():
     """out that the kernels can write is written in place; another layout gets a stand-in."""
-    f32, cpu = torch.float32, torch.device("cpu")
+    f32, like = torch.float32, torch.zeros(1)
     with pytest.raises(ValueError, match="beta != 0 requires out="):
-        selection._Result(None, (3, 4), f32, cpu, 1.0)
+        selection._result(None, (3, 4), like, f32, 1.0)
     for bad in (torch.zeros(4, 3), torch.zeros(3, 4).half()):
         with pytest.raises(ValueError, match="out shape/dtype must match result"):
-            selection._Result(bad, (3, 4), f32, cpu, 0.0)
-    wide = torch.zeros(3, 9)
-    r = selection._Result(wide[:, :4], (3, 4), f32, cpu, 0.0)
-    assert not r.stand_in and r.flat.data_ptr() == wide.data_ptr() and r.flat.stride(0) == 9
+            selection._result(bad, (3, 4), like, f32, 0.0)
+    flat, address, pitch = selection._result(None, (2, 3, 4), like, f32, 0.0)
+    assert flat.shape == (2, 3, 4) and address == flat.data_ptr() and pitch == 4
+    wide = torch.zeros(3, 9)[:, :4]
+    flat, address, pitch = selection._result(wide, (3, 4), like, f32, 0.0)
+    assert address == wide.data_ptr() and pitch == 9
+    version = wide._version
+    assert selection._finish(wide, flat) is wide and wide._version > version
     cols = torch.arange(12.0).reshape(4, 3).t()
-    r = selection._Result(cols, (3, 4), f32, cpu, 1.0)
-    assert r.stand_in and torch.equal(r.flat, cols)      # beta reads what is there
-    r.flat.zero_()
-    assert r.done(cols) is cols and not cols.any()
+    flat, address, pitch = selection._result(cols, (3, 4), like, f32, 1.0)
+    assert address != cols.data_ptr() and pitch == 4 and torch.equal(flat, cols)   # beta reads it
+    flat.zero_()
+    assert selection._finish(cols, flat) is cols and not cols.any()
     deep = torch.zeros(2, 3, 9)[:, :, :4]                # rows of one pitch: a view will do
-    r = selection._Result(deep, (2, 3, 4), f32, cpu, 0.0)
-    assert not r.stand_in and r.flat.shape == (6, 4) and r.flat.stride(0) == 9
+    flat, address, pitch = selection._result(deep, (2, 3, 4), like, f32, 0.0)
+    assert address == deep.data_ptr() and pitch == 9
     deep = torch.zeros(3, 2, 4).transpose(0, 1)
-    assert selection._Result(deep, (2, 3, 4), f32, cpu, 0.0).stand_in
+    flat, address, pitch = selection._result(deep, (2, 3, 4), like, f32, 0.0)
+    assert address != deep.data_ptr() and pitch == 4
+    for empty in (torch.zeros(0, 3, 4), torch.zeros(2, 3, 0)):
+        flat, _, _ = selection._result(empty, tuple(empty.shape), like, f32, 0.0)
+        assert selection._finish(empty, flat) is empty
 
 
 def test_c_entry_points_answer_before_any_launch():
@@ -170,72 +186,91 @@ def test_c_entry_points_answer_before_any_launch():
     assert back(w=None) == arg and back(y=None) == arg and back(wt=5) == dtype
 
 
-# ---- the tiles of the gradient: every entry is summed once, by one owner ---------------------------
-P = 32
+# ---- the ranges of the gradient: every entry is summed once, by one owner --------------------------
+CROSS = 32
 
 
-def _tiles(keys, none):
-    """The decisions of one warp per tile of 32 sorted entries (b2s_select.cu, grad_tile), and of
-    the kernel that joins long runs, on a list of sorted keys (`none`: masked)."""
-    n, rows, head, tail, runs = len(keys), {}, {}, {}, []
+def _first(n, below):
+    """The first index in [0, n) that `below` does not hold for, 32 places at a time."""
+    lo, length = 0, n
+    while length > 1:
+        step, end = -(-length // 32), lo + length
+        hits = sum(lo + i * step < end and below(lo + i * step) for i in range(32))
+        if hits == 0:
+            break
+        lo += (hits - 1) * step + 1
+        length = min(end - lo, step)
+    return lo
 
-    def key(i):
-        return keys[i] if 0 <= i < n else (0xffffffff if i < 0 else none)
 
-    tiles = -(-n // P)
-    for t in range(tiles):
-        at = t * P
-        cur, nxt, prv = ([key(at + d + i) for i in range(P)] for d in (0, P, -P))
-        valid = sum(c < none for c in cur)
-        if not valid:
-            continue
-        before, last, after = prv[-1], cur[valid - 1], nxt[0]
-        in_head, in_prev = cur.count(before), prv.count(before)
-        in_tail, in_next = cur.count(last), nxt.count(last)
-        head_ends = in_head < P or after != before
-        head_began = in_prev < P or key(at - P - 1) != before
-        goes_on = valid == P and after == last
-        tail_begins = in_tail < P or before != last
-        tail_ends = in_next < P or key(at + 2 * P) != last
-        own_head = in_head > 0 and not (head_ends and head_began)
-        lo = in_head if in_head > 0 and not own_head else 0
-        long_tail = goes_on and tail_begins and not tail_ends
-        hi = valid + (in_next if goes_on and tail_begins and tail_ends else 0)
-        if lo < hi and long_tail:
-            runs.append(t)
-        acc = []
+def _held(keys, none):
+    if keys[-1] < none:
+        return len(keys)
+    lo, length = 0, len(keys)
+    while length > 0:
+        step, end = -(-length // 32), lo + length
+        hits = sum(lo + i * step < end and keys[lo + i * step] < none for i in range(32))
+        if hits == 0:
+            break
+        lo += (hits - 1) * step + 1
+        length = min(end - lo, step - 1)
+    return lo
+
+
+def _ranges(keys, none, most):
+    """The decisions of the warps that sum ranges of the sorted entries, and of the kernel that
+    joins the runs they cut (b2s_select.cu); `none`: masked."""
+    m = _held(keys, none)
+    assert m == sum(k < none for k in keys)
+    if m == 0:
+        return {}, 0
+    size = max(8, -(-m // most))
+    rows, head, tail, runs = {}, {}, {}, []
+
+    def crossing(x):
+        if x <= 0 or x >= m:
+            return 0
+        return sum(x + i < m and keys[x + i] == keys[x - 1] for i in range(CROSS))
+
+    for r in range(-(-m // size)):
+        a, b = r * size, min((r + 1) * size, m)
+        into, out = crossing(a), crossing(b)
+        lo = a + (0 if into == CROSS else into)
+        hi = b + (0 if out == CROSS else out)
+        first, acc = into == CROSS, []
         for i in range(lo, hi):
-            k = cur[i] if i < P else last
-            acc.append(at + i)
-            if i + 1 >= hi or (cur[i + 1] if i + 1 < P else last) != k:
-                part = head if own_head and i < in_head else tail if long_tail and i + 1 == hi else None
-                where = (rows, k) if part is None else (part, t)
-                assert where[1] not in where[0]
-                where[0][where[1]], acc = acc, []
-    for first in runs:
-        k, lo, hi = keys[first * P + P - 1], first + 1, tiles - 1
-        while lo < hi:
-            mid = (lo + hi + 1) // 2
-            lo, hi = (mid, hi) if keys[mid * P] <= k else (lo, mid - 1)
-        assert k not in rows
-        rows[k] = sum((tail.pop(t) if t == first else head.pop(t) for t in range(first, lo + 1)), [])
+            acc.append(i)
+            if i + 1 < hi and keys[i + 1] == keys[i]:
+                continue
+            goes_on = out == CROSS and i + 1 == hi
+            where, name = (head, r) if first else (tail, r) if goes_on else (rows, keys[i])
+            assert name not in where
+            where[name], acc = acc, []
+            if first and not goes_on:
+                runs.append((_first(lo, lambda j: keys[j] < keys[i]) // size, r, keys[i]))
+            first = False
+    for begin, end, key in runs:
+        assert key not in rows
+        rows[key] = sum((tail.pop(r) if r == begin else head.pop(r)
+                         for r in range(begin, end + 1)), [])
     assert not head and not tail
     return rows, len(runs)
 
 
-def test_gradient_tiles_cover_every_entry_once():
+def test_gradient_ranges_cover_every_entry_once():
     rng = random.Random(3)
-    long_runs = 0
+    cut = 0
     for _ in range(3000):
-        none, n = rng.choice([1, 2, 5, 50]), rng.choice([1, 31, 32, 33, 64, 65, 97, 130, 300])
+        none = rng.choice([1, 2, 5, 50])
+        n = rng.choice([1, 7, 8, 9, 31, 32, 33, 40, 64, 65, 97, 130, 700, 2000])
         hot = rng.choice([0.1, 0.9])
         keys = sorted(min(none, int(rng.expovariate(1.0))) if rng.random() < hot
                       else rng.randrange(none + 1) for _ in range(n))
-        rows, runs = _tiles(keys, none)
-        long_runs += runs
+        rows, runs = _ranges(keys, none, rng.choice([1, 2, 3, 10, n, n // 24 + 1]))
+        cut += runs
         want = {}
         for i, k in enumerate(keys):
             if k < none:
                 want.setdefault(k, []).append(i)
         assert rows == want
-    assert long_runs > 100
+    assert cut > 100

@@ -208,6 +208,8 @@ PATTERNS = {
     "same": (torch.zeros(1000, dtype=torch.long) + 2, 5),
     "tiles": (runs(31, 1, 32, 33, 31, 64, 1, 63, 65, 62, 96, 97, 95, 2, 300), 20),
     "whole tiles": (runs(32, 32, 64, 96, 32, 1), 6),
+    "short tiles": (runs(7, 1, 8, 9, 7, 15, 16, 17, 1, 24, 23, 25, 2, 40), 20),
+    "half tiles": (runs(15, 1, 16, 17, 15, 31, 32, 33, 1, 47, 48, 49, 2, 80), 20),
     "long": (runs(1, 4000, 3, 2500, 33), 7),
     "even": (torch.from_numpy(np.random.default_rng(1).integers(0, 900, 2000)), 900),
     "one chunk": (torch.from_numpy(np.random.default_rng(2).integers(0, 5000, 4096)), 5000),
@@ -221,10 +223,13 @@ PATTERNS = {
     (torch.float32, torch.float32, 8), (torch.float32, torch.float32, 33),
     (torch.bfloat16, torch.bfloat16, 264), (torch.bfloat16, torch.float32, 40),
     (torch.float16, torch.float16, 7), (torch.float16, torch.float32, 257),
+    (torch.bfloat16, torch.bfloat16, 4104), (torch.float32, torch.float32, 2052),
     (torch.float64, torch.float64, 12), (torch.float64, torch.float64, 5)], ids=ids)
 def test_embedding_grad(pattern, dtype, out_dtype, dim):
     tokens, vocab = PATTERNS[pattern]
     n = tokens.numel()
+    if n * dim > 1 << 24 or vocab * dim > 1 << 24:
+        dim = 392                                    # the wide rows: what the CPU sums in a second
     g = randn(n, dim, dtype=dtype, seed=n)
     tok = tokens.cuda()
     got = fs.flagsparse_embedding_grad(tok, g, vocab, out_dtype=out_dtype)
