@@ -540,6 +540,7 @@ select_grad_kernel(GradRuns runs, int64_t ranges, unsigned sum_blocks, unsigned 
                    const T* __restrict__ grad, int64_t ld_grad, GradOut<T, O> to,
                    const uint8_t* __restrict__ named) {
   extern __shared__ int4 smem4[];
+  follow();
   const int warp = threadIdx.x >> 5;
   const unsigned b = blockIdx.x, rest = gridDim.x - sum_blocks;
   const unsigned both = 2 * (sum_blocks < rest ? sum_blocks : rest);
@@ -585,6 +586,7 @@ __global__ void __launch_bounds__(32 * kLongWarps, sizeof(T) == 8 ? 2 : 3)
 select_grad_long_kernel(GradOut<T, O> to, bool has_beta) {
   using A = typename acc_of<T>::type;
   __shared__ A sums[kLongWarps][E][32];
+  follow();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int count = *to.long_count;
   int4 run = to.long_list[blockIdx.x];  // (there is room for gridDim.x entries)
@@ -972,16 +974,17 @@ int select_grad_go(const GradRuns& runs, const T* grad, int64_t ld_grad,
   if (sums + rest == 0) return B2S_OK;
   auto kernel = &select_grad_kernel<T, O, VE, kBeta>;
   if (smem > 0) ensure_dyn_smem(reinterpret_cast<const void*>(kernel), smem);
-  kernel<<<static_cast<unsigned>(sums + rest), kSelThreads, smem, s>>>(
-      runs, ranges, static_cast<unsigned>(sums), static_cast<unsigned>(slabs), grad, ld_grad, to,
-      named);
+  B2S_TRY(launch_behind(kernel, dim3(static_cast<unsigned>(sums + rest)), kSelThreads, smem, s, runs,
+                        ranges, static_cast<unsigned>(sums), static_cast<unsigned>(slabs), grad,
+                        ld_grad, to, named));
   if (runs.n > kCross) {  // a run that is cut goes on for kCross entries behind a border
     constexpr int kCols = VE > 1 && sizeof(T) == 8 ? 4 : 8;
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>(ranges, 128)),
                     static_cast<unsigned>(ceil_div(to.dim, 32 * kCols)));
-    select_grad_long_kernel<T, O, VE, kCols><<<grid, 32 * kLongWarps, 0, s>>>(to, kBeta);
+    return launch_behind(&select_grad_long_kernel<T, O, VE, kCols>, grid, 32 * kLongWarps, 0, s, to,
+                         kBeta);
   }
-  return launch_status();
+  return B2S_OK;
 }
 
 template <class T, class O>

@@ -89,6 +89,33 @@ struct PlanOut {  // token route: slot of each assignment, token of each slot, f
   }
 };
 
+// ---- kernels of one call that follow each other -------------------------------------------------
+// Each is put in place while the one before it still runs (programmatic dependent launch), which
+// hides its launch.  Every thread calls follow() before it touches memory: it returns when the
+// kernel before has ended and its writes are visible.
+__device__ inline void follow() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+// launches `kernel`, which calls follow(), behind another kernel of the same call
+template <class... Params, class... Args>
+int launch_behind(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t st,
+                  const Args&... args) {
+  cudaLaunchAttribute early;
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = grid;
+  config.blockDim = dim3(static_cast<unsigned>(threads));
+  config.dynamicSmemBytes = smem;
+  config.stream = st;
+  config.attrs = &early;
+  config.numAttrs = 1;
+  return cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...) == cudaSuccess
+             ? launch_status()
+             : B2S_ERR_LAUNCH;
+}
+
 // ---- device pieces of a pass ---------------------------------------------------------------------
 // counts the digits of entries [lo, hi) into hist[bins] (shared, zeroed by the caller)
 template <class Key>
@@ -202,6 +229,7 @@ sort_count_kernel(Key key, int64_t n, int64_t chunk, int shift, int bins, int* _
                   uint8_t* __restrict__ clear, int64_t n_clear, int32_t* counter) {
   extern __shared__ int4 smem4[];
   int* hist = reinterpret_cast<int*>(smem4);
+  follow();
   for (int b = threadIdx.x; b < bins; b += kSortThreads) hist[b] = 0;
   __syncthreads();
   const int64_t lo = blockIdx.x * chunk, hi = lo + chunk < n ? lo + chunk : n;
@@ -222,6 +250,7 @@ sort_place_kernel(Key key, const int32_t* __restrict__ vals, Out out, int64_t n,
                   int shift, int bins, const int* __restrict__ counts) {
   extern __shared__ int4 smem4[];
   __shared__ int warp_tot[kSortWarps];
+  follow();
   int* off = reinterpret_cast<int*>(smem4);
   int* before = off + bins;  // off_next until the first tile
   uint16_t* cnt = reinterpret_cast<uint16_t*>(before + bins);
@@ -263,6 +292,7 @@ sort_one_kernel(Key key, Out out, int64_t n, int bits, int passes, BufferOut buf
                 uint8_t* __restrict__ clear, int64_t n_clear, int32_t* counter) {
   extern __shared__ int4 smem4[];
   __shared__ int warp_tot[kSortWarps];
+  follow();
   const int bins = 1 << bits;
   int* off = reinterpret_cast<int*>(smem4);
   int* next = off + bins;
@@ -351,26 +381,31 @@ int sort_ids(const IdKeys<I>& ids, int64_t n, const Out& out, uint8_t* clear, in
   auto place = [&](const auto& key, const int32_t* vals, const auto& to, int shift) {
     auto kernel = &sort_place_kernel<std::decay_t<decltype(key)>, std::decay_t<decltype(to)>>;
     ensure_dyn_smem(reinterpret_cast<const void*>(kernel), sort_smem(kSortMaxBins));
-    kernel<<<grid, kSortThreads, smem, st>>>(key, vals, to, n, s.chunk, shift, s.bins, counts);
+    return launch_behind(kernel, grid, kSortThreads, smem, st, key, vals, to, n, s.chunk, shift,
+                         s.bins, counts);
   };
   sort_count_kernel<<<grid, kSortThreads, s.bins * sizeof(int), st>>>(
       ids, n, s.chunk, 0, s.bins, counts, clear, n_clear, counter);
+  int status = launch_status();
+  if (status != B2S_OK) return status;
   if constexpr (Out::kOnePass) {
-    place(ids, nullptr, out, 0);
+    status = place(ids, nullptr, out, 0);
   } else {
-    if (s.passes == 1) place(ids, nullptr, out, 0);
-    else place(ids, nullptr, buf[0], 0);
+    status = s.passes == 1 ? place(ids, nullptr, out, 0) : place(ids, nullptr, buf[0], 0);
     for (int p = 1; p < s.passes; ++p) {
       const BufferOut& from = (p & 1) ? buf[0] : buf[1];
       const StoredKeys stored{from.keys};
-      sort_count_kernel<<<grid, kSortThreads, s.bins * sizeof(int), st>>>(
-          stored, n, s.chunk, p * s.bits, s.bins, counts, static_cast<uint8_t*>(nullptr),
-          int64_t(0), static_cast<int32_t*>(nullptr));
-      if (p + 1 == s.passes) place(stored, from.vals, out, p * s.bits);
-      else place(stored, from.vals, (p & 1) ? buf[1] : buf[0], p * s.bits);
+      if (status == B2S_OK)
+        status = launch_behind(&sort_count_kernel<StoredKeys>, grid, kSortThreads,
+                               s.bins * sizeof(int), st, stored, n, s.chunk, p * s.bits, s.bins,
+                               counts, nullptr, 0, nullptr);
+      if (status == B2S_OK)
+        status = p + 1 == s.passes
+                     ? place(stored, from.vals, out, p * s.bits)
+                     : place(stored, from.vals, (p & 1) ? buf[1] : buf[0], p * s.bits);
     }
   }
-  return launch_status();
+  return status;
 }
 
 }  // namespace b2s
