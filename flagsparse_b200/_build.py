@@ -4,7 +4,7 @@
 library.  Objects are rebuilt only when a source or header is newer.  nvcc cross-compiles without
 a GPU, so this also runs on a CPU-only machine.
 
-Two more libraries come from the same sources:
+Three more libraries:
 
 * ``libb200sparse_checked.so`` (``build(checked=True)``, ``--checked``): compiled with
   ``-DB2S_CHECKED``; every column index and row pointer a kernel reads from the matrix is
@@ -12,6 +12,9 @@ Two more libraries come from the same sources:
   device status word instead of touching memory.  Slower; stands in for a memory checker when
   raw C-ABI callers pass matrices nobody validated.  ``B200SPARSE_CHECKED=1`` makes
   ``flagsparse_b200._lib`` load it.
+* ``_b2s_host.so`` (``build_host()``, part of ``python -m flagsparse_b200._build``): a CPython
+  module over PyTorch's C++ headers that makes the usual call of the selection products without
+  Python's share of the time; nothing in it runs on the device.
 * ``libb2sprobe.so`` (``build_probe()``, ``--probe``): the gather-rate probe ``bench.py`` times;
   not part of the product library.
 """
@@ -31,6 +34,7 @@ BUILD_DIR = PKG_DIR / "csrc" / "build"
 LIB_PATH = PKG_DIR / "libb200sparse.so"
 CHECKED_LIB_PATH = PKG_DIR / "libb200sparse_checked.so"
 PROBE_LIB_PATH = PKG_DIR / "libb2sprobe.so"
+HOST_LIB_PATH = PKG_DIR / "_b2s_host.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -92,6 +96,33 @@ def build(force: bool = False, verbose: bool = False, extra_flags=(), checked: b
     return lib_path
 
 
+def build_host(force: bool = False, verbose: bool = False) -> Path:
+    """_b2s_host.so from csrc/host/b2s_host.cpp (host code only; needs PyTorch's headers)."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    src = CSRC / "host" / "b2s_host.cpp"
+    header = PKG_DIR.parent / "include" / "b200sparse.h"
+    if force or _newer(HOST_LIB_PATH, [src, header]):
+        torch_lib = Path(torch.__file__).resolve().parent / "lib"
+        cuda_include = Path(_nvcc()).resolve().parent.parent / "include"
+        includes = [*cpp_extension.include_paths(), str(cuda_include),
+                    sysconfig.get_paths()["include"]]
+        cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+               "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+               *(f"-isystem{path}" for path in includes), str(src), "-o", str(HOST_LIB_PATH),
+               f"-L{torch_lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda",
+               "-lc10_cuda", "-lc10"]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        res = subprocess.run(cmd, capture_output=True, text=True)
+        if res.returncode != 0:
+            raise RuntimeError(f"g++ failed on {src.name}:\n{res.stdout}\n{res.stderr}")
+    return HOST_LIB_PATH
+
+
 def build_probe(force: bool = False) -> Path:
     """libb2sprobe.so from csrc/probe/b2s_probe.cu (measurement aid of bench.py)."""
     src = CSRC / "probe" / "b2s_probe.cu"
@@ -108,5 +139,7 @@ if __name__ == "__main__":
                  extra_flags=("-Xptxas", "-v") if "--ptxas" in sys.argv else (),
                  checked="--checked" in sys.argv)
     print(path)
+    if "--checked" not in sys.argv:
+        print(build_host(force="--force" in sys.argv, verbose=True))
     if "--probe" in sys.argv:
         print(build_probe(force="--force" in sys.argv))

@@ -1101,7 +1101,8 @@ extern "C" int b2s_route_plan(int idx_type, const void* experts_dev, int64_t n_t
   const int64_t n = n_tokens * k;
   if (n > 0 && (!experts_dev || !slots_dev || !indices_dev)) return B2S_ERR_ARG;
   if (n > 0 && !aligned_to(experts_dev, isize(idx_type))) return B2S_ERR_ALIGNMENT;
-  if (!ws_dev || ws_bytes < sort_bytes(n, n_experts)) return B2S_ERR_WORKSPACE;
+  const int64_t need = sort_bytes(n, n_experts);
+  if (ws_bytes < need || (need > 0 && !ws_dev)) return B2S_ERR_WORKSPACE;
   if (!aligned_to(ws_dev, 256)) return B2S_ERR_ALIGNMENT;
   B2S_DISPATCH_I(idx_type, I, {
     const IdKeys<I> ids{static_cast<const I*>(experts_dev), static_cast<uint32_t>(n_experts),

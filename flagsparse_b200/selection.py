@@ -43,6 +43,25 @@ MAX_ENTRIES = 2**31 - 1 - 2**25  # positions are int32
 MAX_ROWS = 2**31 - 2
 MAX_DIM = 1 << 22
 
+
+# The usual call (plain strided tensors, a new result, nothing to record) is made by a C++ module
+# (csrc/host/b2s_host.cpp): it returns None for every other one, which then takes the way below.
+# Without the module all calls do; the kernels are the same.
+def _load_host():
+    try:
+        from . import _b2s_host
+    except ImportError:
+        return None
+    lib = _lib.load()
+    address = [ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+        "b2s_select_rows", "b2s_select_grad_bytes", "b2s_select_grad", "b2s_route_plan_bytes",
+        "b2s_route_plan", "b2s_route_dispatch", "b2s_route_combine", "b2s_route_combine_grad")]
+    _b2s_host.bind(*address, torch.nn.Parameter, torch.OutOfMemoryError)
+    return _b2s_host
+
+
+_host = _load_host() if _lib.LIB_PATH.exists() else None
+
 _WORDS = {}
 _WORDS_LOCK = threading.Lock()
 
@@ -73,6 +92,8 @@ def _status_word(index):
             word = _WORDS.get(index)
             if word is None:
                 word = _WORDS[index] = _StatusWord()
+                if _host is not None:
+                    _host.bind_status(index, word.address)
     word.check()
     return word.address
 
@@ -237,6 +258,10 @@ def flagsparse_embedding(tokens, table, alpha=1.0, ignore_index=None, out=None, 
     alpha, beta are numbers; beta != 0 needs `out`.
     Differentiable in `table` (a dense gradient, see flagsparse_embedding_grad).
     """
+    if _host is not None and out is None and type(beta) in (float, int) and beta == 0:
+        result = _host.embedding(tokens, table, alpha, ignore_index)
+        if result is not None:
+            return result
     _check_ids(tokens, "tokens")
     _check_values(table, "table")
     if table.dim() != 2:
@@ -286,6 +311,11 @@ def flagsparse_embedding_grad(tokens, grad, n_rows, alpha=1.0, ignore_index=None
     The tokens are sorted, and the rows of one token are summed in float32 (float64) in a fixed
     order: the result is the same from run to run.
     """
+    if _host is not None:
+        result = _host.embedding_grad(tokens, grad, n_rows, alpha, ignore_index, out, beta,
+                                      out_dtype)
+        if result is not None:
+            return result
     _check_ids(tokens, "tokens")
     _check_values(grad, "grad")
     n_rows = _as_int(n_rows, "n_rows")
@@ -359,23 +389,37 @@ class TokenRoute:
     have no row: the rows from indptr[-1] on belong to nobody and are kept zero.
     """
 
-    __slots__ = ("n_tokens", "k", "n_experts", "n_rows", "device", "_index", "_buffer", "_address",
-                 "_held", "_stream", "_views")
+    __slots__ = ("n_tokens", "k", "n_experts", "_buffer", "_stream", "_views")
 
     def __init__(self, buffer, n_tokens, k, n_experts, stream):
         """`buffer` (int32): slots, indptr and indices one behind the other."""
         self.n_tokens, self.k, self.n_experts = n_tokens, k, n_experts
-        self.n_rows = n_tokens * k      # of the sorted array, whatever is masked
-        self.device = buffer.device
-        self._index = buffer.get_device()
-        self._buffer = buffer
-        self._address = buffer.data_ptr()                            # of slots
-        self._held = self._address + 4 * (self.n_rows + n_experts)   # of indptr[-1]
-        self._stream = stream
-        self._views = [None, None, None]
+        self._buffer, self._stream = buffer, stream
+        self._views = {}
+
+    @property
+    def n_rows(self):
+        """Rows of the sorted array: n_tokens * k, whatever is masked."""
+        return self.n_tokens * self.k
+
+    @property
+    def device(self):
+        return self._buffer.device
+
+    @property
+    def _index(self):
+        return self._buffer.get_device()
+
+    @property
+    def _address(self):     # of slots
+        return self._buffer.data_ptr()
+
+    @property
+    def _held(self):        # of indptr[-1]
+        return self._buffer.data_ptr() + 4 * (self.n_tokens * self.k + self.n_experts)
 
     def _view(self, which, shape, stride, at):
-        view = self._views[which]
+        view = self._views.get(which)
         if view is None:
             view = self._views[which] = self._buffer.as_strided(shape, stride, at)
         return view
@@ -407,6 +451,11 @@ class TokenRoute:
 def prepare_token_route(experts, n_experts):
     """Sort the assignments experts[t, j] (int32 / int64, -1: masked) by expert, keeping their
     order within an expert, and return the TokenRoute.  Nothing is read back to the host."""
+    if _host is not None:
+        made = _host.route_plan(experts, n_experts)
+        if made is not None:
+            n_tokens, k = experts.shape
+            return TokenRoute(made[0], n_tokens, k, n_experts, made[1])
     _check_ids(experts, "experts")
     if experts.dim() != 2:
         raise ValueError("experts must be a 2D tensor: (n_tokens, k)")
@@ -464,6 +513,11 @@ def flagsparse_token_dispatch(x, route, out=None):
     route.indptr[-1] on (left by masked assignments) zero.  Differentiable in x.
     """
     _check_route(route)
+    if _host is not None and out is None:
+        result = _host.dispatch(route._buffer, route.n_tokens, route.k, route.n_experts,
+                                route._stream, x)
+        if result is not None:
+            return result
     _check_matrix(x, "x", route.n_tokens, "n_tokens")
     if out is not None:
         _refuse_out(out, x)
@@ -493,6 +547,11 @@ def flagsparse_token_dispatch_grad(grad, route, out=None, beta=0.0):
     grad: (n_tokens * k, dim); its rows from route.indptr[-1] on are not read.
     """
     _check_route(route)
+    if _host is not None and out is None and type(beta) in (float, int) and beta == 0:
+        result = _host.combine(route._buffer, route.n_tokens, route.k, route.n_experts,
+                               route._stream, grad, None, 1.0)
+        if result is not None:
+            return result
     _check_matrix(grad, "grad", route.n_rows, "n_tokens * k")
     beta = _scalar(beta, grad.dtype, "beta")
     if out is not None:
@@ -512,6 +571,11 @@ def flagsparse_token_combine(y, route, weights=None, alpha=1.0, out=None, beta=0
     assignments are all masked gets beta * out.  Differentiable in y and weights.
     """
     _check_route(route)
+    if _host is not None and out is None and type(beta) in (float, int) and beta == 0:
+        result = _host.combine(route._buffer, route.n_tokens, route.k, route.n_experts,
+                               route._stream, y, weights, alpha)
+        if result is not None:
+            return result
     _check_matrix(y, "y", route.n_rows, "n_tokens * k")
     _check_weights(weights, route, y.dtype)
     alpha = _scalar(alpha, y.dtype, "alpha")
@@ -554,6 +618,11 @@ def flagsparse_token_combine_grad(grad, y, route, weights=None, alpha=1.0):
     dtype of weights, zero where masked.  Without weights, y may be None and grad_weights is None.
     """
     _check_route(route)
+    if _host is not None and weights is not None:
+        result = _host.combine_grad(route._buffer, route.n_tokens, route.k, route.n_experts,
+                                    route._stream, grad, y, weights, alpha)
+        if result is not None:
+            return result
     _check_matrix(grad, "grad", route.n_tokens, "n_tokens")
     _check_weights(weights, route, grad.dtype)
     if weights is not None:

@@ -118,6 +118,29 @@ def test_route_operators_refuse():
         fs.flagsparse_token_combine(y.requires_grad_(), r, out=torch.zeros(3, 4))
 
 
+def test_the_host_module_is_built_and_leaves_what_it_does_not_take():
+    """It makes the usual calls on CUDA tensors; for any other it answers None."""
+    host = selection._host
+    assert host is not None, "_b2s_host.so not built (python -m flagsparse_b200._build)"
+    r = _route()
+    parts = (r._buffer, r.n_tokens, r.k, r.n_experts, r._stream)
+    x, y = torch.zeros(3, 4), torch.zeros(6, 4)
+    assert host.embedding(TOK, TABLE, 1.0, None) is None
+    assert host.embedding(None, TABLE, 1.0, None) is None
+    assert host.embedding(TOK, TABLE, 1.0) is None
+    assert host.embedding(TOK, TABLE, "1", 2**70) is None
+    assert host.embedding_grad(TOK, x, 5, 1.0, None, None, 0.0, None) is None
+    assert host.embedding_grad(TOK, x, -5, 1.0, None, None, 0.0, "float") is None
+    assert host.route_plan(TOK[None], 4) is None and host.route_plan(TOK, 4.0) is None
+    assert host.dispatch(*parts, x) is None and host.dispatch(x) is None
+    assert host.combine(*parts, y, None, 1.0) is None
+    assert host.combine_grad(*parts, x, y, torch.zeros(3, 2), 1.0) is None
+    with pytest.raises(TypeError):
+        host.bind(1, 2)
+    with pytest.raises(TypeError):
+        host.bind_status("0", 1)
+
+
 def test_result_places():
     """out that the kernels can write is written in place; another layout gets a stand-in."""
     f32, like = torch.float32, torch.zeros(1)
@@ -171,7 +194,7 @@ def test_c_entry_points_answer_before_any_launch():
     plan = lambda i=1, e=d, t=4, k=2, n=8, b=1 << 30: lib.b2s_route_plan(  # noqa: E731
         i, e, t, k, n, d, d, d, d, b, None, None)
     assert plan(i=2) == dtype and plan(e=None) == arg and plan(n=-1) == arg
-    assert plan(n=2048) == rng and plan(t=2**31, k=2) == rng and plan(b=0) == ws
+    assert plan(n=2048) == rng and plan(t=2**31, k=2) == rng and plan(t=4000, b=0) == ws
     assert plan(e=ctypes.c_void_p(4100)) == align
     disp = lambda v=0, x=d, s=d, h=d, t=4, ld=8: lib.b2s_route_dispatch(  # noqa: E731
         v, x, ld, t, 2, 8, s, h, d, 8, None)

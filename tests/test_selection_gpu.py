@@ -15,8 +15,19 @@ import pytest
 import torch
 
 import flagsparse_b200 as fs
+from flagsparse_b200 import selection
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True, params=["host module", "python"])
+def way(request, monkeypatch):
+    """Every test runs with the calls made by the C++ host module and by the Python code."""
+    if request.param == "python":
+        monkeypatch.setattr(selection, "_host", None)
+    else:
+        assert selection._host is not None
+    return request.param
 
 TYPES = [torch.float16, torch.bfloat16, torch.float32, torch.float64]
 HALF_STEP = {torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8, torch.float32: 2.0**-24,
