@@ -2,10 +2,12 @@
 // expert (token route).  Least significant digit first; one digit of up to 11 bits per pass, so
 // that a route needs one pass and a vocabulary of 2^17 rows two.
 //
-// A pass cuts the list into at most 128 chunks, one CTA each.  The first kernel counts the
-// digits of each chunk; the second sums those counts itself (every CTA reads the whole
-// chunks x digits table, which L2 holds) and places its entries in order.  A list of one chunk
-// needs one launch for all passes: the CTA counts, places and goes on to the next digit.
+// A list of up to 16384 entries is sorted in one launch by a cluster of eight CTAs (up to 1024: by
+// one CTA), which read each other's digit counts through distributed shared memory.  On one SM
+// alone the scattered stores are the limit: 16384 entries in two passes took 64 us there, and
+// take 19 us on eight.  The passes of a longer list cut it into at most 128 chunks, one CTA each.
+// The first kernel counts the digits of each chunk; the second sums those counts itself (every CTA
+// reads the whole chunks x digits table, which L2 holds) and places its entries in order.
 #pragma once
 #include <type_traits>
 
@@ -18,7 +20,10 @@ constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kSortRounds = 2;                           // entries per thread and tile
 constexpr int kSortTile = kSortThreads * kSortRounds;
 constexpr int kSortMaxChunks = 128;
-constexpr int kSortOneChunk = 4 * kSortTile;             // lists up to this: one CTA, one launch
+constexpr int kTeamThreads = 1024;                       // CTAs of a cluster that sorts alone
+constexpr int kTeamWarps = kTeamThreads / 32;
+constexpr int kTeamCtas = 8;
+constexpr int64_t kTeamMost = 2 * kTeamThreads * kTeamCtas;
 constexpr int kSortMaxBits = 11;
 constexpr int kSortMaxBins = 1 << kSortMaxBits;
 constexpr int64_t kSortMaxEntries = 0x7fffffff - (1 << 25);  // positions are int32
@@ -131,13 +136,15 @@ __device__ inline void sort_count(const Key& key, int64_t lo, int64_t hi, int sh
   }
 }
 
-// exclusive prefix sum of v[bins] (shared) in place; thread t holds bins t * 4 .. t * 4 + 3
+// exclusive prefix sum of v[bins] (shared) in place, by kThreads threads; bins <= kSortMaxBins
+template <int kThreads>
 __device__ inline void sort_scan(int* v, int bins, int* warp_tot) {
+  constexpr int kPer = kSortMaxBins / kThreads;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int c[4], run = 0;
+  int c[kPer], run = 0;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int b = threadIdx.x * 4 + q;
+  for (int q = 0; q < kPer; ++q) {
+    const int b = threadIdx.x * kPer + q;
     c[q] = b < bins ? v[b] : 0;
     run += c[q];
   }
@@ -148,15 +155,30 @@ __device__ inline void sort_scan(int* v, int bins, int* warp_tot) {
   }
   if (lane == 31) warp_tot[warp] = inc;
   __syncthreads();
-  int at = inc - run;
-  for (int w = 0; w < warp; ++w) at += warp_tot[w];
+  int in_front = lane < warp ? warp_tot[lane] : 0;
+  for (int o = 16; o > 0; o >>= 1) in_front += __shfl_xor_sync(0xffffffffu, in_front, o);
+  int at = in_front + inc - run;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int b = threadIdx.x * 4 + q;
+  for (int q = 0; q < kPer; ++q) {
+    const int b = threadIdx.x * kPer + q;
     if (b < bins) v[b] = at;
     at += c[q];
   }
   __syncthreads();
+}
+
+// Rank of the lane's entry among those of the warp so far that have the same digit (0xffffffff:
+// no entry); `mine` counts them.
+__device__ inline int sort_rank(unsigned digit, uint16_t* mine) {
+  const unsigned peers = __match_any_sync(0xffffffffu, digit);
+  const int before = __popc(peers & ((1u << (threadIdx.x & 31)) - 1u));
+  const bool live = digit != 0xffffffffu;
+  int prev = 0;
+  if (live) prev = mine[digit];
+  __syncwarp();
+  if (live && before == 0) mine[digit] = static_cast<uint16_t>(prev + __popc(peers));
+  __syncwarp();
+  return prev + before;
 }
 
 // Places entries [lo, hi) in order; off[b] is where the next entry with digit b goes.  A warp
@@ -179,15 +201,7 @@ __device__ inline void sort_place(const Key& key, const int32_t* vals, const Out
       const int64_t i = t0 + (warp * kSortRounds + q) * 32 + lane;
       const bool live = i < hi;
       k[q] = live ? key(i) : 0;
-      const unsigned d = live ? (k[q] >> shift) & (bins - 1) : 0xffffffffu;
-      const unsigned peers = __match_any_sync(0xffffffffu, d);
-      const int before = __popc(peers & ((1u << lane) - 1u));
-      int prev = 0;
-      if (live) prev = mine[d];
-      __syncwarp();
-      if (live && before == 0) mine[d] = static_cast<uint16_t>(prev + __popc(peers));
-      __syncwarp();
-      rank[q] = prev + before;
+      rank[q] = sort_rank(live ? (k[q] >> shift) & (bins - 1) : 0xffffffffu, mine);
     }
     __syncthreads();
     for (int b = threadIdx.x; b < bins; b += kSortThreads) {
@@ -275,7 +289,7 @@ sort_place_kernel(Key key, const int32_t* __restrict__ vals, Out out, int64_t n,
     atomicAdd(before + 4 * quad + 2, pre.z); atomicAdd(before + 4 * quad + 3, pre.w);
   }
   __syncthreads();
-  sort_scan(off, bins, warp_tot);
+  sort_scan<kSortThreads>(off, bins, warp_tot);
   for (int b = threadIdx.x; b < bins; b += kSortThreads) {
     if (blockIdx.x == 0) out.first(b, off[b]);
     off[b] += before[b];
@@ -285,51 +299,132 @@ sort_place_kernel(Key key, const int32_t* __restrict__ vals, Out out, int64_t n,
   sort_place(key, vals, out, lo, hi, shift, bins, off, before, cnt);
 }
 
-// a list of one chunk: all passes in one CTA (passes alternate between buf[0] and buf[1])
-template <class Key, class Out>
-__global__ void __launch_bounds__(kSortThreads)
-sort_one_kernel(Key key, Out out, int64_t n, int bits, int passes, BufferOut buf0, BufferOut buf1,
-                uint8_t* __restrict__ clear, int64_t n_clear, int32_t* counter) {
+// All CTAs of the cluster, and their memory accesses before it
+__device__ inline void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+// *p of the CTA `rank` of the cluster (p: shared memory here, the same place there)
+__device__ inline int cluster_load(const int* p, unsigned rank) {
+  uint32_t at;
+  int v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_addr(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
+
+// A list that a cluster sorts (gridDim.x CTAs, all of one cluster).  CTA c takes `chunk` entries,
+// its warps stretches of kRounds * 32, 32 in a round, so that (CTA, warp, round, lane) is the
+// order of the list.  The counters of the warps are summed per digit in place, those of the CTAs
+// through distributed shared memory.
+template <class Key, class Out, int kRounds>
+__global__ void __launch_bounds__(kTeamThreads)
+sort_team_kernel(Key key, Out out, int n, int chunk, int bits, int passes, BufferOut buf0,
+                 BufferOut buf1, uint8_t* __restrict__ clear, int64_t n_clear, int32_t* counter) {
   extern __shared__ int4 smem4[];
-  __shared__ int warp_tot[kSortWarps];
+  __shared__ int warp_tot[kTeamWarps];
   follow();
-  const int bins = 1 << bits;
+  const int bins = 1 << bits, warp = threadIdx.x >> 5;
+  const unsigned me = blockIdx.x, ctas = gridDim.x;
   int* off = reinterpret_cast<int*>(smem4);
-  int* next = off + bins;
-  uint16_t* cnt = reinterpret_cast<uint16_t*>(next + bins);
-  for (int64_t i = threadIdx.x; i < (n_clear + 15) / 16; i += kSortThreads)
+  int* total = off + bins;                                     // of this CTA, read by the others
+  uint32_t* cnt2 = reinterpret_cast<uint32_t*>(total + bins);  // two 16-bit counters a word
+  uint16_t* mine = reinterpret_cast<uint16_t*>(cnt2) + warp * bins;
+  const int lo = static_cast<int>(me) * chunk, hi = n - lo < chunk ? n : lo + chunk;
+  const int first = lo + warp * (kRounds * 32) + (threadIdx.x & 31);  // entry of round 0
+  for (int64_t i = me * kTeamThreads + threadIdx.x; i < (n_clear + 15) / 16;
+       i += ctas * kTeamThreads)
     reinterpret_cast<uint4*>(clear)[i] = make_uint4(0, 0, 0, 0);
-  if (counter && threadIdx.x == 0) *counter = 0;
+  if (counter && me == 0 && threadIdx.x == 0) *counter = 0;
   for (int p = 0; p < passes; ++p) {
-    const BufferOut& from = (p & 1) ? buf0 : buf1;  // pass p reads what pass p - 1 wrote
-    const BufferOut& to = (p & 1) ? buf1 : buf0;
     const int shift = p * bits;
-    for (int b = threadIdx.x; b < bins; b += kSortThreads) off[b] = 0;
+    const BufferOut& from = (p & 1) ? buf0 : buf1;  // pass p reads what pass p - 1 wrote
+    auto digit = [&](uint32_t key_) { return (key_ >> shift) & (bins - 1); };
+    uint32_t k[kRounds];
+    int place[kRounds];
+#pragma unroll
+    for (int q = 0; q < kRounds; ++q) {
+      const int i = first + 32 * q;
+      k[q] = 0;
+      if (i < hi) {
+        if (p == 0) k[q] = key(i);
+        else if constexpr (!Out::kOnePass) k[q] = __ldcg(from.keys + i);
+      }
+    }
+    for (int i = threadIdx.x; i < kTeamWarps * bins / 2; i += kTeamThreads) cnt2[i] = 0;
     __syncthreads();
-    if (p == 0) {
-      sort_count(key, 0, n, shift, bins, off);
-    } else if constexpr (!Out::kOnePass) {
-      sort_count(StoredKeys{from.keys}, 0, n, shift, bins, off);
+#pragma unroll
+    for (int q = 0; q < kRounds; ++q)
+      place[q] = sort_rank(first + 32 * q < hi ? digit(k[q]) : 0xffffffffu, mine);
+    __syncthreads();
+    for (int b = threadIdx.x; b < bins / 2; b += kTeamThreads) {
+      uint32_t run = 0;
+#pragma unroll 8
+      for (int w = 0; w < kTeamWarps; ++w) {
+        const uint32_t c = cnt2[w * (bins / 2) + b];
+        cnt2[w * (bins / 2) + b] = run;
+        run += c;
+      }
+      total[2 * b] = run & 0xffff;
+      total[2 * b + 1] = run >> 16;
+    }
+    cluster_barrier();
+    int before[kSortMaxBins / kTeamThreads];
+#pragma unroll
+    for (int u = 0; u < kSortMaxBins / kTeamThreads; ++u) {
+      const int b = threadIdx.x + u * kTeamThreads;
+      before[u] = 0;
+      if (b < bins) {
+        int all = 0;
+        for (unsigned c = 0; c < ctas; ++c) {
+          const int v = cluster_load(total + b, c);
+          all += v;
+          if (c < me) before[u] += v;
+        }
+        off[b] = all;
+      }
     }
     __syncthreads();
-    sort_scan(off, bins, warp_tot);
+    sort_scan<kTeamThreads>(off, bins, warp_tot);
     const bool last = p + 1 == passes;
-    if (last)
-      for (int b = threadIdx.x; b < bins; b += kSortThreads) out.first(b, off[b]);
-    if (p == 0 && last) sort_place(key, nullptr, out, 0, n, shift, bins, off, next, cnt);
-    if constexpr (!Out::kOnePass) {
-      const StoredKeys stored{from.keys};
-      if (p == 0 && !last) sort_place(key, nullptr, to, 0, n, shift, bins, off, next, cnt);
-      if (p > 0 && last) sort_place(stored, from.vals, out, 0, n, shift, bins, off, next, cnt);
-      if (p > 0 && !last) sort_place(stored, from.vals, to, 0, n, shift, bins, off, next, cnt);
+#pragma unroll
+    for (int u = 0; u < kSortMaxBins / kTeamThreads; ++u) {
+      const int b = threadIdx.x + u * kTeamThreads;
+      if (b < bins) {
+        if (last && me == 0) out.first(b, off[b]);
+        off[b] += before[u];
+      }
     }
     __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kRounds; ++q) {
+      const int i = first + 32 * q;
+      if (i < hi) {
+        const int dst = place[q] + off[digit(k[q])] + mine[digit(k[q])];
+        int32_t val = i;
+        if constexpr (!Out::kOnePass) {
+          if (p > 0) val = __ldcg(from.vals + i);
+          if (!last) ((p & 1) ? buf1 : buf0)(k[q], val, dst);
+        }
+        if (last) out(k[q], val, dst);
+      }
+    }
+    // what was placed is read by other CTAs; no CTA may end, or count anew, while its counts are read
+    cluster_barrier();
   }
+}
+
+// flags that are too many for the cluster
+__global__ void __launch_bounds__(256) sort_clear_kernel(uint4* p, int64_t n) {
+  const int64_t i = blockIdx.x * 256LL + threadIdx.x;
+  if (i < n) p[i] = make_uint4(0, 0, 0, 0);
 }
 
 // ---- host ----------------------------------------------------------------------------------------
 struct SortShape {
   int passes, bits, bins;
+  bool team;  // sorted by one cluster
+  int lists;  // (key, value) lists between passes
   int64_t chunk, chunks;
 };
 inline SortShape sort_shape(int64_t n, int64_t n_keys) {
@@ -339,21 +434,44 @@ inline SortShape sort_shape(int64_t n, int64_t n_keys) {
   s.passes = (width + kSortMaxBits - 1) / kSortMaxBits;
   s.bits = (width + s.passes - 1) / s.passes;
   s.bins = 1 << s.bits;
-  if (n <= kSortOneChunk) {
-    s.chunk = kSortOneChunk;
-    s.chunks = 1;
-  } else {
-    const int64_t tiles = (n + kSortTile - 1) / kSortTile;
-    s.chunk = (tiles + kSortMaxChunks - 1) / kSortMaxChunks * kSortTile;
-    s.chunks = (n + s.chunk - 1) / s.chunk;
-  }
+  s.lists = s.passes > 2 ? 2 : s.passes - 1;
+  s.team = n <= kTeamMost;
+  const int64_t tiles = (n + kSortTile - 1) / kSortTile;
+  s.chunk = (tiles + kSortMaxChunks - 1) / kSortMaxChunks * kSortTile;
+  s.chunks = s.team ? 0 : (n + s.chunk - 1) / s.chunk;
   return s;
 }
-// scratch: two (key, value) lists between passes, and the table of counts
+// scratch: the lists between passes, and the table of counts
 inline int64_t sort_bytes(int64_t n, int64_t n_keys) {
   const SortShape s = sort_shape(n, n_keys);
-  const int lists = s.passes > 2 ? 2 : s.passes - 1;
-  return lists * 2 * align256(n * 4) + (s.chunks > 1 ? align256(s.chunks * s.bins * 4) : 0);
+  return s.lists * 2 * align256(n * 4) + align256(s.chunks * s.bins * 4);
+}
+
+template <class Key, class Out, int kRounds>
+int sort_team(const Key& key, int64_t n, const Out& out, const SortShape& s, const BufferOut* buf,
+              uint8_t* clear, int64_t n_clear, int32_t* counter, cudaStream_t st) {
+  auto kernel = &sort_team_kernel<Key, Out, kRounds>;
+  auto smem = [](int bins) {
+    return bins * (2 * sizeof(int) + kTeamWarps * sizeof(uint16_t));
+  };
+  ensure_dyn_smem(reinterpret_cast<const void*>(kernel), smem(kSortMaxBins));
+  const unsigned ctas = n <= kTeamThreads ? 1 : kTeamCtas;
+  cudaLaunchAttribute cluster;
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim = {ctas, 1, 1};
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(ctas);
+  config.blockDim = dim3(kTeamThreads);
+  config.dynamicSmemBytes = smem(s.bins);
+  config.stream = st;
+  config.attrs = &cluster;
+  config.numAttrs = 1;
+  const int64_t step = 32 * kRounds;
+  const int chunk = static_cast<int>((n + ctas * step - 1) / (ctas * step) * step);
+  return cudaLaunchKernelEx(&config, kernel, key, out, static_cast<int>(n), chunk, s.bits, s.passes,
+                            buf[0], buf[1], clear, n_clear, counter) == cudaSuccess
+             ? launch_status()
+             : B2S_ERR_LAUNCH;
 }
 
 // Sorts ids 0 .. n - 1 into `out`; zeroes clear[0 .. n_clear) (padded to 16) and *counter before
@@ -362,21 +480,26 @@ template <class I, class Out>
 int sort_ids(const IdKeys<I>& ids, int64_t n, const Out& out, uint8_t* clear, int64_t n_clear,
              int32_t* counter, unsigned char* ws, cudaStream_t st) {
   const SortShape s = sort_shape(n, ids.n_keys);
-  const int lists = s.passes > 2 ? 2 : s.passes - 1;
   BufferOut buf[2] = {{nullptr, nullptr}, {nullptr, nullptr}};
-  for (int b = 0; b < lists; ++b) {
+  for (int b = 0; b < s.lists; ++b) {
     buf[b].keys = reinterpret_cast<uint32_t*>(ws); ws += align256(n * 4);
     buf[b].vals = reinterpret_cast<int32_t*>(ws); ws += align256(n * 4);
   }
+  if (s.team) {
+    if (n_clear > (1 << 20)) {
+      const int64_t words = (n_clear + 15) / 16;
+      sort_clear_kernel<<<static_cast<unsigned>((words + 255) / 256), 256, 0, st>>>(
+          reinterpret_cast<uint4*>(clear), words);
+      const int status = launch_status();
+      if (status != B2S_OK) return status;
+      n_clear = 0;
+    }
+    auto go = [&](auto run) { return run(ids, n, out, s, buf, clear, n_clear, counter, st); };
+    if (n <= kTeamThreads * kTeamCtas) return go(&sort_team<IdKeys<I>, Out, 1>);
+    return go(&sort_team<IdKeys<I>, Out, 2>);
+  }
   int* counts = reinterpret_cast<int*>(ws);
   const size_t smem = sort_smem(s.bins);
-  if (s.chunks == 1) {
-    ensure_dyn_smem(reinterpret_cast<const void*>(&sort_one_kernel<IdKeys<I>, Out>),
-                    sort_smem(kSortMaxBins));
-    sort_one_kernel<IdKeys<I>, Out><<<1, kSortThreads, smem, st>>>(
-        ids, out, n, s.bits, s.passes, buf[0], buf[1], clear, n_clear, counter);
-    return launch_status();
-  }
   const unsigned grid = static_cast<unsigned>(s.chunks);
   auto place = [&](const auto& key, const int32_t* vals, const auto& to, int shift) {
     auto kernel = &sort_place_kernel<std::decay_t<decltype(key)>, std::decay_t<decltype(to)>>;

@@ -224,6 +224,10 @@ PATTERNS = {
     "long": (runs(1, 4000, 3, 2500, 33), 7),
     "even": (torch.from_numpy(np.random.default_rng(1).integers(0, 900, 2000)), 900),
     "one chunk": (torch.from_numpy(np.random.default_rng(2).integers(0, 5000, 4096)), 5000),
+    "team of one": (torch.from_numpy(np.random.default_rng(5).zipf(1.3, 1024) % 30000), 30000),
+    "team": (torch.from_numpy(np.random.default_rng(5).zipf(1.3, 1025) % 30000), 30000),
+    "full team": (torch.from_numpy(np.random.default_rng(6).zipf(1.3, 16384) % 30000), 30000),
+    "no team": (torch.from_numpy(np.random.default_rng(7).zipf(1.3, 16385) % 30000), 30000),
     "two passes": (torch.from_numpy(np.random.default_rng(3).zipf(1.2, 9001) % 40000), 40000),
     "many chunks": (torch.from_numpy(np.random.default_rng(4).zipf(1.1, 140001) % 3000), 3000),
 }
@@ -290,7 +294,7 @@ def test_embedding_grad_masked_tokens(n, ignore):
 def test_embedding_grad_three_digit_vocabulary():
     """A vocabulary of more than 2^22 rows is sorted in three passes."""
     vocab = (1 << 22) + 1000
-    for n in (100, 10000):
+    for n in (100, 5000, 10000, 17000):
         tokens = torch.randint(0, vocab, (n,), device="cuda")
         tokens[:3] = torch.tensor([vocab - 1, 0, vocab - 1])
         g = randn(n, 4)
@@ -348,7 +352,8 @@ def plain_route(experts, n_experts):
     return slots.reshape(experts.shape), indptr, order // max(experts.shape[1], 1)
 
 
-ROUTES = [(1, 1, 1, 0.0), (1, 8, 8, 0.0), (7, 3, 5, 0.3), (64, 8, 256, 0.0), (100, 2, 2047, 0.1),
+ROUTES = [(1, 1, 1, 0.0), (1024, 1, 9, 0.1), (1025, 1, 9, 0.1), (1024, 4, 500, 0.0), (8192, 1, 70, 0.2),
+          (8193, 1, 64, 0.2), (8192, 2, 2047, 0.0), (16385, 2, 2047, 0.1), (1, 8, 8, 0.0), (7, 3, 5, 0.3), (64, 8, 256, 0.0), (100, 2, 2047, 0.1),
           (513, 8, 3, 0.0), (2100, 2, 64, 0.05), (16384, 1, 128, 0.0), (17000, 8, 60, 0.1),
           (50, 40, 64, 0.0), (6, 4, 10, 1.0), (0, 4, 10, 0.0), (5, 0, 10, 0.0)]
 
