@@ -276,19 +276,19 @@ select_rows_kernel(IdKeys<I> ids, int64_t n, const T* __restrict__ table, int64_
 // as a partial row, and select_grad_long_kernel adds the pieces in order.  No floating-point
 // atomics: the sums have one order whatever the scheduling.
 struct GradRuns {
-  const uint32_t* keys;  // sorted tokens; the masked ones at the end
-  const int32_t* vals;   // their positions
+  const Entry* list;  // tokens and their positions, sorted; the masked ones at the end
   int64_t n;
   uint32_t n_keys;
+  __device__ uint32_t key(int64_t i) const { return list[i].key; }
 };
 // how many entries are not masked (made by whole warps)
 __device__ inline int64_t grad_held(const GradRuns& runs) {
-  if (runs.keys[runs.n - 1] < runs.n_keys) return runs.n;
+  if (runs.key(runs.n - 1) < runs.n_keys) return runs.n;
   int64_t lo = 0, len = runs.n;  // the answer is in [lo, lo + len)
   while (len > 0) {
     const int64_t step = (len + 31) / 32, end = lo + len;
     const int64_t at = lo + (threadIdx.x & 31) * step;
-    const int hits = __popc(__ballot_sync(0xffffffffu, at < end && runs.keys[at] < runs.n_keys));
+    const int hits = __popc(__ballot_sync(0xffffffffu, at < end && runs.key(at) < runs.n_keys));
     if (hits == 0) break;
     lo += (hits - 1) * step + 1;  // the entry in front of lo is held
     len = end - lo < step - 1 ? end - lo : step - 1;
@@ -315,12 +315,12 @@ struct GradRanges {
 constexpr int kCross = 32;
 __device__ inline int grad_crossing(const GradRuns& runs, int64_t m, int64_t x) {
   if (x <= 0 || x >= m) return 0;
-  const uint32_t key = runs.keys[x - 1];
+  const uint32_t key = runs.key(x - 1);
   int n = 0;
 #pragma unroll
   for (int q = 0; q < kCross / 32; ++q) {
     const int64_t i = x + 32 * q + (threadIdx.x & 31);
-    n += __popc(__ballot_sync(0xffffffffu, i < m && runs.keys[i] == key));
+    n += __popc(__ballot_sync(0xffffffffu, i < m && runs.key(i) == key));
   }
   return n;
 }
@@ -368,7 +368,7 @@ template <class T, class O> struct GradOut {
     int64_t lo = 0, len = g.lo;  // its first entry is in [lo, lo + len)
     while (len > 1) {
       const int64_t step = (len + 31) / 32, end = lo + len, at = lo + lane * step;
-      const int below = __popc(__ballot_sync(0xffffffffu, at < end && runs.keys[at] < key));
+      const int below = __popc(__ballot_sync(0xffffffffu, at < end && runs.key(at) < key));
       if (below == 0) break;  // it is the entry at lo
       lo += (below - 1) * step + 1;
       len = end - lo < step ? end - lo : step;
@@ -405,14 +405,15 @@ __device__ inline void grad_sum(const GradRuns& runs, const GradRange& g,
   Rows rows(warp_smem);
   Olds olds(warp_smem + Rows::kWarpBytes);  // not touched unless kBeta
   const int lane = threadIdx.x & 31, dim = to.dim;
-  const uint32_t* keys = runs.keys + g.lo;
-  const int32_t* vals = runs.vals + g.lo;
+  const Entry* list = runs.list + g.lo;
   const int count = static_cast<int>(g.hi - g.lo);
-  auto key_of = [&](int i) { return i < count ? keys[i] : 0xffffffffu; };
-  auto pos_of = [&](int i) { return i < count ? vals[i] : 0; };
+  auto entry = [&](int i) { return i < count ? list[i] : Entry{0xffffffffu, 0}; };
 
-  int ask = 0, ask_pos = pos_of(lane), next_pos = pos_of(32 + lane);
-  uint32_t sum_keys = key_of(lane), next_keys = key_of(32 + lane);
+  // the stretch that rows are asked for from and the one behind it; the keys of the stretch that
+  // is summed and of the one behind it
+  const Entry e0 = entry(lane), e1 = entry(32 + lane);
+  int ask = 0, ask_pos = e0.pos, next_pos = e1.pos;
+  uint32_t sum_keys = e0.key, next_keys = e1.key;
   uint32_t sum_ends = run_ends(sum_keys, next_keys);
   uint32_t ask_keys = sum_keys, ask_next = next_keys, ask_ends = sum_ends;
   bool ask_head = g.head, sum_head = g.head;
@@ -432,11 +433,12 @@ __device__ inline void grad_sum(const GradRuns& runs, const GradRange& g,
     if constexpr (kBeta) olds.skip();
     ++ask;
     if ((ask & 31) == 0) {
+      const Entry e = entry(ask + 32 + lane);
       ask_pos = next_pos;
-      next_pos = pos_of(ask + 32 + lane);
+      next_pos = e.pos;
       if constexpr (kBeta) {
         ask_keys = ask_next;
-        ask_next = key_of(ask + 32 + lane);
+        ask_next = e.key;
         ask_ends = run_ends(ask_keys, ask_next);
       }
     }
@@ -461,7 +463,7 @@ __device__ inline void grad_sum(const GradRuns& runs, const GradRange& g,
     if constexpr (kBeta) olds.done();
     if (at == 31) {
       sum_keys = next_keys;
-      next_keys = key_of(i + 33 + lane);
+      next_keys = entry(i + 33 + lane).key;
       sum_ends = run_ends(sum_keys, next_keys);
     }
   }
@@ -485,10 +487,11 @@ __device__ inline void grad_sum_plain(const GradRuns& runs, const GradRange& g,
   acc.clear();
   bool head = g.head;
   for (int64_t c = g.lo; c < g.hi; c += 32) {
-    const uint32_t keys = c + lane < g.hi ? runs.keys[c + lane] : 0xffffffffu;
-    const uint32_t next = c + 32 + lane < g.hi ? runs.keys[c + 32 + lane] : 0xffffffffu;
-    const int pos = c + lane < g.hi ? runs.vals[c + lane] : 0;
-    const uint32_t ends = run_ends(keys, next);
+    const Entry none{0xffffffffu, 0};
+    const Entry e = c + lane < g.hi ? runs.list[c + lane] : none;
+    const Entry f = c + 32 + lane < g.hi ? runs.list[c + 32 + lane] : none;
+    const uint32_t keys = e.key, ends = run_ends(e.key, f.key);
+    const int pos = e.pos;
     const int m = g.hi - c < 32 ? static_cast<int>(g.hi - c) : 32;
     for (int i0 = 0; i0 < m; i0 += kAhead) {
       Part<T, 1> r[kAhead];
@@ -909,7 +912,7 @@ inline int64_t grad_ranges(int64_t n, int64_t slabs, int64_t ctas_per_sm) {
   return std::max<int64_t>(std::max(most, least), 1);
 }
 struct GradLayout {
-  int64_t keys, vals, words, head, tail, named, end;
+  int64_t list, words, head, tail, named, end;
   int64_t ranges;  // partial rows there is room for
 };
 // words: the number of cut runs, the list of them
@@ -920,8 +923,7 @@ inline GradLayout grad_layout(int vtype, int64_t n, int64_t n_rows, int64_t dim)
   l.ranges = grad_ranges(n, slabs > 0 ? slabs : 1, kQueueCtas);
   const int64_t part = align256(l.ranges * dim * static_cast<int64_t>(acc_size(vtype)));
   int64_t at = sort_bytes(n, n_rows);
-  l.keys = at; at += align256(n * 4);
-  l.vals = at; at += align256(n * 4);
+  l.list = at; at += align256(n * static_cast<int64_t>(sizeof(Entry)));
   l.words = at; at += align256((l.ranges + 1) * 16);
   l.head = at; at += part;
   l.tail = at; at += part;
@@ -1060,16 +1062,15 @@ extern "C" int b2s_select_grad(int val_type, int out_type, int idx_type, const v
   if (!aligned_to(ws_dev, 256)) return B2S_ERR_ALIGNMENT;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   unsigned char* ws = static_cast<unsigned char*>(ws_dev);
-  uint32_t* keys = reinterpret_cast<uint32_t*>(ws + l.keys);
-  int32_t* vals = reinterpret_cast<int32_t*>(ws + l.vals);
+  Entry* list = reinterpret_cast<Entry*>(ws + l.list);
   int32_t* words = reinterpret_cast<int32_t*>(ws + l.words);
   B2S_DISPATCH_I(idx_type, I, {
     const IdKeys<I> ids{static_cast<const I*>(idx_dev), static_cast<uint32_t>(n_rows),
                         has_ignore != 0, ignore, status};
-    const RunsOut sink{keys, vals, ws + l.named, static_cast<uint32_t>(n_rows)};
+    const RunsOut sink{list, ws + l.named, static_cast<uint32_t>(n_rows)};
     B2S_TRY(sort_ids(ids, n, sink, ws + l.named, n_rows, words, ws, s));
   });
-  const GradRuns runs{keys, vals, n, static_cast<uint32_t>(n_rows)};
+  const GradRuns runs{list, n, static_cast<uint32_t>(n_rows)};
   if (out_type == val_type) {
     B2S_DISPATCH_REAL(val_type, return (select_grad_run<T, T>(runs, grad_dev, ld_grad, dim,
                                                               out_dev, ld_out, alpha, beta, ws,

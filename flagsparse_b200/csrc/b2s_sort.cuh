@@ -51,31 +51,41 @@ template <class I> struct IdKeys {
   }
 };
 
-struct StoredKeys {
-  const uint32_t* keys;
-  __device__ uint32_t operator()(int64_t i) const { return keys[i]; }
+// A sorted entry: its key and its position in the caller's list.  The two are stored together: the
+// scattered stores are what a pass waits for.
+struct __align__(8) Entry {
+  uint32_t key;
+  int32_t pos;
+};
+__device__ inline Entry load_entry(const Entry* p) {
+  const uint2 v = __ldcg(reinterpret_cast<const uint2*>(p));
+  return {v.x, static_cast<int32_t>(v.y)};
+}
+
+// Where a pass takes its entries from: the caller's ids, or the list of the pass before.
+template <class I> struct FromIds {
+  IdKeys<I> key;
+  __device__ Entry operator()(int64_t i) const { return {key(i), static_cast<int32_t>(i)}; }
+};
+struct FromList {
+  const Entry* list;
+  __device__ Entry operator()(int64_t i) const { return load_entry(list + i); }
 };
 
 // ---- where the sorted entries go ---------------------------------------------------------------
-struct BufferOut {  // between two passes
-  uint32_t* keys;
-  int32_t* vals;
-  __device__ void operator()(uint32_t key, int32_t val, int dst) const {
-    keys[dst] = key;
-    vals[dst] = val;
-  }
+struct ListOut {  // between two passes
+  Entry* list;
+  __device__ void operator()(Entry e, int dst) const { list[dst] = e; }
   __device__ void first(int, int) const {}
 };
 struct RunsOut {  // embedding gradient: the sorted list, and which rows are named at all
   static constexpr bool kOnePass = false;
-  uint32_t* keys;
-  int32_t* vals;
+  Entry* list;
   uint8_t* named;
   uint32_t n_keys;
-  __device__ void operator()(uint32_t key, int32_t val, int dst) const {
-    keys[dst] = key;
-    vals[dst] = val;
-    if (key < n_keys) named[key] = 1;
+  __device__ void operator()(Entry e, int dst) const {
+    list[dst] = e;
+    if (e.key < n_keys) named[e.key] = 1;
   }
   __device__ void first(int, int) const {}
 };
@@ -85,9 +95,9 @@ struct PlanOut {  // token route: slot of each assignment, token of each slot, f
   int32_t* indptr;
   int32_t* indices;
   uint32_t n_experts, k;
-  __device__ void operator()(uint32_t key, int32_t val, int dst) const {
-    slots[val] = key < n_experts ? dst : -1;
-    indices[dst] = static_cast<int32_t>(static_cast<uint32_t>(val) / k);
+  __device__ void operator()(Entry e, int dst) const {
+    slots[e.pos] = e.key < n_experts ? dst : -1;
+    indices[dst] = static_cast<int32_t>(static_cast<uint32_t>(e.pos) / k);
   }
   __device__ void first(int bin, int at) const {
     if (bin <= static_cast<int>(n_experts)) indptr[bin] = at;
@@ -123,14 +133,14 @@ int launch_behind(void (*kernel)(Params...), dim3 grid, int threads, size_t smem
 
 // ---- device pieces of a pass ---------------------------------------------------------------------
 // counts the digits of entries [lo, hi) into hist[bins] (shared, zeroed by the caller)
-template <class Key>
-__device__ inline void sort_count(const Key& key, int64_t lo, int64_t hi, int shift, int bins,
+template <class From>
+__device__ inline void sort_count(const From& from, int64_t lo, int64_t hi, int shift, int bins,
                                   int* hist) {
   const int lane = threadIdx.x & 31;
   for (int64_t i0 = lo; i0 < hi; i0 += kSortThreads) {
     const int64_t i = i0 + threadIdx.x;
     unsigned d = 0xffffffffu;
-    if (i < hi) d = (key(i) >> shift) & (bins - 1);
+    if (i < hi) d = (from(i).key >> shift) & (bins - 1);
     const unsigned peers = __match_any_sync(0xffffffffu, d);
     if (i < hi && (peers & ((1u << lane) - 1u)) == 0) atomicAdd(hist + d, __popc(peers));
   }
@@ -184,24 +194,23 @@ __device__ inline int sort_rank(unsigned digit, uint16_t* mine) {
 // Places entries [lo, hi) in order; off[b] is where the next entry with digit b goes.  A warp
 // takes 32 neighbouring entries per round: those with the same digit are ranked by lane, the
 // rounds and warps of a tile by the counters cnt[warp][digit], tiles by off.
-template <class Key, class Out>
-__device__ inline void sort_place(const Key& key, const int32_t* vals, const Out& out, int64_t lo,
-                                  int64_t hi, int shift, int bins, int* off, int* off_next,
-                                  uint16_t* cnt) {
+template <class From, class Out>
+__device__ inline void sort_place(const From& from, const Out& out, int64_t lo, int64_t hi,
+                                  int shift, int bins, int* off, int* off_next, uint16_t* cnt) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int64_t t0 = lo; t0 < hi; t0 += kSortTile) {
     uint32_t* z = reinterpret_cast<uint32_t*>(cnt);
     for (int i = threadIdx.x; i < kSortWarps * bins / 2; i += kSortThreads) z[i] = 0;
     __syncthreads();
-    uint32_t k[kSortRounds];
+    Entry e[kSortRounds];
     int rank[kSortRounds];
     uint16_t* mine = cnt + warp * bins;
 #pragma unroll
     for (int q = 0; q < kSortRounds; ++q) {
       const int64_t i = t0 + (warp * kSortRounds + q) * 32 + lane;
       const bool live = i < hi;
-      k[q] = live ? key(i) : 0;
-      rank[q] = sort_rank(live ? (k[q] >> shift) & (bins - 1) : 0xffffffffu, mine);
+      if (live) e[q] = from(i);
+      rank[q] = sort_rank(live ? (e[q].key >> shift) & (bins - 1) : 0xffffffffu, mine);
     }
     __syncthreads();
     for (int b = threadIdx.x; b < bins; b += kSortThreads) {
@@ -219,8 +228,8 @@ __device__ inline void sort_place(const Key& key, const int32_t* vals, const Out
     for (int q = 0; q < kSortRounds; ++q) {
       const int64_t i = t0 + (warp * kSortRounds + q) * 32 + lane;
       if (i < hi) {
-        const int d = (k[q] >> shift) & (bins - 1);
-        out(k[q], vals ? vals[i] : static_cast<int32_t>(i), off[d] + mine[d] + rank[q]);
+        const int d = (e[q].key >> shift) & (bins - 1);
+        out(e[q], off[d] + mine[d] + rank[q]);
       }
     }
     int* swap = off;
@@ -237,9 +246,9 @@ inline size_t sort_smem(int bins) {
 
 // ---- kernels -------------------------------------------------------------------------------------
 // counts[chunk][digit]; the CTAs also zero `clear` (flags of the caller) and *counter
-template <class Key>
+template <class From>
 __global__ void __launch_bounds__(kSortThreads)
-sort_count_kernel(Key key, int64_t n, int64_t chunk, int shift, int bins, int* __restrict__ counts,
+sort_count_kernel(From from, int64_t n, int64_t chunk, int shift, int bins, int* __restrict__ counts,
                   uint8_t* __restrict__ clear, int64_t n_clear, int32_t* counter) {
   extern __shared__ int4 smem4[];
   int* hist = reinterpret_cast<int*>(smem4);
@@ -247,7 +256,7 @@ sort_count_kernel(Key key, int64_t n, int64_t chunk, int shift, int bins, int* _
   for (int b = threadIdx.x; b < bins; b += kSortThreads) hist[b] = 0;
   __syncthreads();
   const int64_t lo = blockIdx.x * chunk, hi = lo + chunk < n ? lo + chunk : n;
-  sort_count(key, lo, hi, shift, bins, hist);
+  sort_count(from, lo, hi, shift, bins, hist);
   const int64_t stride = static_cast<int64_t>(gridDim.x) * kSortThreads;
   for (int64_t i = blockIdx.x * static_cast<int64_t>(kSortThreads) + threadIdx.x;
        i < (n_clear + 15) / 16; i += stride)
@@ -258,10 +267,10 @@ sort_count_kernel(Key key, int64_t n, int64_t chunk, int shift, int bins, int* _
     counts[blockIdx.x * static_cast<int64_t>(bins) + b] = hist[b];
 }
 
-template <class Key, class Out>
+template <class From, class Out>
 __global__ void __launch_bounds__(kSortThreads)
-sort_place_kernel(Key key, const int32_t* __restrict__ vals, Out out, int64_t n, int64_t chunk,
-                  int shift, int bins, const int* __restrict__ counts) {
+sort_place_kernel(From from, Out out, int64_t n, int64_t chunk, int shift, int bins,
+                  const int* __restrict__ counts) {
   extern __shared__ int4 smem4[];
   __shared__ int warp_tot[kSortWarps];
   follow();
@@ -296,7 +305,7 @@ sort_place_kernel(Key key, const int32_t* __restrict__ vals, Out out, int64_t n,
   }
   __syncthreads();
   const int64_t lo = blockIdx.x * chunk, hi = lo + chunk < n ? lo + chunk : n;
-  sort_place(key, vals, out, lo, hi, shift, bins, off, before, cnt);
+  sort_place(from, out, lo, hi, shift, bins, off, before, cnt);
 }
 
 // All CTAs of the cluster, and their memory accesses before it
@@ -317,10 +326,10 @@ __device__ inline int cluster_load(const int* p, unsigned rank) {
 // its warps stretches of kRounds * 32, 32 in a round, so that (CTA, warp, round, lane) is the
 // order of the list.  The counters of the warps are summed per digit in place, those of the CTAs
 // through distributed shared memory.
-template <class Key, class Out, int kRounds>
+template <class I, class Out, int kRounds>
 __global__ void __launch_bounds__(kTeamThreads)
-sort_team_kernel(Key key, Out out, int n, int chunk, int bits, int passes, BufferOut buf0,
-                 BufferOut buf1, uint8_t* __restrict__ clear, int64_t n_clear, int32_t* counter) {
+sort_team_kernel(FromIds<I> ids, Out out, int n, int chunk, int bits, int passes, Entry* list0,
+                 Entry* list1, uint8_t* __restrict__ clear, int64_t n_clear, int32_t* counter) {
   extern __shared__ int4 smem4[];
   __shared__ int warp_tot[kTeamWarps];
   follow();
@@ -338,24 +347,22 @@ sort_team_kernel(Key key, Out out, int n, int chunk, int bits, int passes, Buffe
   if (counter && me == 0 && threadIdx.x == 0) *counter = 0;
   for (int p = 0; p < passes; ++p) {
     const int shift = p * bits;
-    const BufferOut& from = (p & 1) ? buf0 : buf1;  // pass p reads what pass p - 1 wrote
-    auto digit = [&](uint32_t key_) { return (key_ >> shift) & (bins - 1); };
-    uint32_t k[kRounds];
+    auto digit = [&](const Entry& x) { return (x.key >> shift) & (bins - 1); };
+    Entry e[kRounds];
     int place[kRounds];
 #pragma unroll
     for (int q = 0; q < kRounds; ++q) {
       const int i = first + 32 * q;
-      k[q] = 0;
       if (i < hi) {
-        if (p == 0) k[q] = key(i);
-        else if constexpr (!Out::kOnePass) k[q] = __ldcg(from.keys + i);
+        if (Out::kOnePass || p == 0) e[q] = ids(i);
+        else e[q] = load_entry(((p & 1) ? list0 : list1) + i);  // what pass p - 1 wrote
       }
     }
     for (int i = threadIdx.x; i < kTeamWarps * bins / 2; i += kTeamThreads) cnt2[i] = 0;
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < kRounds; ++q)
-      place[q] = sort_rank(first + 32 * q < hi ? digit(k[q]) : 0xffffffffu, mine);
+      place[q] = sort_rank(first + 32 * q < hi ? digit(e[q]) : 0xffffffffu, mine);
     __syncthreads();
     for (int b = threadIdx.x; b < bins / 2; b += kTeamThreads) {
       uint32_t run = 0;
@@ -398,15 +405,10 @@ sort_team_kernel(Key key, Out out, int n, int chunk, int bits, int passes, Buffe
     __syncthreads();
 #pragma unroll
     for (int q = 0; q < kRounds; ++q) {
-      const int i = first + 32 * q;
-      if (i < hi) {
-        const int dst = place[q] + off[digit(k[q])] + mine[digit(k[q])];
-        int32_t val = i;
-        if constexpr (!Out::kOnePass) {
-          if (p > 0) val = __ldcg(from.vals + i);
-          if (!last) ((p & 1) ? buf1 : buf0)(k[q], val, dst);
-        }
-        if (last) out(k[q], val, dst);
+      if (first + 32 * q < hi) {
+        const int dst = place[q] + off[digit(e[q])] + mine[digit(e[q])];
+        if (Out::kOnePass || last) out(e[q], dst);
+        else ((p & 1) ? list1 : list0)[dst] = e[q];
       }
     }
     // what was placed is read by other CTAs; no CTA may end, or count anew, while its counts are read
@@ -424,7 +426,7 @@ __global__ void __launch_bounds__(256) sort_clear_kernel(uint4* p, int64_t n) {
 struct SortShape {
   int passes, bits, bins;
   bool team;  // sorted by one cluster
-  int lists;  // (key, value) lists between passes
+  int lists;  // lists between passes
   int64_t chunk, chunks;
 };
 inline SortShape sort_shape(int64_t n, int64_t n_keys) {
@@ -444,13 +446,14 @@ inline SortShape sort_shape(int64_t n, int64_t n_keys) {
 // scratch: the lists between passes, and the table of counts
 inline int64_t sort_bytes(int64_t n, int64_t n_keys) {
   const SortShape s = sort_shape(n, n_keys);
-  return s.lists * 2 * align256(n * 4) + align256(s.chunks * s.bins * 4);
+  return s.lists * align256(n * static_cast<int64_t>(sizeof(Entry))) +
+         align256(s.chunks * s.bins * 4);
 }
 
-template <class Key, class Out, int kRounds>
-int sort_team(const Key& key, int64_t n, const Out& out, const SortShape& s, const BufferOut* buf,
+template <class I, class Out, int kRounds>
+int sort_team(const FromIds<I>& ids, int64_t n, const Out& out, const SortShape& s, Entry** list,
               uint8_t* clear, int64_t n_clear, int32_t* counter, cudaStream_t st) {
-  auto kernel = &sort_team_kernel<Key, Out, kRounds>;
+  auto kernel = &sort_team_kernel<I, Out, kRounds>;
   auto smem = [](int bins) {
     return bins * (2 * sizeof(int) + kTeamWarps * sizeof(uint16_t));
   };
@@ -468,8 +471,8 @@ int sort_team(const Key& key, int64_t n, const Out& out, const SortShape& s, con
   config.numAttrs = 1;
   const int64_t step = 32 * kRounds;
   const int chunk = static_cast<int>((n + ctas * step - 1) / (ctas * step) * step);
-  return cudaLaunchKernelEx(&config, kernel, key, out, static_cast<int>(n), chunk, s.bits, s.passes,
-                            buf[0], buf[1], clear, n_clear, counter) == cudaSuccess
+  return cudaLaunchKernelEx(&config, kernel, ids, out, static_cast<int>(n), chunk, s.bits, s.passes,
+                            list[0], list[1], clear, n_clear, counter) == cudaSuccess
              ? launch_status()
              : B2S_ERR_LAUNCH;
 }
@@ -480,10 +483,11 @@ template <class I, class Out>
 int sort_ids(const IdKeys<I>& ids, int64_t n, const Out& out, uint8_t* clear, int64_t n_clear,
              int32_t* counter, unsigned char* ws, cudaStream_t st) {
   const SortShape s = sort_shape(n, ids.n_keys);
-  BufferOut buf[2] = {{nullptr, nullptr}, {nullptr, nullptr}};
+  const FromIds<I> from_ids{ids};
+  Entry* list[2] = {nullptr, nullptr};
   for (int b = 0; b < s.lists; ++b) {
-    buf[b].keys = reinterpret_cast<uint32_t*>(ws); ws += align256(n * 4);
-    buf[b].vals = reinterpret_cast<int32_t*>(ws); ws += align256(n * 4);
+    list[b] = reinterpret_cast<Entry*>(ws);
+    ws += align256(n * static_cast<int64_t>(sizeof(Entry)));
   }
   if (s.team) {
     if (n_clear > (1 << 20)) {
@@ -494,38 +498,36 @@ int sort_ids(const IdKeys<I>& ids, int64_t n, const Out& out, uint8_t* clear, in
       if (status != B2S_OK) return status;
       n_clear = 0;
     }
-    auto go = [&](auto run) { return run(ids, n, out, s, buf, clear, n_clear, counter, st); };
-    if (n <= kTeamThreads * kTeamCtas) return go(&sort_team<IdKeys<I>, Out, 1>);
-    return go(&sort_team<IdKeys<I>, Out, 2>);
+    auto go = [&](auto run) { return run(from_ids, n, out, s, list, clear, n_clear, counter, st); };
+    if (n <= kTeamThreads * kTeamCtas) return go(&sort_team<I, Out, 1>);
+    return go(&sort_team<I, Out, 2>);
   }
   int* counts = reinterpret_cast<int*>(ws);
   const size_t smem = sort_smem(s.bins);
   const unsigned grid = static_cast<unsigned>(s.chunks);
-  auto place = [&](const auto& key, const int32_t* vals, const auto& to, int shift) {
-    auto kernel = &sort_place_kernel<std::decay_t<decltype(key)>, std::decay_t<decltype(to)>>;
+  auto place = [&](const auto& from, const auto& to, int shift) {
+    auto kernel = &sort_place_kernel<std::decay_t<decltype(from)>, std::decay_t<decltype(to)>>;
     ensure_dyn_smem(reinterpret_cast<const void*>(kernel), sort_smem(kSortMaxBins));
-    return launch_behind(kernel, grid, kSortThreads, smem, st, key, vals, to, n, s.chunk, shift,
-                         s.bins, counts);
+    return launch_behind(kernel, grid, kSortThreads, smem, st, from, to, n, s.chunk, shift, s.bins,
+                         counts);
   };
   sort_count_kernel<<<grid, kSortThreads, s.bins * sizeof(int), st>>>(
-      ids, n, s.chunk, 0, s.bins, counts, clear, n_clear, counter);
+      from_ids, n, s.chunk, 0, s.bins, counts, clear, n_clear, counter);
   int status = launch_status();
   if (status != B2S_OK) return status;
   if constexpr (Out::kOnePass) {
-    status = place(ids, nullptr, out, 0);
+    status = place(from_ids, out, 0);
   } else {
-    status = s.passes == 1 ? place(ids, nullptr, out, 0) : place(ids, nullptr, buf[0], 0);
+    status = s.passes == 1 ? place(from_ids, out, 0) : place(from_ids, ListOut{list[0]}, 0);
     for (int p = 1; p < s.passes; ++p) {
-      const BufferOut& from = (p & 1) ? buf[0] : buf[1];
-      const StoredKeys stored{from.keys};
+      const FromList from{(p & 1) ? list[0] : list[1]};
       if (status == B2S_OK)
-        status = launch_behind(&sort_count_kernel<StoredKeys>, grid, kSortThreads,
-                               s.bins * sizeof(int), st, stored, n, s.chunk, p * s.bits, s.bins,
+        status = launch_behind(&sort_count_kernel<FromList>, grid, kSortThreads,
+                               s.bins * sizeof(int), st, from, n, s.chunk, p * s.bits, s.bins,
                                counts, nullptr, 0, nullptr);
       if (status == B2S_OK)
-        status = p + 1 == s.passes
-                     ? place(stored, from.vals, out, p * s.bits)
-                     : place(stored, from.vals, (p & 1) ? buf[1] : buf[0], p * s.bits);
+        status = p + 1 == s.passes ? place(from, out, p * s.bits)
+                                   : place(from, ListOut{(p & 1) ? list[1] : list[0]}, p * s.bits);
     }
   }
   return status;
