@@ -245,6 +245,7 @@ select_rows_kernel(IdKeys<I> ids, int64_t n, const T* __restrict__ table, int64_
                    typename acc_of<T>::type alpha, typename acc_of<T>::type beta, bool has_beta,
                    unsigned groups) {
   using A = typename acc_of<T>::type;
+  follow();
   const unsigned tb = blockIdx.x / groups, g = blockIdx.x - tb * groups;
   const int64_t i = static_cast<int64_t>(tb) * kSelWarps + (threadIdx.x >> 5);
   if (i >= n) return;
@@ -651,6 +652,7 @@ route_dispatch_kernel(const unsigned char* __restrict__ x, int64_t ld_x, int64_t
                       int64_t ld_rows, unsigned slabs) {
   using Raw = typename raw_of<UB>::type;
   constexpr int U = UB == 16 ? 4 : 8;
+  follow();
   const unsigned tb = blockIdx.x / slabs, slab = blockIdx.x - tb * slabs;
   const int64_t t = static_cast<int64_t>(tb) * kSelWarps + (threadIdx.x >> 5);
   if (t >= n) return;
@@ -703,6 +705,7 @@ route_combine_kernel(const T* __restrict__ y, int64_t ld_y, const int32_t* __res
   constexpr int E = kQueueCols<T, VE>, B = kQueueBatch;
   using Queue = PartQueue<Part<T, VE, E>, B, kQueueStages>;
   extern __shared__ int4 smem4[];
+  follow();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const unsigned w = blockIdx.x * kSelWarps + warp;
   const unsigned range = w / slabs, slab = w - range * slabs;
@@ -782,6 +785,7 @@ route_combine_plain_kernel(const T* __restrict__ y, int64_t ld_y,
                            typename acc_of<T>::type beta, bool has_beta, unsigned slabs) {
   using A = typename acc_of<T>::type;
   constexpr int kAhead = 4;
+  follow();
   const unsigned tb = blockIdx.x / slabs, slab = blockIdx.x - tb * slabs;
   const int64_t t = static_cast<int64_t>(tb) * kSelWarps + (threadIdx.x >> 5);
   if (t >= n) return;
@@ -828,6 +832,7 @@ route_combine_grad_kernel(const T* __restrict__ g, int64_t ld_g, const T* __rest
                           int dim, typename acc_of<T>::type alpha, T* __restrict__ grad_y,
                           int64_t ld_gy, void* __restrict__ grad_w) {
   using A = typename acc_of<T>::type;
+  follow();
   const int64_t a = blockIdx.x * static_cast<int64_t>(kSelWarps) + (threadIdx.x >> 5);
   if (a >= n * k) return;
   const int lane = threadIdx.x & 31;
@@ -946,17 +951,13 @@ int select_rows_run(const IdKeys<I>& ids, int64_t n, const void* table, int64_t 
   const T* tp = static_cast<const T*>(table);
   T* op = static_cast<T*>(out);
   const A a = static_cast<A>(alpha), b = static_cast<A>(beta);
-#define B2S_GO(VE, GG)                                                                          \
-  select_rows_kernel<T, I, VE, GG><<<static_cast<unsigned>(blocks), kSelThreads, 0, s>>>(       \
-      ids, n, tp, ld_table, static_cast<int>(dim), op, ld_out, a, b, b != A(0),                 \
-      static_cast<unsigned>(groups))
-  if (wide) {
-    if (G == 1) B2S_GO(16 / sizeof(T), 1); else B2S_GO(16 / sizeof(T), 4);
-  } else {
-    if (G == 1) B2S_GO(1, 1); else B2S_GO(1, 4);
-  }
-#undef B2S_GO
-  return launch_status();
+  auto go = [&](auto kernel) {
+    return launch_behind(kernel, dim3(static_cast<unsigned>(blocks)), kSelThreads, 0, s, ids, n, tp,
+                         ld_table, dim, op, ld_out, a, b, b != A(0), groups);
+  };
+  constexpr int VE = 16 / sizeof(T);
+  if (wide) return G == 1 ? go(&select_rows_kernel<T, I, VE, 1>) : go(&select_rows_kernel<T, I, VE, 4>);
+  return G == 1 ? go(&select_rows_kernel<T, I, 1, 1>) : go(&select_rows_kernel<T, I, 1, 4>);
 }
 
 template <class T, class O, int VE, bool kBeta>
@@ -1144,19 +1145,20 @@ int route_combine_go(const T* y, int64_t ld_y, const int32_t* slots, const void*
       kSelWarps * PartQueue<Part<T, VE, E>, kQueueBatch, kQueueStages>::kWarpBytes;
   ensure_dyn_smem(reinterpret_cast<const void*>(kernel), smem);
   const int64_t slabs = ceil_div(dim, 32 * E);
-  // every warp that fits the GPU at once gets one range
+  // A range per warp that fits the GPU at once, and ranges of 16 rows where that makes more of
+  // them: some SMs are a third faster than others at this, and take what the others leave (8192
+  // x 8 rows of 4096 bf16: 101 us, 109 with one range a warp).
   constexpr int64_t kResident = 148 * kCombineCtas<T, VE> * kSelWarps;
-  int64_t ranges = kResident / slabs;
+  int64_t ranges = std::max<int64_t>(kResident / slabs, n * k / 16);
   ranges = ranges < 1 ? 1 : ranges > n ? n : ranges;
   // a warp counts its assignments in 32 bits (with two stretches to spare)
   while (ceil_div(n, ranges) * k > 0x7fff0000) ++ranges;
   const int64_t blocks = ceil_div(ranges * slabs, kSelWarps);
+  if (blocks > kMaxGrid) return B2S_ERR_RANGE;
   const A b = static_cast<A>(beta);
-  kernel<<<static_cast<unsigned>(blocks), kSelThreads, smem, s>>>(
-      y, ld_y, slots, weights, w_f32, n, static_cast<int>(k), static_cast<int>(dim), out, ld_out,
-      static_cast<A>(alpha), b, b != A(0), static_cast<unsigned>(slabs),
-      static_cast<unsigned>(ranges));
-  return launch_status();
+  return launch_behind(kernel, dim3(static_cast<unsigned>(blocks)), kSelThreads, smem, s, y, ld_y,
+                       slots, weights, w_f32, n, k, dim, out, ld_out, alpha, b, b != A(0), slabs,
+                       ranges);
 }
 
 template <class T>
@@ -1177,10 +1179,9 @@ int route_combine_run(const void* y, int64_t ld_y, const int32_t* slots, const v
     const int64_t slabs = ceil_div(dim, kSelCols), blocks = ceil_div(n, kSelWarps) * slabs;
     if (blocks > kMaxGrid) return B2S_ERR_RANGE;
     const float b = static_cast<float>(beta);
-    route_combine_plain_kernel<T><<<static_cast<unsigned>(blocks), kSelThreads, 0, s>>>(
-        yp, ld_y, slots, weights, w_f32, n, static_cast<int>(k), static_cast<int>(dim), op, ld_out,
-        static_cast<float>(alpha), b, b != 0, static_cast<unsigned>(slabs));
-    return launch_status();
+    return launch_behind(&route_combine_plain_kernel<T>, dim3(static_cast<unsigned>(blocks)),
+                         kSelThreads, 0, s, yp, ld_y, slots, weights, w_f32, n, k, dim, op, ld_out,
+                         alpha, b, b != 0, slabs);
   }
 }
 
@@ -1196,11 +1197,10 @@ int route_combine_grad_run(const void* g, int64_t ld_g, const void* y, int64_t l
                     (!grad_w || wide_rows(y, ld_y, dim, sizeof(T))) &&
                     wide_rows(grad_y, ld_gy, dim, sizeof(T));
   auto go = [&](auto kernel) {
-    kernel<<<static_cast<unsigned>(blocks), kSelThreads, 0, s>>>(
-        static_cast<const T*>(g), ld_g, static_cast<const T*>(y), ld_y, slots, held, weights,
-        w_f32, n, static_cast<int>(k), static_cast<int>(dim), static_cast<A>(alpha),
-        static_cast<T*>(grad_y), ld_gy, grad_w);
-    return launch_status();
+    return launch_behind(kernel, dim3(static_cast<unsigned>(blocks)), kSelThreads, 0, s,
+                         static_cast<const T*>(g), ld_g, static_cast<const T*>(y), ld_y, slots,
+                         held, weights, w_f32, n, k, dim, alpha, static_cast<T*>(grad_y), ld_gy,
+                         grad_w);
   };
   return wide ? go(&route_combine_grad_kernel<T, 16 / sizeof(T)>)
               : go(&route_combine_grad_kernel<T, 1>);
@@ -1223,19 +1223,16 @@ extern "C" int b2s_route_dispatch(int val_type, const void* x_dev, int64_t ld_x,
   const int64_t slabs = ceil_div(units, wide ? 128 : 256);
   const int64_t blocks = ceil_div(n_tokens, kSelWarps) * slabs;
   if (blocks > kMaxGrid) return B2S_ERR_RANGE;
-#define B2S_GO(VB)                                                                             \
-  route_dispatch_kernel<VB><<<static_cast<unsigned>(blocks), kSelThreads, 0,                   \
-                              static_cast<cudaStream_t>(stream)>>>(                            \
-      static_cast<const unsigned char*>(x_dev), ld_x * static_cast<int64_t>(es), n_tokens,     \
-      static_cast<int>(k), static_cast<int>(units), slots_dev, held_dev,                       \
-      static_cast<unsigned char*>(rows_dev), ld_rows * static_cast<int64_t>(es),               \
-      static_cast<unsigned>(slabs))
-  if (wide) B2S_GO(16);
-  else if (es == 2) B2S_GO(2);
-  else if (es == 4) B2S_GO(4);
-  else B2S_GO(8);
-#undef B2S_GO
-  return launch_status();
+  auto go = [&](auto kernel) {
+    return launch_behind(kernel, dim3(static_cast<unsigned>(blocks)), kSelThreads, 0,
+                         static_cast<cudaStream_t>(stream), static_cast<const unsigned char*>(x_dev),
+                         ld_x * static_cast<int64_t>(es), n_tokens, k, units, slots_dev, held_dev,
+                         static_cast<unsigned char*>(rows_dev), ld_rows * static_cast<int64_t>(es),
+                         slabs);
+  };
+  if (wide) return go(&route_dispatch_kernel<16>);
+  return es == 2 ? go(&route_dispatch_kernel<2>)
+                 : es == 4 ? go(&route_dispatch_kernel<4>) : go(&route_dispatch_kernel<8>);
 }
 
 extern "C" int b2s_route_combine(int val_type, const void* y_dev, int64_t ld_y,

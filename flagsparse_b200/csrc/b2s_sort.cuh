@@ -104,15 +104,16 @@ struct PlanOut {  // token route: slot of each assignment, token of each slot, f
   }
 };
 
-// ---- kernels of one call that follow each other -------------------------------------------------
-// Each is put in place while the one before it still runs (programmatic dependent launch), which
-// hides its launch.  Every thread calls follow() before it touches memory: it returns when the
-// kernel before has ended and its writes are visible.
+// ---- kernels that follow each other --------------------------------------------------------------
+// Each kernel is put in place while the one before it in the stream still runs (programmatic
+// dependent launch), which hides its launch: 1 to 2 us of each.  Every thread of every kernel calls
+// follow() before it touches memory or ends: it returns when the kernel before has ended and its
+// writes are visible, and lets the kernel behind be put in place.
 __device__ inline void follow() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
-// launches `kernel`, which calls follow(), behind another kernel of the same call
+// launches `kernel`, which calls follow()
 template <class... Params, class... Args>
 int launch_behind(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t st,
                   const Args&... args) {
@@ -418,6 +419,7 @@ sort_team_kernel(FromIds<I> ids, Out out, int n, int chunk, int bits, int passes
 
 // flags that are too many for the cluster
 __global__ void __launch_bounds__(256) sort_clear_kernel(uint4* p, int64_t n) {
+  follow();
   const int64_t i = blockIdx.x * 256LL + threadIdx.x;
   if (i < n) p[i] = make_uint4(0, 0, 0, 0);
 }
@@ -459,16 +461,18 @@ int sort_team(const FromIds<I>& ids, int64_t n, const Out& out, const SortShape&
   };
   ensure_dyn_smem(reinterpret_cast<const void*>(kernel), smem(kSortMaxBins));
   const unsigned ctas = n <= kTeamThreads ? 1 : kTeamCtas;
-  cudaLaunchAttribute cluster;
-  cluster.id = cudaLaunchAttributeClusterDimension;
-  cluster.val.clusterDim = {ctas, 1, 1};
+  cudaLaunchAttribute how[2];
+  how[0].id = cudaLaunchAttributeClusterDimension;
+  how[0].val.clusterDim = {ctas, 1, 1};
+  how[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  how[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(ctas);
   config.blockDim = dim3(kTeamThreads);
   config.dynamicSmemBytes = smem(s.bins);
   config.stream = st;
-  config.attrs = &cluster;
-  config.numAttrs = 1;
+  config.attrs = how;
+  config.numAttrs = 2;
   const int64_t step = 32 * kRounds;
   const int chunk = static_cast<int>((n + ctas * step - 1) / (ctas * step) * step);
   return cudaLaunchKernelEx(&config, kernel, ids, out, static_cast<int>(n), chunk, s.bits, s.passes,
@@ -492,9 +496,9 @@ int sort_ids(const IdKeys<I>& ids, int64_t n, const Out& out, uint8_t* clear, in
   if (s.team) {
     if (n_clear > (1 << 20)) {
       const int64_t words = (n_clear + 15) / 16;
-      sort_clear_kernel<<<static_cast<unsigned>((words + 255) / 256), 256, 0, st>>>(
-          reinterpret_cast<uint4*>(clear), words);
-      const int status = launch_status();
+      const int status = launch_behind(&sort_clear_kernel,
+                                       dim3(static_cast<unsigned>((words + 255) / 256)), 256, 0, st,
+                                       reinterpret_cast<uint4*>(clear), words);
       if (status != B2S_OK) return status;
       n_clear = 0;
     }
@@ -511,9 +515,9 @@ int sort_ids(const IdKeys<I>& ids, int64_t n, const Out& out, uint8_t* clear, in
     return launch_behind(kernel, grid, kSortThreads, smem, st, from, to, n, s.chunk, shift, s.bins,
                          counts);
   };
-  sort_count_kernel<<<grid, kSortThreads, s.bins * sizeof(int), st>>>(
-      from_ids, n, s.chunk, 0, s.bins, counts, clear, n_clear, counter);
-  int status = launch_status();
+  int status = launch_behind(&sort_count_kernel<FromIds<I>>, grid, kSortThreads,
+                             s.bins * sizeof(int), st, from_ids, n, s.chunk, 0, s.bins, counts,
+                             clear, n_clear, counter);
   if (status != B2S_OK) return status;
   if constexpr (Out::kOnePass) {
     status = place(from_ids, out, 0);
