@@ -90,6 +90,10 @@ template <class A, int E> struct Sums {
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = A(0);
   }
+  template <class P> __device__ void set(const P& p) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = p.get(e);
+  }
   template <class P> __device__ void add(const P& p) {
 #pragma unroll
     for (int e = 0; e < E; ++e) v[e] = v[e] + p.get(e);
@@ -104,6 +108,10 @@ template <int E> struct Sums<float, E> {
   __device__ void clear() {
 #pragma unroll
     for (int e = 0; e < E / 2; ++e) v2[e] = make_float2(0.f, 0.f);
+  }
+  template <class P> __device__ void set(const P& p) {
+#pragma unroll
+    for (int e = 0; e < E / 2; ++e) v2[e] = p.pair(e);
   }
   template <class P> __device__ void add(const P& p) {
 #pragma unroll
@@ -176,7 +184,9 @@ __device__ inline void scale_row(O* row, int dim, A beta) {
 
 // A warp's queue of row parts on their way from global to shared memory.  Every lane copies and
 // later reads its own pieces (of 16 bytes, or single elements of 4 or 8), so that no barrier is
-// needed, and the bytes in flight do not cost registers.  Parts are asked for in batches: kStages batches of kBatch parts.
+// needed, and the bytes in flight do not cost registers.  Parts are asked for in batches: kStages
+// batches of kBatch parts.  (With four or eight rows in flight in registers the combine reached
+// half of the copy rate; it was waiting for latency with few warps, or short of registers.)
 template <class P, int kBatch, int kStages> struct PartQueue {
   static constexpr int kPieces = P::U * P::N;
   static constexpr int kWarpBytes = kBatch * kStages * static_cast<int>(sizeof(P)) * 32;
@@ -221,8 +231,8 @@ template <class P, int kBatch, int kStages> struct PartQueue {
     for (int i = 0; i < kPieces; ++i) v.r[i] = at[i * 32];
     return v;
   }
-  // nothing may be under way when the warp ends
   __device__ void skip() { put = put + 1 == kStages ? 0 : put + 1; }  // shares another's groups
+  // nothing may be under way when the warp ends
   __device__ void drain() { asm volatile("cp.async.wait_all;" ::: "memory"); }
   __device__ void done() { take = take + 1 == kStages ? 0 : take + 1; }
 };
@@ -263,7 +273,7 @@ select_rows_kernel(IdKeys<I> ids, int64_t n, const T* __restrict__ table, int64_
   for (int s = 0; s < G; ++s) {
     Sums<A, 8> v;
     v.clear();
-    if (live) v.add(r[s]);
+    if (live) v.set(r[s]);
     // (a masked row is zero whatever alpha is)
     store_axpby<T, VE, A, 8>(o, col0 + s * kSelCols, dim, v, live ? alpha : A(1), has_beta, beta);
   }
@@ -1154,7 +1164,7 @@ int route_combine_go(const T* y, int64_t ld_y, const int32_t* slots, const void*
   // a warp counts its assignments in 32 bits (with two stretches to spare)
   while (ceil_div(n, ranges) * k > 0x7fff0000) ++ranges;
   const int64_t blocks = ceil_div(ranges * slabs, kSelWarps);
-  if (blocks > kMaxGrid) return B2S_ERR_RANGE;
+  if (blocks > kMaxGrid / kSelWarps) return B2S_ERR_RANGE;  // (warps are counted in 32 bits)
   const A b = static_cast<A>(beta);
   return launch_behind(kernel, dim3(static_cast<unsigned>(blocks)), kSelThreads, smem, s, y, ld_y,
                        slots, weights, w_f32, n, k, dim, out, ld_out, alpha, b, b != A(0), slabs,

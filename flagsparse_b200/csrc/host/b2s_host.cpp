@@ -183,7 +183,8 @@ PyObject* embedding_grad(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     if (a[5] != Py_None) {
       out = plain(a[5]);
       if (!out || out->get_device() != dev || out->dim() != 2 || out->size(0) != n_rows ||
-          out->size(1) != dim || recorded(*out) || recorded(*grad) || !row_major(*out, &out_pitch))
+          out->size(1) != dim || recorded(*out) || recorded(*grad) ||
+          out->storage().is_alias_of(grad->storage()) || !row_major(*out, &out_pitch))
         NOT_HERE;
       if (a[7] == Py_None) {
         if (out->scalar_type() != out_type && !(out->scalar_type() == at::kFloat &&
@@ -206,7 +207,7 @@ PyObject* embedding_grad(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
                       alpha, beta, ws.data_ptr(), bytes, status, on.stream) != B2S_OK)
       NOT_HERE;
     if (a[5] == Py_None) return THPVariable_Wrap(std::move(made));
-    out->unsafeGetTensorImpl()->bump_version();
+    if (!out->is_inference()) out->unsafeGetTensorImpl()->bump_version();
     Py_INCREF(a[5]);
     return a[5];
   })

@@ -159,7 +159,7 @@ def _as_int(value, name):
 
 
 def _scalar(value, dtype, name):
-    return value if type(value) is float else check_scalar(value, dtype, name)
+    return value if type(value) is float else float(check_scalar(value, dtype, name))
 
 
 def _wants_grad(t, other=None):
@@ -178,6 +178,26 @@ def _refuse_out(out, t, other=None):
     if _wants_grad(out, t) or _wants_grad(out, other):
         raise RuntimeError("out= does not support automatic differentiation, but one of the "
                            "arguments requires grad")
+
+
+def _refuse_overlap(out, *inputs):
+    """The kernels read their inputs while they write `out`."""
+    for t in inputs:
+        if (t is None or not t.numel() or not out.numel()
+                or t.untyped_storage().data_ptr() != out.untyped_storage().data_ptr()):
+            continue
+        size = out.element_size()
+        ends = [(v.data_ptr(), v.data_ptr() + size * (1 + sum(
+            (n - 1) * abs(s) for n, s in zip(v.shape, v.stride())))) for v in (out, t)]
+        if ends[0][1] <= ends[1][0] or ends[1][1] <= ends[0][0]:
+            continue
+        # rows of one array side by side: columns that do not meet
+        if out.dim() == t.dim() == 2 and t.dtype == out.dtype and out.stride() == t.stride():
+            pitch = out.stride(0)
+            apart = (ends[1][0] - ends[0][0]) // size % pitch
+            if out.stride(1) == 1 and out.shape[1] <= apart <= pitch - t.shape[1]:
+                continue
+        raise ValueError("out must not overlap the tensors that are read")
 
 
 def _rows(t):
@@ -290,6 +310,8 @@ def _embedding(tokens, table, alpha, has_ignore, ignore, out, beta, index):
         _check_size("the number of rows of table", n_rows, MAX_ROWS)
         _check_size("dim", dim, MAX_DIM)
     flat, address, pitch = _result(out, (*tokens.shape, dim), table, table.dtype, beta)
+    if out is not None:
+        _refuse_overlap(out, table)
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
     table = _rows(table)
@@ -309,7 +331,7 @@ def flagsparse_embedding_grad(tokens, grad, n_rows, alpha=1.0, ignore_index=None
     bfloat16, of float32 (`out_dtype`, or the dtype of `out`).  beta = 0 writes every row (zero
     where no token names it); beta = 1 adds to `out` and touches the named rows only.
     The tokens are sorted, and the rows of one token are summed in float32 (float64) in a fixed
-    order: the result is the same from run to run.
+    order: the result is the same from run to run.  The call itself is not differentiable.
     """
     if _host is not None:
         result = _host.embedding_grad(tokens, grad, n_rows, alpha, ignore_index, out, beta,
@@ -344,6 +366,8 @@ def flagsparse_embedding_grad(tokens, grad, n_rows, alpha=1.0, ignore_index=None
     _check_size("n_rows", n_rows, MAX_ROWS)
     _check_size("dim", dim, MAX_DIM)
     flat, address, pitch = _result(out, (n_rows, dim), grad, out_dtype, beta)
+    if out is not None:
+        _refuse_overlap(out, grad)
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
     grad = _rows(grad if grad.dim() == 2 else grad.reshape(n, dim))
@@ -533,6 +557,8 @@ def flagsparse_token_dispatch(x, route, out=None):
 def _dispatch(x, route, out):
     dim = x.shape[1]
     flat, address, pitch = _result(out, (route.n_rows, dim), x, x.dtype, 0.0)
+    if out is not None:
+        _refuse_overlap(out, x)
     x = _rows(x)
     route._use()
     _call(route._index, _lib.load().b2s_route_dispatch, _lib.VALUE_CODE[x.dtype], x.data_ptr(),
@@ -597,6 +623,8 @@ def flagsparse_token_combine(y, route, weights=None, alpha=1.0, out=None, beta=0
 def _combine(y, route, weights, alpha, out, beta):
     dim = y.shape[1]
     flat, address, pitch = _result(out, (route.n_tokens, dim), y, y.dtype, beta)
+    if out is not None:
+        _refuse_overlap(out, y, weights)
     y = _rows(y)
     wcode, waddress = 0, None
     if weights is not None:

@@ -31,6 +31,7 @@ def test_public_names():
     ((TOK, TABLE[0]), {}, ValueError, "table must be a 2D tensor"),
     ((TOK, TABLE), {"alpha": 1j}, TypeError, "alpha is complex"),
     ((TOK, TABLE), {"alpha": torch.ones(2)}, ValueError, "alpha must be a scalar"),
+    ((TOK, TABLE), {"alpha": "two"}, ValueError, "could not convert"),
     ((TOK, TABLE), {"ignore_index": 1.0}, TypeError, "ignore_index must be an integer"),
     ((TOK, TABLE), {"ignore_index": True}, TypeError, "ignore_index must be an integer"),
     ((TOK, TABLE), {"ignore_index": 2**63}, ValueError, "ignore_index must fit int64"),
@@ -172,6 +173,23 @@ def test_result_places():
         assert selection._finish(empty, flat) is empty
 
 
+def test_overlap_of_out_and_what_is_read():
+    wide = torch.zeros(6, 10)
+    refuse = lambda out, *t: pytest.raises(ValueError, selection._refuse_overlap, out, *t)  # noqa: E731
+    selection._refuse_overlap(wide, None, torch.zeros(6, 10), wide[:0])
+    selection._refuse_overlap(wide[:3], wide[3:])
+    selection._refuse_overlap(wide[:, :4], wide[:, 4:])      # columns side by side
+    selection._refuse_overlap(wide[:, 6:], wide[:, :6], wide[:, 2:6])
+    selection._refuse_overlap(wide[2:, 6:], wide[:, :6])
+    refuse(wide, wide)
+    refuse(wide[:4], wide[3:])
+    refuse(wide[:, :5], wide[:, 4:])
+    refuse(wide[:, 4:], wide[:, :5])
+    refuse(wide[1:, :5], wide[:, 4:])
+    refuse(wide[:, :4], wide.view(-1))
+    refuse(wide, torch.zeros(1), wide[2])
+
+
 def test_c_entry_points_answer_before_any_launch():
     lib, d = _lib.load(), ctypes.c_void_p(4096)          # never read: every call below is refused
     odd = ctypes.c_void_p(4097)
@@ -194,7 +212,7 @@ def test_c_entry_points_answer_before_any_launch():
     plan = lambda i=1, e=d, t=4, k=2, n=8, b=1 << 30: lib.b2s_route_plan(  # noqa: E731
         i, e, t, k, n, d, d, d, d, b, None, None)
     assert plan(i=2) == dtype and plan(e=None) == arg and plan(n=-1) == arg
-    assert plan(n=2048) == rng and plan(t=2**31, k=2) == rng and plan(t=4000, b=0) == ws
+    assert plan(n=2048) == rng and plan(t=2**31, k=2) == rng and plan(t=9000, b=0) == ws
     assert plan(e=ctypes.c_void_p(4100)) == align
     disp = lambda v=0, x=d, s=d, h=d, t=4, ld=8: lib.b2s_route_dispatch(  # noqa: E731
         v, x, ld, t, 2, 8, s, h, d, 8, None)

@@ -74,6 +74,7 @@ def cpu(t):
     (70, 33, 1032, 8), (700, 1000, 1001, 3), (2500, 500, 2048, 0)])
 def test_embedding(dtype, n, vocab, dim, pad):
     table = randn(vocab, dim, dtype=dtype, seed=n, pad=pad)
+    table[:, ::7] *= 0.0                                                # zeros of both signs
     rng = np.random.default_rng(n)
     tokens = torch.from_numpy(rng.integers(0, vocab, n))
     want = cpu(table)[tokens]
@@ -81,6 +82,7 @@ def test_embedding(dtype, n, vocab, dim, pad):
         tok = tokens.to(index).cuda()
         got = fs.flagsparse_embedding(tok, table)
         assert got.dtype == dtype and torch.equal(cpu(got), want)       # a copy, bit for bit
+        assert torch.equal(torch.signbit(got).cpu(), torch.signbit(want))
         got = fs.flagsparse_embedding(tok, table, alpha=1.375)
         assert_close(got, 1.375 * want, 1.375 * want.abs(), 0)
     out = randn(n, dim, dtype=dtype, seed=5, pad=pad)
@@ -592,6 +594,32 @@ def test_only_what_needs_a_gradient_is_recorded():
     g, = torch.autograd.grad(y.sum(), table, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()                           # once differentiable
+
+
+def test_scalars_outputs_and_inference_tensors():
+    table, tokens = randn(20, 16), torch.randint(0, 20, (9,), device="cuda")
+    for alpha in (2, np.float32(2), np.float64(2), torch.tensor(2.0), torch.tensor(2, device="cuda"),
+                  2 + 0j):
+        assert torch.equal(fs.flagsparse_embedding(tokens, table, alpha=alpha), table[tokens] * 2)
+    with torch.inference_mode():
+        frozen, grad = table.clone(), torch.zeros(20, 16, device="cuda")
+        y = fs.flagsparse_embedding(tokens, frozen)
+        fs.flagsparse_embedding_grad(tokens, y, 20, out=grad, beta=1.0)
+    fs.flagsparse_embedding_grad(tokens, y, 20, out=grad, beta=1.0)
+    assert torch.equal(y, table[tokens])
+    assert torch.equal(grad, 2 * fs.flagsparse_embedding_grad(tokens, y, 20))
+    watched = torch.zeros(20, 16, device="cuda")
+    version = watched._version
+    fs.flagsparse_embedding_grad(tokens, y, 20, out=watched, beta=1.0)
+    assert watched._version > version
+    both = randn(20, 32)
+    with pytest.raises(ValueError, match="must not overlap"):
+        fs.flagsparse_embedding_grad(torch.arange(20, device="cuda"), both[:, :20], 20,
+                                     out=both[:, 12:], beta=1.0)
+    want = fs.flagsparse_embedding_grad(torch.arange(20, device="cuda"), both[:, :16].clone(), 20)
+    fs.flagsparse_embedding_grad(torch.arange(20, device="cuda"), both[:, :16], 20,
+                                 out=both[:, 16:])
+    assert torch.equal(both[:, 16:], want)
 
 
 def test_other_streams_and_a_freed_route():
