@@ -312,12 +312,12 @@ struct GradRange {
   bool head, tail;      // its first run began before it; its last run goes on behind it
 };
 
-// The ranges of m entries: `most` of them, or fewer (of eight entries at least).
+// The ranges of m entries: `most` of them, or fewer (of two entries at least).
 struct GradRanges {
   int64_t m, size, count;
   __device__ GradRanges(int64_t held, int64_t most) : m(held) {
     const int64_t even = (held + most - 1) / most;
-    size = even > 8 ? even : 8;
+    size = even > 2 ? even : 2;
     count = (held + size - 1) / size;
   }
   __device__ int64_t border(int64_t r) const { return r * size < m ? r * size : m; }
@@ -919,11 +919,11 @@ constexpr int64_t kMaxGrid = 0x7fffffff;
 
 // How the sorted list is cut: ranges of 24 entries (rows that are also read and written take
 // longer than others: the more ranges a warp slot gets, the more even the work), longer ones where
-// every slot has eight ranges already, and down to 8 entries where half the slots would have none.
+// every slot has eight ranges already, and down to 2 entries where half the slots would have none.
 inline int64_t grad_ranges(int64_t n, int64_t slabs, int64_t ctas_per_sm) {
   const int64_t slots = 148 * ctas_per_sm * kSelWarps;
   const int64_t most = std::min(8 * slots / slabs, ceil_div(n, 24));
-  const int64_t least = std::min(slots / (2 * slabs), ceil_div(n, 8));
+  const int64_t least = std::min(slots / (2 * slabs), ceil_div(n, 2));
   return std::max<int64_t>(std::max(most, least), 1);
 }
 struct GradLayout {

@@ -90,7 +90,8 @@ struct RunsOut {  // embedding gradient: the sorted list, and which rows are nam
   __device__ void first(int, int) const {}
 };
 struct PlanOut {  // token route: slot of each assignment, token of each slot, first slot per expert
-  static constexpr bool kOnePass = true;  // its keys fit one digit: no kernel for a second pass
+  static constexpr bool kOnePass = true;  // its keys fit one digit: no kernel for a second pass,
+                                          // and first() needs the counts of a digit
   int32_t* slots;
   int32_t* indptr;
   int32_t* indices;
@@ -417,6 +418,34 @@ sort_team_kernel(FromIds<I> ids, Out out, int n, int chunk, int bits, int passes
   }
 }
 
+// A list of at most kFewMost entries: every thread counts the entries that stand before its own.
+// (256 entries: 1 us of counting; the two passes of the cluster kernel take 5 to 7 us.)
+constexpr int kFewMost = 256;
+template <class I, class Out>
+__global__ void __launch_bounds__(kFewMost)
+sort_few_kernel(FromIds<I> ids, Out out, int n, uint8_t* __restrict__ clear, int64_t n_clear,
+                int32_t* counter) {
+  __shared__ __align__(16) uint32_t keys[kFewMost];
+  follow();
+  const int i = threadIdx.x;
+  const Entry mine = i < n ? ids(i) : Entry{0xffffffffu, 0};
+  keys[i] = mine.key;
+  for (int64_t c = i; c < (n_clear + 15) / 16; c += kFewMost)
+    reinterpret_cast<uint4*>(clear)[c] = make_uint4(0, 0, 0, 0);
+  if (counter && i == 0) *counter = 0;
+  __syncthreads();
+  if (i >= n) return;
+  int before = 0;
+  for (int j = 0; j < n; j += 4) {
+    const uint4 k = *reinterpret_cast<const uint4*>(keys + j);  // (behind n: the largest)
+    before += k.x < mine.key || (k.x == mine.key && j < i);
+    before += k.y < mine.key || (k.y == mine.key && j + 1 < i);
+    before += k.z < mine.key || (k.z == mine.key && j + 2 < i);
+    before += k.w < mine.key || (k.w == mine.key && j + 3 < i);
+  }
+  out(mine, before);
+}
+
 // flags that are too many for the cluster
 __global__ void __launch_bounds__(256) sort_clear_kernel(uint4* p, int64_t n) {
   follow();
@@ -494,13 +523,18 @@ int sort_ids(const IdKeys<I>& ids, int64_t n, const Out& out, uint8_t* clear, in
     ws += align256(n * static_cast<int64_t>(sizeof(Entry)));
   }
   if (s.team) {
-    if (n_clear > (1 << 20)) {
+    if (n_clear > (n <= kFewMost ? 1 << 17 : 1 << 20)) {
       const int64_t words = (n_clear + 15) / 16;
       const int status = launch_behind(&sort_clear_kernel,
                                        dim3(static_cast<unsigned>((words + 255) / 256)), 256, 0, st,
                                        reinterpret_cast<uint4*>(clear), words);
       if (status != B2S_OK) return status;
       n_clear = 0;
+    }
+    if constexpr (!Out::kOnePass) {
+      if (n <= kFewMost)
+        return launch_behind(&sort_few_kernel<I, Out>, dim3(1), kFewMost, 0, st, from_ids, out, n,
+                             clear, n_clear, counter);
     }
     auto go = [&](auto run) { return run(from_ids, n, out, s, list, clear, n_clear, counter, st); };
     if (n <= kTeamThreads * kTeamCtas) return go(&sort_team<I, Out, 1>);

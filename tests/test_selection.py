@@ -265,7 +265,7 @@ def _ranges(keys, none, most):
     assert m == sum(k < none for k in keys)
     if m == 0:
         return {}, 0
-    size = max(8, -(-m // most))
+    size = max(2, -(-m // most))
     rows, head, tail, runs = {}, {}, {}, []
 
     def crossing(x):
@@ -307,7 +307,7 @@ def test_gradient_ranges_cover_every_entry_once():
         hot = rng.choice([0.1, 0.9])
         keys = sorted(min(none, int(rng.expovariate(1.0))) if rng.random() < hot
                       else rng.randrange(none + 1) for _ in range(n))
-        rows, runs = _ranges(keys, none, rng.choice([1, 2, 3, 10, n, n // 24 + 1]))
+        rows, runs = _ranges(keys, none, rng.choice([1, 2, 3, 10, n, n // 2 + 1, n // 24 + 1]))
         cut += runs
         want = {}
         for i, k in enumerate(keys):
