@@ -7,6 +7,7 @@
 // On a few rows the kernels take 2 to 8 microseconds; the same steps in Python take 10.
 #include <ATen/ATen.h>
 #include <ATen/core/grad_mode.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
@@ -109,6 +110,11 @@ struct On {
   }
 };
 
+// a new tensor beside `like`
+at::Tensor fresh(c10::IntArrayRef shape, at::ScalarType type, const at::Tensor& like) {
+  return at::detail::empty_cuda(shape, type, like.device(), std::nullopt);
+}
+
 #define NOT_HERE Py_RETURN_NONE
 // C++ exceptions (an allocation that failed) become Python's
 #define GUARDED(...)                                    \
@@ -141,7 +147,7 @@ PyObject* embedding(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const int64_t dim = table->size(1);
     c10::DimVector shape(tokens->sizes().begin(), tokens->sizes().end());
     shape.push_back(dim);
-    at::Tensor out = at::empty(shape, table->options());
+    at::Tensor out = fresh(shape, table->scalar_type(), *table);
     if (p_select_rows(vcode, icode, tokens->const_data_ptr(), tokens->numel(), has, ignore,
                       table->const_data_ptr(), table->size(0), pitch, dim, out.data_ptr(), dim,
                       alpha, 0.0, status, on.stream) != B2S_OK)
@@ -196,12 +202,12 @@ PyObject* embedding_grad(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       }
     } else {
       if (beta != 0) NOT_HERE;
-      made = at::empty({n_rows, dim}, grad->options().dtype(out_type));
+      made = fresh({n_rows, dim}, out_type, *grad);
       out = &made;
       out_pitch = dim;
     }
     const int64_t bytes = p_select_grad_bytes(vcode, n, n_rows, dim);
-    at::Tensor ws = at::empty({bytes}, grad->options().dtype(at::kByte));
+    at::Tensor ws = fresh({bytes}, at::kByte, *grad);
     if (p_select_grad(vcode, value_code(*out), icode, tokens->const_data_ptr(), n, has, ignore,
                       grad->const_data_ptr(), pitch, n_rows, dim, out->data_ptr(), out_pitch,
                       alpha, beta, ws.data_ptr(), bytes, status, on.stream) != B2S_OK)
@@ -250,7 +256,7 @@ PyObject* route_plan(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const On on(static_cast<c10::DeviceIndex>(dev));
     const int64_t bytes = p_route_plan_bytes(n_tokens, k, n_experts);
     const int64_t scratch = (2 * n + n_experts + 1 + 63) / 64 * 64;
-    at::Tensor buffer = at::empty({scratch + bytes / 4}, experts->options().dtype(at::kInt));
+    at::Tensor buffer = fresh({scratch + bytes / 4}, at::kInt, *experts);
     int32_t* arrays = buffer.data_ptr<int32_t>();
     if (p_route_plan(icode, experts->const_data_ptr(), n_tokens, k, n_experts, arrays, arrays + n,
                      arrays + n + n_experts + 1, arrays + scratch, bytes, status, on.stream) != B2S_OK)
@@ -279,7 +285,7 @@ PyObject* dispatch(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const On on(static_cast<c10::DeviceIndex>(r.dev));
     if (vcode < 0 || on.stream != made_on) NOT_HERE;
     const int64_t dim = x->size(1);
-    at::Tensor out = at::empty({r.n_rows, dim}, x->options());
+    at::Tensor out = fresh({r.n_rows, dim}, x->scalar_type(), *x);
     if (p_route_dispatch(vcode, x->const_data_ptr(), pitch, r.n_tokens, r.k, dim, r.slots, r.held,
                          out.data_ptr(), dim, on.stream) != B2S_OK)
       NOT_HERE;
@@ -321,7 +327,7 @@ PyObject* combine(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         !weights_of(a[kRouteArgs + 1], r, vcode, &w, &wcode) || (w && recorded(*w)))
       NOT_HERE;
     const int64_t dim = y->size(1);
-    at::Tensor out = at::empty({r.n_tokens, dim}, y->options());
+    at::Tensor out = fresh({r.n_tokens, dim}, y->scalar_type(), *y);
     if (p_route_combine(vcode, y->const_data_ptr(), pitch, r.slots, wcode,
                         w ? w->const_data_ptr() : nullptr, r.n_tokens, r.k, dim, out.data_ptr(),
                         dim, alpha, 0.0, on.stream) != B2S_OK)
@@ -353,8 +359,8 @@ PyObject* combine_grad(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         !weights_of(a[kRouteArgs + 2], r, vcode, &w, &wcode))
       NOT_HERE;
     const int64_t dim = g->size(1);
-    at::Tensor grad_y = at::empty({r.n_rows, dim}, g->options());
-    at::Tensor grad_w = at::empty({r.n_tokens, r.k}, w->options());
+    at::Tensor grad_y = fresh({r.n_rows, dim}, g->scalar_type(), *g);
+    at::Tensor grad_w = fresh({r.n_tokens, r.k}, w->scalar_type(), *w);
     if (p_route_combine_grad(vcode, g->const_data_ptr(), pitch, y->const_data_ptr(), y_pitch,
                              r.slots, r.held, wcode, w->const_data_ptr(), r.n_tokens, r.k, dim,
                              alpha, grad_y.data_ptr(), dim, grad_w.data_ptr(),
