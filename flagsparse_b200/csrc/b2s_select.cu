@@ -1,8 +1,11 @@
 // Products with a selection matrix that is never written out: the embedding lookup
 // (Y = alpha S W + beta Y, S one-hot rows given by token ids), its gradient
 // (dW = alpha S^T G + beta dW), and the routing of tokens to experts and back (S has k entries a
-// row).  All of them move rows of `dim` values; a warp owns 256 columns of a row at a time, eight
-// per lane, so that every load and store of a warp is one contiguous piece of a row.
+// row).  All of them move rows of `dim` values and do one multiply-add a value at most (0.25 to 0.5
+// flop a byte): memory bounds them, and on short lists latency does.  A warp takes a slab of the
+// columns of a row at a time, so that every load and store of a warp is one contiguous piece of a
+// row.  Rates below are the bytes that a call cannot do without per time, on one B200 whose copy
+// rate is 6.55 TB/s.
 #include <algorithm>
 
 #include "b2s_sort.cuh"
@@ -12,7 +15,7 @@ namespace b2s {
 constexpr int kSelWarps = 8;            // warps per CTA of the row kernels
 constexpr int kSelThreads = 32 * kSelWarps;
 constexpr int kSelCols = 256;           // columns of a row a warp holds at a time (8 per lane)
-constexpr int64_t kSelMaxDim = 1 << 22; // grids carry column slabs in their y / division
+constexpr int64_t kSelMaxDim = 1 << 22; // columns are 32-bit numbers, and slabs few
 
 template <class T> struct acc_of { using type = float; };
 template <> struct acc_of<double> { using type = double; };
@@ -247,7 +250,9 @@ constexpr int kQueueCols = VE == 1 ? 8 : 32 / static_cast<int>(sizeof(T));  // o
 template <class T, int VE> constexpr bool kQueued = VE * sizeof(T) >= 4;
 
 // ---- embedding lookup ------------------------------------------------------------------------
-// One warp per (token, group of G slabs).
+// One warp per (token, group of G slabs): 2 KB of a 16-bit row in four loads a lane (16384 tokens,
+// 131072 x 4096 bf16: 33 us, 5.8 TB/s; with two loads 36 us, with eight 33 us but odd widths 7.5
+// instead of 5.1 us).  Lists too short for that many warps take one slab each (64 tokens: 2.0 us).
 template <class T, class I, int VE, int G>
 __global__ void __launch_bounds__(kSelThreads)
 select_rows_kernel(IdKeys<I> ids, int64_t n, const T* __restrict__ table, int64_t ld_table,
@@ -280,12 +285,20 @@ select_rows_kernel(IdKeys<I> ids, int64_t n, const T* __restrict__ table, int64_
 }
 
 // ---- embedding gradient ----------------------------------------------------------------------
-// The sorted (token, position) list is cut into as many ranges as the GPU holds warps for one slab
-// of columns; a warp sums the rows of its range and writes each token's row when its run of equal
+// The sorted (token, position) list is cut into ranges of some 24 entries (grad_ranges); a warp sums
+// the rows of a range over one slab of columns and writes each token's row when its run of equal
 // tokens ends.  A run that crosses a border and ends within 31 entries behind it is read to its
 // end by the warp in front of the border.  A longer one is cut there: each range writes its piece
 // as a partial row, and select_grad_long_kernel adds the pieces in order.  No floating-point
-// atomics: the sums have one order whatever the scheduling.
+// atomics: the sums have one order whatever the scheduling.  Sums and pieces are float32 (float64)
+// and rounded once, in the row of the result.
+//
+// What it measured: new gradient of 131072 x 2048 bf16 from 16384 tokens 106 us (5.7 TB/s, mostly
+// zeros written; 17 us of it the sort); 32768 rows of 4096 bf16 added to 32000 x 4096 float32
+// 136 us (4.1 TB/s: 18 us sort, 108 us sums, of whose issue slots 63 % are taken; two to six
+// stages, and 16 or 32 bytes a lane, make no difference).  One range for every warp slot of the
+// GPU took 150 us for these sums: a row that is read and written costs five times one that
+// continues a run, so that equal numbers of entries are unequal work.
 struct GradRuns {
   const Entry* list;  // tokens and their positions, sorted; the masked ones at the end
   int64_t n;
@@ -322,7 +335,9 @@ struct GradRanges {
   }
   __device__ int64_t border(int64_t r) const { return r * size < m ? r * size : m; }
 };
-// entries from border x on that continue the run in front of it, kCross for that many or more
+// Entries from border x on that continue the run in front of it, kCross for that many or more.
+// (With 64 fewer runs are cut, but the warp that reads on is late: 50257 x 771 float32 with a token
+// on a third of 6001 places took 6 us more.)
 constexpr int kCross = 32;
 __device__ inline int grad_crossing(const GradRuns& runs, int64_t m, int64_t x) {
   if (x <= 0 || x >= m) return 0;
@@ -487,12 +502,12 @@ constexpr int kGradWarpBytes =
     (kBeta ? PartQueue<Part<O, VE, kGradCols<T, O, VE, kBeta>>, 1, kGradStages<kBeta>>::kWarpBytes
            : 0);
 
-// The same for rows that cannot be taken 16 bytes at a time: groups of rows in registers.
+// The same for 16-bit rows that cannot be taken 16 bytes at a time: groups of rows in registers.
 template <class T, class O, bool kBeta>
 __device__ inline void grad_sum_plain(const GradRuns& runs, const GradRange& g,
                                       const GradOut<T, O>& to, int col0,
                                       const T* __restrict__ grad, int64_t ld_grad) {
-  constexpr int kAhead = sizeof(T) == 8 ? 2 : 4;
+  constexpr int kAhead = 4;
   const int lane = threadIdx.x & 31;
   Sums<typename acc_of<T>::type, 8> acc;
   acc.clear();
@@ -592,7 +607,8 @@ select_grad_kernel(GradRuns runs, int64_t ranges, unsigned sum_blocks, unsigned 
 
 // A run that was cut: the piece of the range it begins in, then the pieces of those behind.  One
 // CTA per (run, slab of 32 E columns): its warps take the pieces in turn and the warps' sums are
-// added in warp order.
+// added in warp order.  The list names each run's first and last range, so that the sums wait for
+// two loads in a row and no search (7 instead of 16 us for one run of 95 pieces).
 constexpr int kLongWarps = 8;
 
 template <class T, class O, int VE, int E>
@@ -653,7 +669,7 @@ __device__ inline bool is_row(int32_t s, int64_t rows) {
 
 // Rows are only moved: units of UB bytes, whatever the value type.  One warp per (token, slab);
 // the token's row is read once and written to its slots.  The rows behind the last expert's are
-// zeroed by the same warps.
+// zeroed by the same warps.  (8192 tokens to 8 rows each, 4096 bf16: 94 us, 6.4 TB/s.)
 template <int UB>
 __global__ void __launch_bounds__(kSelThreads)
 route_dispatch_kernel(const unsigned char* __restrict__ x, int64_t ld_x, int64_t n, int k,
@@ -666,27 +682,28 @@ route_dispatch_kernel(const unsigned char* __restrict__ x, int64_t ld_x, int64_t
   const unsigned tb = blockIdx.x / slabs, slab = blockIdx.x - tb * slabs;
   const int64_t t = static_cast<int64_t>(tb) * kSelWarps + (threadIdx.x >> 5);
   if (t >= n) return;
-  const int u0 = static_cast<int>(slab) * (32 * U) + (threadIdx.x & 31);
+  const int lane = threadIdx.x & 31, u0 = static_cast<int>(slab) * (32 * U) + lane;
+  // the row, its slots and the number of rows held are asked for together
   Raw r[U];
 #pragma unroll
   for (int u = 0; u < U; ++u)
     if (u0 + 32 * u < units)
       r[u] = *reinterpret_cast<const Raw*>(x + t * ld_x + static_cast<int64_t>(u0 + 32 * u) * UB);
-  for (int j = 0; j < k; ++j) {
-    const int32_t s = slots[t * k + j];
-    if (!is_row(s, n * k)) continue;
+  int32_t my_slot = lane < k ? slots[t * k + lane] : -1;
+  const int64_t held = *held_at;
+  auto store = [&](int64_t row) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
       if (u0 + 32 * u < units)
-        *reinterpret_cast<Raw*>(rows + s * ld_rows + static_cast<int64_t>(u0 + 32 * u) * UB) = r[u];
+        *reinterpret_cast<Raw*>(rows + row * ld_rows + (u0 + 32 * u) * int64_t{UB}) = r[u];
+  };
+  for (int j = 0; j < k; ++j) {
+    if ((j & 31) == 0 && j > 0) my_slot = j + lane < k ? slots[t * k + j + lane] : -1;
+    const int32_t s = __shfl_sync(0xffffffffu, my_slot, j & 31);
+    if (is_row(s, n * k)) store(s);
   }
   memset(r, 0, sizeof(r));
-  for (int64_t z = *held_at + t; z < n * k; z += n) {
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (u0 + 32 * u < units)
-        *reinterpret_cast<Raw*>(rows + z * ld_rows + static_cast<int64_t>(u0 + 32 * u) * UB) = r[u];
-  }
+  for (int64_t z = held + t; z < n * k; z += n) store(z);
 }
 
 // weights may be absent (1), of the value type, or float32
@@ -701,7 +718,9 @@ __device__ inline typename acc_of<T>::type route_weight(const void* w, bool w_is
 // out[t] = alpha * sum_j w[t, j] * y[slots[t, j]] + beta * out[t].  A warp takes a range of tokens
 // and one slab of columns; the assignments of its tokens are one stretch of `slots`, read 32 at a
 // time and a stretch ahead, and their rows stream through the warp's queue without a pause
-// between tokens.  A masked assignment is a part of zeros with weight zero.
+// between tokens.  A masked assignment is a part of zeros with weight zero.  (8192 x 8 rows of 4096
+// bf16: 101 us, 6.0 TB/s; 16384 x 4 rows of 2048: 55 us, 6.1 TB/s.  With 16 bytes a lane and a wait
+// for every row, 134 us: 82 % of the issue slots were taken.)
 template <class T, int VE>
 constexpr int kCombineCtas = VE == 1 && sizeof(T) == 8 ? 2 : kQueueCtas;
 template <class T, int VE>
@@ -784,8 +803,8 @@ route_combine_kernel(const T* __restrict__ y, int64_t ld_y, const int32_t* __res
   queue.drain();
 }
 
-// The same for rows that cannot be taken 16 bytes at a time: one warp per (token, slab), up to 32
-// slots and weights read at once, four rows in flight in registers.
+// The same for 16-bit rows that cannot be taken 16 bytes at a time: one warp per (token, slab), up
+// to 32 slots and weights read at once, four rows in flight in registers.
 template <class T>
 __global__ void __launch_bounds__(kSelThreads)
 route_combine_plain_kernel(const T* __restrict__ y, int64_t ld_y,
@@ -832,7 +851,9 @@ route_combine_plain_kernel(const T* __restrict__ y, int64_t ld_y,
 
 // grad_y[slots[a]] = alpha * w[a] * g[a / k], grad_w[a] = alpha * <g[a / k], y[slots[a]]>: one
 // warp per assignment a, over the whole row (the dot product ends in the warp); the warps of one
-// token share its row of g through the caches.  Rows behind the last expert's are zeroed.
+// token share its row of g through the caches.  Rows behind the last expert's are zeroed.  Held to
+// 32 registers, so that 64 warps share an SM: 16384 x 4 rows of 2048 bf16 98 us, 6.2 TB/s (118 us
+// with the 48 registers that the compiler takes otherwise).
 template <class T, int VE>
 __global__ void __launch_bounds__(kSelThreads, sizeof(T) < 8 ? 8 : 4)
 route_combine_grad_kernel(const T* __restrict__ g, int64_t ld_g, const T* __restrict__ y,
@@ -847,6 +868,7 @@ route_combine_grad_kernel(const T* __restrict__ g, int64_t ld_g, const T* __rest
   if (a >= n * k) return;
   const int lane = threadIdx.x & 31;
   const int32_t s = slots[a];
+  const int64_t z = *held_at + a;
   A dot = A(0);
   if (is_row(s, n * k)) {
     const T* gr = g + (a / k) * ld_g;
@@ -879,7 +901,6 @@ route_combine_grad_kernel(const T* __restrict__ g, int64_t ld_g, const T* __rest
         static_cast<T*>(grad_w)[a] = storage_of<T>::from_acc(dot);
     }
   }
-  const int64_t z = *held_at + a;
   if (z < n * k) zero_row(grad_y + z * ld_gy, dim);
 }
 
@@ -918,8 +939,10 @@ constexpr int64_t kMaxGrid = 0x7fffffff;
   } while (0)
 
 // How the sorted list is cut: ranges of 24 entries (rows that are also read and written take
-// longer than others: the more ranges a warp slot gets, the more even the work), longer ones where
-// every slot has eight ranges already, and down to 2 entries where half the slots would have none.
+// longer than others: the more ranges a warp slot gets, the more even the work; with ranges of 64
+// the sums above took 127 us, with 16 the joining of runs grew by what they gained), longer ones
+// where every slot has eight ranges already, and down to 2 entries where half the slots would have
+// none (256 tokens: 7.7 us with ranges of 2, 10 us with 8).
 inline int64_t grad_ranges(int64_t n, int64_t slabs, int64_t ctas_per_sm) {
   const int64_t slots = 148 * ctas_per_sm * kSelWarps;
   const int64_t most = std::min(8 * slots / slabs, ceil_div(n, 24));
@@ -966,7 +989,8 @@ int select_rows_run(const IdKeys<I>& ids, int64_t n, const void* table, int64_t 
                          ld_table, dim, op, ld_out, a, b, b != A(0), groups);
   };
   constexpr int VE = 16 / sizeof(T);
-  if (wide) return G == 1 ? go(&select_rows_kernel<T, I, VE, 1>) : go(&select_rows_kernel<T, I, VE, 4>);
+  if (wide)
+    return G == 1 ? go(&select_rows_kernel<T, I, VE, 1>) : go(&select_rows_kernel<T, I, VE, 4>);
   return G == 1 ? go(&select_rows_kernel<T, I, 1, 1>) : go(&select_rows_kernel<T, I, 1, 4>);
 }
 
@@ -979,7 +1003,8 @@ int select_grad_go(const GradRuns& runs, const T* grad, int64_t ld_grad,
   constexpr size_t smem = kQueued<T, VE> ? kSelWarps * kGradWarpBytes<T, O, VE, kBeta> : 0;
   const int64_t slabs = ceil_div(to.dim, 32 * E);
   const int64_t ranges =
-      runs.n == 0 ? 0 : std::min(grad_ranges(runs.n, slabs, kGradCtas<T, O, VE, kBeta>), most_ranges);
+      runs.n == 0 ? 0
+                  : std::min(grad_ranges(runs.n, slabs, kGradCtas<T, O, VE, kBeta>), most_ranges);
   const int64_t sums = ceil_div(ranges * slabs, kSelWarps);
   const int64_t rest = to.beta == A(1) ? 0 : ceil_div(static_cast<int64_t>(runs.n_keys),
                                                         kRestRows<T, VE> * kSelWarps);
@@ -987,9 +1012,8 @@ int select_grad_go(const GradRuns& runs, const T* grad, int64_t ld_grad,
   if (sums + rest == 0) return B2S_OK;
   auto kernel = &select_grad_kernel<T, O, VE, kBeta>;
   if (smem > 0) ensure_dyn_smem(reinterpret_cast<const void*>(kernel), smem);
-  B2S_TRY(launch_behind(kernel, dim3(static_cast<unsigned>(sums + rest)), kSelThreads, smem, s, runs,
-                        ranges, static_cast<unsigned>(sums), static_cast<unsigned>(slabs), grad,
-                        ld_grad, to, named));
+  B2S_TRY(launch_behind(kernel, dim3(static_cast<unsigned>(sums + rest)), kSelThreads, smem, s,
+                        runs, ranges, sums, slabs, grad, ld_grad, to, named));
   if (runs.n > kCross) {  // a run that is cut goes on for kCross entries behind a border
     constexpr int kCols = VE > 1 && sizeof(T) == 8 ? 4 : 8;
     const dim3 grid(static_cast<unsigned>(std::min<int64_t>(ranges, 128)),

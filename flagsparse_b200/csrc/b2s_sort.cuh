@@ -413,7 +413,7 @@ sort_team_kernel(FromIds<I> ids, Out out, int n, int chunk, int bits, int passes
         else ((p & 1) ? list1 : list0)[dst] = e[q];
       }
     }
-    // what was placed is read by other CTAs; no CTA may end, or count anew, while its counts are read
+    // what was placed is read by other CTAs, and no CTA may end or count anew while its counts are
     cluster_barrier();
   }
 }

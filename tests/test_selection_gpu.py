@@ -226,7 +226,7 @@ PATTERNS = {
     "long": (runs(1, 4000, 3, 2500, 33), 7),
     "even": (torch.from_numpy(np.random.default_rng(1).integers(0, 900, 2000)), 900),
     "one chunk": (torch.from_numpy(np.random.default_rng(2).integers(0, 5000, 4096)), 5000),
-    "few": (torch.from_numpy(np.random.default_rng(5).zipf(1.2, 256) % 300000), 300000),
+    "few": (torch.from_numpy(np.random.default_rng(5).zipf(1.2, 256) % 30000), 30000),
     "not few": (torch.from_numpy(np.random.default_rng(5).zipf(1.2, 257) % 3000), 3000),
     "few and same": (torch.full((250,), 3), 4),
     "team of one": (torch.from_numpy(np.random.default_rng(5).zipf(1.3, 1024) % 30000), 30000),
