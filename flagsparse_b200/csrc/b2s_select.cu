@@ -255,12 +255,15 @@ template <class T, int VE> constexpr bool kQueued = VE * sizeof(T) >= 4;
 // instead of 5.1 us).  Lists too short for that many warps take one slab each (64 tokens: 2.0 us).
 template <class T, class I, int VE, int G>
 __global__ void __launch_bounds__(kSelThreads)
-select_rows_kernel(IdKeys<I> ids, int64_t n, const T* __restrict__ table, int64_t ld_table,
-                   int dim, T* __restrict__ out, int64_t ld_out,
+select_rows_kernel(IdKeys<I> ids, int64_t n, const T* table, int64_t ld_table,
+                   int dim, T* out, int64_t ld_out,
                    typename acc_of<T>::type alpha, typename acc_of<T>::type beta, bool has_beta,
                    unsigned groups) {
   using A = typename acc_of<T>::type;
   follow();
+  ids = behind(ids);
+  table = behind(table);
+  out = behind(out);
   const unsigned tb = blockIdx.x / groups, g = blockIdx.x - tb * groups;
   const int64_t i = static_cast<int64_t>(tb) * kSelWarps + (threadIdx.x >> 5);
   if (i >= n) return;
@@ -285,8 +288,8 @@ select_rows_kernel(IdKeys<I> ids, int64_t n, const T* __restrict__ table, int64_
 }
 
 // ---- embedding gradient ----------------------------------------------------------------------
-// The sorted (token, position) list is cut into ranges of some 24 entries (grad_ranges); a warp sums
-// the rows of a range over one slab of columns and writes each token's row when its run of equal
+// The sorted (token, position) list is cut into ranges of some 24 entries (grad_ranges); a warp
+// sums the rows of a range over one slab of columns and writes each token's row when its run of equal
 // tokens ends.  A run that crosses a border and ends within 31 entries behind it is read to its
 // end by the warp in front of the border.  A longer one is cut there: each range writes its piece
 // as a partial row, and select_grad_long_kernel adds the pieces in order.  No floating-point
@@ -424,7 +427,7 @@ constexpr int kGradCols = kBeta && sizeof(O) > sizeof(T) ? 8 : kQueueCols<T, VE>
 template <class T, class O, int VE, bool kBeta>
 __device__ inline void grad_sum(const GradRuns& runs, const GradRange& g,
                                 const GradOut<T, O>& to, unsigned char* warp_smem, int col0,
-                                const T* __restrict__ grad, int64_t ld_grad) {
+                                const T* grad, int64_t ld_grad) {
   constexpr int E = kGradCols<T, O, VE, kBeta>, S = kGradStages<kBeta>;
   using Rows = PartQueue<Part<T, VE, E>, 1, S>;
   using Olds = PartQueue<Part<O, VE, E>, 1, S>;
@@ -506,7 +509,7 @@ constexpr int kGradWarpBytes =
 template <class T, class O, bool kBeta>
 __device__ inline void grad_sum_plain(const GradRuns& runs, const GradRange& g,
                                       const GradOut<T, O>& to, int col0,
-                                      const T* __restrict__ grad, int64_t ld_grad) {
+                                      const T* grad, int64_t ld_grad) {
   constexpr int kAhead = 4;
   const int lane = threadIdx.x & 31;
   Sums<typename acc_of<T>::type, 8> acc;
@@ -566,10 +569,14 @@ template <class T, int VE> constexpr int kRestRows = kQueued<T, VE> ? 1 : 4;
 template <class T, class O, int VE, bool kBeta>
 __global__ void __launch_bounds__(kSelThreads, kGradCtas<T, O, VE, kBeta>)
 select_grad_kernel(GradRuns runs, int64_t ranges, unsigned sum_blocks, unsigned slabs,
-                   const T* __restrict__ grad, int64_t ld_grad, GradOut<T, O> to,
-                   const uint8_t* __restrict__ named) {
+                   const T* grad, int64_t ld_grad, GradOut<T, O> to,
+                   const uint8_t* named) {
   extern __shared__ int4 smem4[];
   follow();
+  runs.list = behind(runs.list);
+  grad = behind(grad);
+  to.out = behind(to.out);
+  named = behind(named);
   const int warp = threadIdx.x >> 5;
   const unsigned b = blockIdx.x, rest = gridDim.x - sum_blocks;
   const unsigned both = 2 * (sum_blocks < rest ? sum_blocks : rest);
@@ -617,6 +624,11 @@ select_grad_long_kernel(GradOut<T, O> to, bool has_beta) {
   using A = typename acc_of<T>::type;
   __shared__ A sums[kLongWarps][E][32];
   follow();
+  to.long_count = behind(to.long_count);
+  to.long_list = behind(to.long_list);
+  to.head = behind(to.head);
+  to.tail = behind(to.tail);
+  to.out = behind(to.out);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int count = *to.long_count;
   int4 run = to.long_list[blockIdx.x];  // (there is room for gridDim.x entries)
@@ -672,13 +684,16 @@ __device__ inline bool is_row(int32_t s, int64_t rows) {
 // zeroed by the same warps.  (8192 tokens to 8 rows each, 4096 bf16: 94 us, 6.4 TB/s.)
 template <int UB>
 __global__ void __launch_bounds__(kSelThreads)
-route_dispatch_kernel(const unsigned char* __restrict__ x, int64_t ld_x, int64_t n, int k,
-                      int units, const int32_t* __restrict__ slots,
-                      const int32_t* __restrict__ held_at, unsigned char* __restrict__ rows,
+route_dispatch_kernel(const unsigned char* x, int64_t ld_x, int64_t n, int k,
+                      int units, const int32_t* slots,
+                      const int32_t* held_at, unsigned char* rows,
                       int64_t ld_rows, unsigned slabs) {
   using Raw = typename raw_of<UB>::type;
   constexpr int U = UB == 16 ? 4 : 8;
   follow();
+  x = behind(x);
+  slots = behind(slots);
+  held_at = behind(held_at);
   const unsigned tb = blockIdx.x / slabs, slab = blockIdx.x - tb * slabs;
   const int64_t t = static_cast<int64_t>(tb) * kSelWarps + (threadIdx.x >> 5);
   if (t >= n) return;
@@ -725,9 +740,9 @@ template <class T, int VE>
 constexpr int kCombineCtas = VE == 1 && sizeof(T) == 8 ? 2 : kQueueCtas;
 template <class T, int VE>
 __global__ void __launch_bounds__(kSelThreads, kCombineCtas<T, VE>)
-route_combine_kernel(const T* __restrict__ y, int64_t ld_y, const int32_t* __restrict__ slots,
-                     const void* __restrict__ weights, bool w_is_f32, int64_t n, int k, int dim,
-                     T* __restrict__ out, int64_t ld_out, typename acc_of<T>::type alpha,
+route_combine_kernel(const T* y, int64_t ld_y, const int32_t* slots,
+                     const void* weights, bool w_is_f32, int64_t n, int k, int dim,
+                     T* out, int64_t ld_out, typename acc_of<T>::type alpha,
                      typename acc_of<T>::type beta, bool has_beta, unsigned slabs,
                      unsigned ranges) {
   using A = typename acc_of<T>::type;
@@ -735,6 +750,10 @@ route_combine_kernel(const T* __restrict__ y, int64_t ld_y, const int32_t* __res
   using Queue = PartQueue<Part<T, VE, E>, B, kQueueStages>;
   extern __shared__ int4 smem4[];
   follow();
+  y = behind(y);
+  slots = behind(slots);
+  weights = behind(weights);
+  out = behind(out);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const unsigned w = blockIdx.x * kSelWarps + warp;
   const unsigned range = w / slabs, slab = w - range * slabs;
@@ -807,14 +826,18 @@ route_combine_kernel(const T* __restrict__ y, int64_t ld_y, const int32_t* __res
 // to 32 slots and weights read at once, four rows in flight in registers.
 template <class T>
 __global__ void __launch_bounds__(kSelThreads)
-route_combine_plain_kernel(const T* __restrict__ y, int64_t ld_y,
-                           const int32_t* __restrict__ slots, const void* __restrict__ weights,
-                           bool w_is_f32, int64_t n, int k, int dim, T* __restrict__ out,
+route_combine_plain_kernel(const T* y, int64_t ld_y,
+                           const int32_t* slots, const void* weights,
+                           bool w_is_f32, int64_t n, int k, int dim, T* out,
                            int64_t ld_out, typename acc_of<T>::type alpha,
                            typename acc_of<T>::type beta, bool has_beta, unsigned slabs) {
   using A = typename acc_of<T>::type;
   constexpr int kAhead = 4;
   follow();
+  y = behind(y);
+  slots = behind(slots);
+  weights = behind(weights);
+  out = behind(out);
   const unsigned tb = blockIdx.x / slabs, slab = blockIdx.x - tb * slabs;
   const int64_t t = static_cast<int64_t>(tb) * kSelWarps + (threadIdx.x >> 5);
   if (t >= n) return;
@@ -856,14 +879,19 @@ route_combine_plain_kernel(const T* __restrict__ y, int64_t ld_y,
 // with the 48 registers that the compiler takes otherwise).
 template <class T, int VE>
 __global__ void __launch_bounds__(kSelThreads, sizeof(T) < 8 ? 8 : 4)
-route_combine_grad_kernel(const T* __restrict__ g, int64_t ld_g, const T* __restrict__ y,
-                          int64_t ld_y, const int32_t* __restrict__ slots,
-                          const int32_t* __restrict__ held_at,
-                          const void* __restrict__ weights, bool w_is_f32, int64_t n, int k,
-                          int dim, typename acc_of<T>::type alpha, T* __restrict__ grad_y,
-                          int64_t ld_gy, void* __restrict__ grad_w) {
+route_combine_grad_kernel(const T* g, int64_t ld_g, const T* y,
+                          int64_t ld_y, const int32_t* slots,
+                          const int32_t* held_at,
+                          const void* weights, bool w_is_f32, int64_t n, int k,
+                          int dim, typename acc_of<T>::type alpha, T* grad_y,
+                          int64_t ld_gy, void* grad_w) {
   using A = typename acc_of<T>::type;
   follow();
+  g = behind(g);
+  y = behind(y);
+  slots = behind(slots);
+  held_at = behind(held_at);
+  weights = behind(weights);
   const int64_t a = blockIdx.x * static_cast<int64_t>(kSelWarps) + (threadIdx.x >> 5);
   if (a >= n * k) return;
   const int lane = threadIdx.x & 31;
@@ -1259,8 +1287,8 @@ extern "C" int b2s_route_dispatch(int val_type, const void* x_dev, int64_t ld_x,
   if (blocks > kMaxGrid) return B2S_ERR_RANGE;
   auto go = [&](auto kernel) {
     return launch_behind(kernel, dim3(static_cast<unsigned>(blocks)), kSelThreads, 0,
-                         static_cast<cudaStream_t>(stream), static_cast<const unsigned char*>(x_dev),
-                         ld_x * static_cast<int64_t>(es), n_tokens, k, units, slots_dev, held_dev,
+                         static_cast<cudaStream_t>(stream),
+                         static_cast<const unsigned char*>(x_dev), ld_x * static_cast<int64_t>(es), n_tokens, k, units, slots_dev, held_dev,
                          static_cast<unsigned char*>(rows_dev), ld_rows * static_cast<int64_t>(es),
                          slabs);
   };

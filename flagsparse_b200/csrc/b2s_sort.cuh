@@ -27,7 +27,7 @@ constexpr int64_t kTeamMost = 2 * kTeamThreads * kTeamCtas;
 constexpr int kSortMaxBits = 11;
 constexpr int kSortMaxBins = 1 << kSortMaxBits;
 constexpr int64_t kSortMaxEntries = 0x7fffffff - (1 << 25);  // positions are int32
-constexpr int64_t kSortMaxKeys = 0x7ffffffe;             // keys are uint32, n_keys stands for masked
+constexpr int64_t kSortMaxKeys = 0x7ffffffe;             // n_keys itself stands for masked
 
 inline int64_t align256(int64_t b) { return (b + 255) / 256 * 256; }
 
@@ -114,6 +114,25 @@ __device__ inline void follow() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
+// A pointer as it is known behind follow().  What is read through it cannot be read before (the
+// compiler may move loads that it takes for constant in front of a wait; a pointer that it knows
+// nothing of until then leaves it nothing to move).
+template <class T> __device__ inline T* behind(T* p) {
+  asm volatile("" : "+l"(p)::"memory");
+  return p;
+}
+template <class I> __device__ inline IdKeys<I> behind(IdKeys<I> ids) {
+  ids.ids = behind(ids.ids);
+  return ids;
+}
+template <class I> __device__ inline FromIds<I> behind(FromIds<I> from) {
+  from.key = behind(from.key);
+  return from;
+}
+__device__ inline FromList behind(FromList from) {
+  from.list = behind(from.list);
+  return from;
+}
 // launches `kernel`, which calls follow()
 template <class... Params, class... Args>
 int launch_behind(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t st,
@@ -128,9 +147,8 @@ int launch_behind(void (*kernel)(Params...), dim3 grid, int threads, size_t smem
   config.stream = st;
   config.attrs = &early;
   config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...) == cudaSuccess
-             ? launch_status()
-             : B2S_ERR_LAUNCH;
+  cudaLaunchKernelEx(&config, kernel, static_cast<Params>(args)...);
+  return launch_status();  // (reads and clears the error of a launch that was refused)
 }
 
 // ---- device pieces of a pass ---------------------------------------------------------------------
@@ -250,11 +268,12 @@ inline size_t sort_smem(int bins) {
 // counts[chunk][digit]; the CTAs also zero `clear` (flags of the caller) and *counter
 template <class From>
 __global__ void __launch_bounds__(kSortThreads)
-sort_count_kernel(From from, int64_t n, int64_t chunk, int shift, int bins, int* __restrict__ counts,
-                  uint8_t* __restrict__ clear, int64_t n_clear, int32_t* counter) {
+sort_count_kernel(From from, int64_t n, int64_t chunk, int shift, int bins,
+                  int* counts, uint8_t* clear, int64_t n_clear, int32_t* counter) {
   extern __shared__ int4 smem4[];
   int* hist = reinterpret_cast<int*>(smem4);
   follow();
+  from = behind(from);
   for (int b = threadIdx.x; b < bins; b += kSortThreads) hist[b] = 0;
   __syncthreads();
   const int64_t lo = blockIdx.x * chunk, hi = lo + chunk < n ? lo + chunk : n;
@@ -272,10 +291,12 @@ sort_count_kernel(From from, int64_t n, int64_t chunk, int shift, int bins, int*
 template <class From, class Out>
 __global__ void __launch_bounds__(kSortThreads)
 sort_place_kernel(From from, Out out, int64_t n, int64_t chunk, int shift, int bins,
-                  const int* __restrict__ counts) {
+                  const int* counts) {
   extern __shared__ int4 smem4[];
   __shared__ int warp_tot[kSortWarps];
   follow();
+  from = behind(from);
+  counts = behind(counts);
   int* off = reinterpret_cast<int*>(smem4);
   int* before = off + bins;  // off_next until the first tile
   uint16_t* cnt = reinterpret_cast<uint16_t*>(before + bins);
@@ -331,10 +352,11 @@ __device__ inline int cluster_load(const int* p, unsigned rank) {
 template <class I, class Out, int kRounds>
 __global__ void __launch_bounds__(kTeamThreads)
 sort_team_kernel(FromIds<I> ids, Out out, int n, int chunk, int bits, int passes, Entry* list0,
-                 Entry* list1, uint8_t* __restrict__ clear, int64_t n_clear, int32_t* counter) {
+                 Entry* list1, uint8_t* clear, int64_t n_clear, int32_t* counter) {
   extern __shared__ int4 smem4[];
   __shared__ int warp_tot[kTeamWarps];
   follow();
+  ids = behind(ids);
   const int bins = 1 << bits, warp = threadIdx.x >> 5;
   const unsigned me = blockIdx.x, ctas = gridDim.x;
   int* off = reinterpret_cast<int*>(smem4);
@@ -423,10 +445,11 @@ sort_team_kernel(FromIds<I> ids, Out out, int n, int chunk, int bits, int passes
 constexpr int kFewMost = 256;
 template <class I, class Out>
 __global__ void __launch_bounds__(kFewMost)
-sort_few_kernel(FromIds<I> ids, Out out, int n, uint8_t* __restrict__ clear, int64_t n_clear,
+sort_few_kernel(FromIds<I> ids, Out out, int n, uint8_t* clear, int64_t n_clear,
                 int32_t* counter) {
   __shared__ __align__(16) uint32_t keys[kFewMost];
   follow();
+  ids = behind(ids);
   const int i = threadIdx.x;
   const Entry mine = i < n ? ids(i) : Entry{0xffffffffu, 0};
   keys[i] = mine.key;
@@ -504,10 +527,9 @@ int sort_team(const FromIds<I>& ids, int64_t n, const Out& out, const SortShape&
   config.numAttrs = 2;
   const int64_t step = 32 * kRounds;
   const int chunk = static_cast<int>((n + ctas * step - 1) / (ctas * step) * step);
-  return cudaLaunchKernelEx(&config, kernel, ids, out, static_cast<int>(n), chunk, s.bits, s.passes,
-                            list[0], list[1], clear, n_clear, counter) == cudaSuccess
-             ? launch_status()
-             : B2S_ERR_LAUNCH;
+  cudaLaunchKernelEx(&config, kernel, ids, out, static_cast<int>(n), chunk, s.bits, s.passes,
+                     list[0], list[1], clear, n_clear, counter);
+  return launch_status();
 }
 
 // Sorts ids 0 .. n - 1 into `out`; zeroes clear[0 .. n_clear) (padded to 16) and *counter before

@@ -166,15 +166,16 @@ PyObject* embedding_grad(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         !ignored(a[4], &has, &ignore) || !number(a[6], &beta))
       NOT_HERE;
     const at::Tensor *tokens = plain(a[0]), *grad = plain(a[1]);
-    if (!tokens || !grad || tokens->dim() != 1 || grad->dim() != 2 ||
-        grad->size(0) != tokens->size(0))
+    if (!tokens || !grad || grad->dim() != tokens->dim() + 1 ||
+        grad->sizes().slice(0, tokens->dim()) != tokens->sizes())
       NOT_HERE;
     const int vcode = value_code(*grad), icode = index_code(*tokens), dev = grad->get_device();
     int32_t* status = clean_status(dev);
+    const int64_t n = tokens->numel(), dim = grad->size(grad->dim() - 1);
+    pitch = dim;
     if (vcode < 0 || icode < 0 || !status || tokens->get_device() != dev ||
-        !tokens->is_contiguous() || !row_major(*grad, &pitch))
+        !tokens->is_contiguous() || !(row_major(*grad, &pitch) || grad->is_contiguous()))
       NOT_HERE;
-    const int64_t n = tokens->numel(), dim = grad->size(1);
     at::ScalarType out_type = grad->scalar_type();
     if (a[7] != Py_None) {
       if (!THPDtype_Check(a[7])) NOT_HERE;
@@ -259,7 +260,8 @@ PyObject* route_plan(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     at::Tensor buffer = fresh({scratch + bytes / 4}, at::kInt, *experts);
     int32_t* arrays = buffer.data_ptr<int32_t>();
     if (p_route_plan(icode, experts->const_data_ptr(), n_tokens, k, n_experts, arrays, arrays + n,
-                     arrays + n + n_experts + 1, arrays + scratch, bytes, status, on.stream) != B2S_OK)
+                     arrays + n + n_experts + 1, arrays + scratch, bytes, status,
+                     on.stream) != B2S_OK)
       NOT_HERE;
     PyObject* stream = PyLong_FromLongLong(reinterpret_cast<intptr_t>(on.stream));
     PyObject* wrapped = THPVariable_Wrap(std::move(buffer));
@@ -414,9 +416,9 @@ PyObject* bind_status(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
 
 #define METHOD(name) \
   {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {METHOD(embedding),  METHOD(embedding_grad), METHOD(route_plan),
-                         METHOD(dispatch),   METHOD(combine),        METHOD(combine_grad),
-                         METHOD(bind),       METHOD(bind_status),    {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {METHOD(embedding), METHOD(embedding_grad), METHOD(route_plan),
+                         METHOD(dispatch),  METHOD(combine),        METHOD(combine_grad),
+                         METHOD(bind),      METHOD(bind_status),    {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_b2s_host", nullptr, -1, methods,
                       nullptr,               nullptr,     nullptr, nullptr};
 

@@ -21,8 +21,8 @@ capture that is refused (autograd may run a leaf's accumulation on a stream outs
 captured training steps call the ``*_grad`` functions.
 
 Nothing synchronises.  Ids are checked by the kernels: one outside its range selects nothing, and
-IndexError is raised by the next call on that device, or by ``check_selection_ids()``, which waits
-for the device.
+IndexError is raised by the next call on that device that takes ids (a lookup, its gradient, a
+route), or by ``check_selection_ids()``, which waits for the device.
 """
 
 from __future__ import annotations

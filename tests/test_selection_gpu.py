@@ -357,8 +357,10 @@ def plain_route(experts, n_experts):
     return slots.reshape(experts.shape), indptr, order // max(experts.shape[1], 1)
 
 
-ROUTES = [(1, 1, 1, 0.0), (1024, 1, 9, 0.1), (1025, 1, 9, 0.1), (1024, 4, 500, 0.0), (8192, 1, 70, 0.2),
-          (8193, 1, 64, 0.2), (8192, 2, 2047, 0.0), (16385, 2, 2047, 0.1), (1, 8, 8, 0.0), (7, 3, 5, 0.3), (64, 8, 256, 0.0), (100, 2, 2047, 0.1),
+ROUTES = [(1, 1, 1, 0.0), (1024, 1, 9, 0.1), (1025, 1, 9, 0.1), (1024, 4, 500, 0.0),
+          (8192, 1, 70, 0.2),
+          (8193, 1, 64, 0.2), (8192, 2, 2047, 0.0), (16385, 2, 2047, 0.1), (1, 8, 8, 0.0),
+          (7, 3, 5, 0.3), (64, 8, 256, 0.0), (100, 2, 2047, 0.1),
           (513, 8, 3, 0.0), (2100, 2, 64, 0.05), (16384, 1, 128, 0.0), (17000, 8, 60, 0.1),
           (50, 40, 64, 0.0), (6, 4, 10, 1.0), (0, 4, 10, 0.0), (5, 0, 10, 0.0)]
 
