@@ -7,7 +7,8 @@
 // alone the scattered stores are the limit: 16384 entries in two passes took 64 us there, and
 // take 19 us on eight.  The passes of a longer list cut it into at most 128 chunks, one CTA each.
 // The first kernel counts the digits of each chunk; the second sums those counts itself (every CTA
-// reads the whole chunks x digits table, which L2 holds) and places its entries in order.
+// reads the whole chunks x digits table, which L2 holds), places its entries in order and counts
+// the next digit of each in the chunk that it is placed in.
 #pragma once
 #include <type_traits>
 
@@ -17,7 +18,7 @@ namespace b2s {
 
 constexpr int kSortThreads = 512;
 constexpr int kSortWarps = kSortThreads / 32;
-constexpr int kSortRounds = 2;                           // entries per thread and tile
+constexpr int kSortRounds = 1;                           // entries per thread and tile
 constexpr int kSortTile = kSortThreads * kSortRounds;
 constexpr int kSortMaxChunks = 128;
 constexpr int kTeamThreads = 1024;                       // CTAs of a cluster that sorts alone
@@ -211,12 +212,25 @@ __device__ inline int sort_rank(unsigned digit, uint16_t* mine) {
   return prev + before;
 }
 
+// The counts of the pass behind: entry by entry, where it is placed (integer sums: any order).
+struct NextCounts {
+  int* table;  // NULL: there is no pass behind
+  unsigned chunk;
+  int shift;
+  __device__ void operator()(const Entry& e, int dst, int bins) const {
+    if (table)
+      atomicAdd(table + static_cast<int64_t>(dst / chunk) * bins + ((e.key >> shift) & (bins - 1)),
+                1);
+  }
+};
+
 // Places entries [lo, hi) in order; off[b] is where the next entry with digit b goes.  A warp
 // takes 32 neighbouring entries per round: those with the same digit are ranked by lane, the
 // rounds and warps of a tile by the counters cnt[warp][digit], tiles by off.
 template <class From, class Out>
 __device__ inline void sort_place(const From& from, const Out& out, int64_t lo, int64_t hi,
-                                  int shift, int bins, int* off, int* off_next, uint16_t* cnt) {
+                                  int shift, int bins, int* off, int* off_next, uint16_t* cnt,
+                                  const NextCounts& next) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int64_t t0 = lo; t0 < hi; t0 += kSortTile) {
     uint32_t* z = reinterpret_cast<uint32_t*>(cnt);
@@ -249,7 +263,9 @@ __device__ inline void sort_place(const From& from, const Out& out, int64_t lo, 
       const int64_t i = t0 + (warp * kSortRounds + q) * 32 + lane;
       if (i < hi) {
         const int d = (e[q].key >> shift) & (bins - 1);
-        out(e[q], off[d] + mine[d] + rank[q]);
+        const int dst = off[d] + mine[d] + rank[q];
+        out(e[q], dst);
+        next(e[q], dst, bins);
       }
     }
     int* swap = off;
@@ -265,11 +281,12 @@ inline size_t sort_smem(int bins) {
 }
 
 // ---- kernels -------------------------------------------------------------------------------------
-// counts[chunk][digit]; the CTAs also zero `clear` (flags of the caller) and *counter
-template <class From>
+// counts[chunk][digit] of the first digit; the CTAs also zero the tables of the others behind it,
+// `clear` (flags of the caller) and *counter
+template <class I>
 __global__ void __launch_bounds__(kSortThreads)
-sort_count_kernel(From from, int64_t n, int64_t chunk, int shift, int bins,
-                  int* counts, uint8_t* clear, int64_t n_clear, int32_t* counter) {
+sort_count_kernel(FromIds<I> from, int64_t n, int64_t chunk, int bins, int passes, int* counts,
+                  uint8_t* clear, int64_t n_clear, int32_t* counter) {
   extern __shared__ int4 smem4[];
   int* hist = reinterpret_cast<int*>(smem4);
   follow();
@@ -277,12 +294,16 @@ sort_count_kernel(From from, int64_t n, int64_t chunk, int shift, int bins,
   for (int b = threadIdx.x; b < bins; b += kSortThreads) hist[b] = 0;
   __syncthreads();
   const int64_t lo = blockIdx.x * chunk, hi = lo + chunk < n ? lo + chunk : n;
-  sort_count(from, lo, hi, shift, bins, hist);
+  sort_count(from, lo, hi, 0, bins, hist);
   const int64_t stride = static_cast<int64_t>(gridDim.x) * kSortThreads;
   for (int64_t i = blockIdx.x * static_cast<int64_t>(kSortThreads) + threadIdx.x;
        i < (n_clear + 15) / 16; i += stride)
     reinterpret_cast<uint4*>(clear)[i] = make_uint4(0, 0, 0, 0);
   if (counter && blockIdx.x == 0 && threadIdx.x == 0) *counter = 0;
+  const int64_t table = static_cast<int64_t>(gridDim.x) * bins;
+  for (int64_t i = table + blockIdx.x * static_cast<int64_t>(kSortThreads) + threadIdx.x;
+       i < passes * table; i += stride)
+    counts[i] = 0;
   __syncthreads();
   for (int b = threadIdx.x; b < bins; b += kSortThreads)
     counts[blockIdx.x * static_cast<int64_t>(bins) + b] = hist[b];
@@ -291,7 +312,7 @@ sort_count_kernel(From from, int64_t n, int64_t chunk, int shift, int bins,
 template <class From, class Out>
 __global__ void __launch_bounds__(kSortThreads)
 sort_place_kernel(From from, Out out, int64_t n, int64_t chunk, int shift, int bins,
-                  const int* counts) {
+                  const int* counts, NextCounts next) {
   extern __shared__ int4 smem4[];
   __shared__ int warp_tot[kSortWarps];
   follow();
@@ -328,7 +349,7 @@ sort_place_kernel(From from, Out out, int64_t n, int64_t chunk, int shift, int b
   }
   __syncthreads();
   const int64_t lo = blockIdx.x * chunk, hi = lo + chunk < n ? lo + chunk : n;
-  sort_place(from, out, lo, hi, shift, bins, off, before, cnt);
+  sort_place(from, out, lo, hi, shift, bins, off, before, cnt, next);
 }
 
 // All CTAs of the cluster, and their memory accesses before it
@@ -497,11 +518,11 @@ inline SortShape sort_shape(int64_t n, int64_t n_keys) {
   s.chunks = s.team ? 0 : (n + s.chunk - 1) / s.chunk;
   return s;
 }
-// scratch: the lists between passes, and the table of counts
+// scratch: the lists between passes, and a table of counts for each
 inline int64_t sort_bytes(int64_t n, int64_t n_keys) {
   const SortShape s = sort_shape(n, n_keys);
   return s.lists * align256(n * static_cast<int64_t>(sizeof(Entry))) +
-         align256(s.chunks * s.bins * 4);
+         align256(s.passes * s.chunks * s.bins * 4);
 }
 
 template <class I, class Out, int kRounds>
@@ -565,29 +586,27 @@ int sort_ids(const IdKeys<I>& ids, int64_t n, const Out& out, uint8_t* clear, in
   int* counts = reinterpret_cast<int*>(ws);
   const size_t smem = sort_smem(s.bins);
   const unsigned grid = static_cast<unsigned>(s.chunks);
-  auto place = [&](const auto& from, const auto& to, int shift) {
+  const int64_t table = s.chunks * s.bins;
+  auto place = [&](const auto& from, const auto& to, int p) {
     auto kernel = &sort_place_kernel<std::decay_t<decltype(from)>, std::decay_t<decltype(to)>>;
     ensure_dyn_smem(reinterpret_cast<const void*>(kernel), sort_smem(kSortMaxBins));
-    return launch_behind(kernel, grid, kSortThreads, smem, st, from, to, n, s.chunk, shift, s.bins,
-                         counts);
+    const NextCounts next{p + 1 < s.passes ? counts + (p + 1) * table : nullptr,
+                          static_cast<unsigned>(s.chunk), (p + 1) * s.bits};
+    return launch_behind(kernel, grid, kSortThreads, smem, st, from, to, n, s.chunk, p * s.bits,
+                         s.bins, counts + p * table, next);
   };
-  int status = launch_behind(&sort_count_kernel<FromIds<I>>, grid, kSortThreads,
-                             s.bins * sizeof(int), st, from_ids, n, s.chunk, 0, s.bins, counts,
-                             clear, n_clear, counter);
+  int status = launch_behind(&sort_count_kernel<I>, grid, kSortThreads, s.bins * sizeof(int), st,
+                             from_ids, n, s.chunk, s.bins, s.passes, counts, clear, n_clear,
+                             counter);
   if (status != B2S_OK) return status;
   if constexpr (Out::kOnePass) {
     status = place(from_ids, out, 0);
   } else {
     status = s.passes == 1 ? place(from_ids, out, 0) : place(from_ids, ListOut{list[0]}, 0);
-    for (int p = 1; p < s.passes; ++p) {
+    for (int p = 1; p < s.passes && status == B2S_OK; ++p) {
       const FromList from{(p & 1) ? list[0] : list[1]};
-      if (status == B2S_OK)
-        status = launch_behind(&sort_count_kernel<FromList>, grid, kSortThreads,
-                               s.bins * sizeof(int), st, from, n, s.chunk, p * s.bits, s.bins,
-                               counts, nullptr, 0, nullptr);
-      if (status == B2S_OK)
-        status = p + 1 == s.passes ? place(from, out, p * s.bits)
-                                   : place(from, ListOut{(p & 1) ? list[1] : list[0]}, p * s.bits);
+      status = p + 1 == s.passes ? place(from, out, p)
+                                 : place(from, ListOut{(p & 1) ? list[1] : list[0]}, p);
     }
   }
   return status;
