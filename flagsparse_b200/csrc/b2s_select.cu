@@ -296,9 +296,9 @@ select_rows_kernel(IdKeys<I> ids, int64_t n, const T* table, int64_t ld_table,
 // atomics: the sums have one order whatever the scheduling.  Sums and pieces are float32 (float64)
 // and rounded once, in the row of the result.
 //
-// What it measured: new gradient of 131072 x 2048 bf16 from 16384 tokens 106 us (5.7 TB/s, mostly
-// zeros written; 17 us of it the sort); 32768 rows of 4096 bf16 added to 32000 x 4096 float32
-// 136 us (4.1 TB/s: 18 us sort, 108 us sums, of whose issue slots 63 % are taken; two to six
+// What it measured: new gradient of 131072 x 2048 bf16 from 16384 tokens 104 us (5.8 TB/s, mostly
+// zeros written; 14 us of it the sort); 32768 rows of 4096 bf16 added to 32000 x 4096 float32
+// 131 us (4.3 TB/s: 14 us sort, 108 us sums, of whose issue slots 63 % are taken; two to six
 // stages, and 16 or 32 bytes a lane, make no difference).  One range for every warp slot of the
 // GPU took 150 us for these sums: a row that is read and written costs five times one that
 // continues a run, so that equal numbers of entries are unequal work.

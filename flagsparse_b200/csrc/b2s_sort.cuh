@@ -2,10 +2,11 @@
 // expert (token route).  Least significant digit first; one digit of up to 11 bits per pass, so
 // that a route needs one pass and a vocabulary of 2^17 rows two.
 //
-// A list of up to 16384 entries is sorted in one launch by a cluster of eight CTAs (up to 1024: by
-// one CTA), which read each other's digit counts through distributed shared memory.  On one SM
-// alone the scattered stores are the limit: 16384 entries in two passes took 64 us there, and
-// take 19 us on eight.  The passes of a longer list cut it into at most 128 chunks, one CTA each.
+// A list of up to 8192 entries is sorted in one launch by a cluster of eight CTAs (up to 1024: by
+// one CTA), which read each other's digit counts through distributed shared memory (6001 entries
+// in two passes: 10 us).  Where an SM has more entries, its scattered stores are the limit: 16384
+// took 64 us on one SM, 17 us on eight, and 14 us in three launches.  The passes of a longer list
+// cut it into at most 128 chunks, one CTA each.
 // The first kernel counts the digits of each chunk; the second sums those counts itself (every CTA
 // reads the whole chunks x digits table, which L2 holds), places its entries in order and counts
 // the next digit of each in the chunk that it is placed in.
@@ -24,7 +25,7 @@ constexpr int kSortMaxChunks = 128;
 constexpr int kTeamThreads = 1024;                       // CTAs of a cluster that sorts alone
 constexpr int kTeamWarps = kTeamThreads / 32;
 constexpr int kTeamCtas = 8;
-constexpr int64_t kTeamMost = 2 * kTeamThreads * kTeamCtas;
+constexpr int64_t kTeamMost = kTeamThreads * kTeamCtas;
 constexpr int kSortMaxBits = 11;
 constexpr int kSortMaxBins = 1 << kSortMaxBits;
 constexpr int64_t kSortMaxEntries = 0x7fffffff - (1 << 25);  // positions are int32
@@ -366,11 +367,10 @@ __device__ inline int cluster_load(const int* p, unsigned rank) {
   return v;
 }
 
-// A list that a cluster sorts (gridDim.x CTAs, all of one cluster).  CTA c takes `chunk` entries,
-// its warps stretches of kRounds * 32, 32 in a round, so that (CTA, warp, round, lane) is the
-// order of the list.  The counters of the warps are summed per digit in place, those of the CTAs
-// through distributed shared memory.
-template <class I, class Out, int kRounds>
+// A list that a cluster sorts (gridDim.x CTAs, all of one cluster).  CTA c takes `chunk` entries, a
+// thread one of them, so that (CTA, warp, lane) is the order of the list.  The counters of the
+// warps are summed per digit in place, those of the CTAs through distributed shared memory.
+template <class I, class Out>
 __global__ void __launch_bounds__(kTeamThreads)
 sort_team_kernel(FromIds<I> ids, Out out, int n, int chunk, int bits, int passes, Entry* list0,
                  Entry* list1, uint8_t* clear, int64_t n_clear, int32_t* counter) {
@@ -385,29 +385,22 @@ sort_team_kernel(FromIds<I> ids, Out out, int n, int chunk, int bits, int passes
   uint32_t* cnt2 = reinterpret_cast<uint32_t*>(total + bins);  // two 16-bit counters a word
   uint16_t* mine = reinterpret_cast<uint16_t*>(cnt2) + warp * bins;
   const int lo = static_cast<int>(me) * chunk, hi = n - lo < chunk ? n : lo + chunk;
-  const int first = lo + warp * (kRounds * 32) + (threadIdx.x & 31);  // entry of round 0
-  for (int64_t i = me * kTeamThreads + threadIdx.x; i < (n_clear + 15) / 16;
-       i += ctas * kTeamThreads)
-    reinterpret_cast<uint4*>(clear)[i] = make_uint4(0, 0, 0, 0);
+  const int i = lo + static_cast<int>(threadIdx.x);  // this thread's entry
+  for (int64_t c = me * kTeamThreads + threadIdx.x; c < (n_clear + 15) / 16;
+       c += ctas * kTeamThreads)
+    reinterpret_cast<uint4*>(clear)[c] = make_uint4(0, 0, 0, 0);
   if (counter && me == 0 && threadIdx.x == 0) *counter = 0;
   for (int p = 0; p < passes; ++p) {
     const int shift = p * bits;
-    auto digit = [&](const Entry& x) { return (x.key >> shift) & (bins - 1); };
-    Entry e[kRounds];
-    int place[kRounds];
-#pragma unroll
-    for (int q = 0; q < kRounds; ++q) {
-      const int i = first + 32 * q;
-      if (i < hi) {
-        if (Out::kOnePass || p == 0) e[q] = ids(i);
-        else e[q] = load_entry(((p & 1) ? list0 : list1) + i);  // what pass p - 1 wrote
-      }
+    Entry e{0, 0};
+    if (i < hi) {
+      if (Out::kOnePass || p == 0) e = ids(i);
+      else e = load_entry(((p & 1) ? list0 : list1) + i);  // what pass p - 1 wrote
     }
-    for (int i = threadIdx.x; i < kTeamWarps * bins / 2; i += kTeamThreads) cnt2[i] = 0;
+    const unsigned digit = (e.key >> shift) & (bins - 1);
+    for (int c = threadIdx.x; c < kTeamWarps * bins / 2; c += kTeamThreads) cnt2[c] = 0;
     __syncthreads();
-#pragma unroll
-    for (int q = 0; q < kRounds; ++q)
-      place[q] = sort_rank(first + 32 * q < hi ? digit(e[q]) : 0xffffffffu, mine);
+    const int rank = sort_rank(i < hi ? digit : 0xffffffffu, mine);
     __syncthreads();
     for (int b = threadIdx.x; b < bins / 2; b += kTeamThreads) {
       uint32_t run = 0;
@@ -448,13 +441,10 @@ sort_team_kernel(FromIds<I> ids, Out out, int n, int chunk, int bits, int passes
       }
     }
     __syncthreads();
-#pragma unroll
-    for (int q = 0; q < kRounds; ++q) {
-      if (first + 32 * q < hi) {
-        const int dst = place[q] + off[digit(e[q])] + mine[digit(e[q])];
-        if (Out::kOnePass || last) out(e[q], dst);
-        else ((p & 1) ? list1 : list0)[dst] = e[q];
-      }
+    if (i < hi) {
+      const int dst = rank + off[digit] + mine[digit];
+      if (Out::kOnePass || last) out(e, dst);
+      else ((p & 1) ? list1 : list0)[dst] = e;
     }
     // what was placed is read by other CTAs, and no CTA may end or count anew while its counts are
     cluster_barrier();
@@ -525,10 +515,10 @@ inline int64_t sort_bytes(int64_t n, int64_t n_keys) {
          align256(s.passes * s.chunks * s.bins * 4);
 }
 
-template <class I, class Out, int kRounds>
+template <class I, class Out>
 int sort_team(const FromIds<I>& ids, int64_t n, const Out& out, const SortShape& s, Entry** list,
               uint8_t* clear, int64_t n_clear, int32_t* counter, cudaStream_t st) {
-  auto kernel = &sort_team_kernel<I, Out, kRounds>;
+  auto kernel = &sort_team_kernel<I, Out>;
   auto smem = [](int bins) {
     return bins * (2 * sizeof(int) + kTeamWarps * sizeof(uint16_t));
   };
@@ -546,8 +536,7 @@ int sort_team(const FromIds<I>& ids, int64_t n, const Out& out, const SortShape&
   config.stream = st;
   config.attrs = how;
   config.numAttrs = 2;
-  const int64_t step = 32 * kRounds;
-  const int chunk = static_cast<int>((n + ctas * step - 1) / (ctas * step) * step);
+  const int chunk = static_cast<int>((n + ctas * 32 - 1) / (ctas * 32) * 32);
   cudaLaunchKernelEx(&config, kernel, ids, out, static_cast<int>(n), chunk, s.bits, s.passes,
                      list[0], list[1], clear, n_clear, counter);
   return launch_status();
@@ -579,9 +568,7 @@ int sort_ids(const IdKeys<I>& ids, int64_t n, const Out& out, uint8_t* clear, in
         return launch_behind(&sort_few_kernel<I, Out>, dim3(1), kFewMost, 0, st, from_ids, out, n,
                              clear, n_clear, counter);
     }
-    auto go = [&](auto run) { return run(from_ids, n, out, s, list, clear, n_clear, counter, st); };
-    if (n <= kTeamThreads * kTeamCtas) return go(&sort_team<I, Out, 1>);
-    return go(&sort_team<I, Out, 2>);
+    return sort_team<I, Out>(from_ids, n, out, s, list, clear, n_clear, counter, st);
   }
   int* counts = reinterpret_cast<int*>(ws);
   const size_t smem = sort_smem(s.bins);

@@ -231,8 +231,8 @@ PATTERNS = {
     "few and same": (torch.full((250,), 3), 4),
     "team of one": (torch.from_numpy(np.random.default_rng(5).zipf(1.3, 1024) % 30000), 30000),
     "team": (torch.from_numpy(np.random.default_rng(5).zipf(1.3, 1025) % 30000), 30000),
-    "full team": (torch.from_numpy(np.random.default_rng(6).zipf(1.3, 16384) % 30000), 30000),
-    "no team": (torch.from_numpy(np.random.default_rng(7).zipf(1.3, 16385) % 30000), 30000),
+    "full team": (torch.from_numpy(np.random.default_rng(6).zipf(1.3, 8192) % 30000), 30000),
+    "no team": (torch.from_numpy(np.random.default_rng(7).zipf(1.3, 8193) % 30000), 30000),
     "two passes": (torch.from_numpy(np.random.default_rng(3).zipf(1.2, 9001) % 40000), 40000),
     "many chunks": (torch.from_numpy(np.random.default_rng(4).zipf(1.1, 140001) % 3000), 3000),
 }
@@ -299,14 +299,14 @@ def test_embedding_grad_masked_tokens(n, ignore):
 def test_embedding_grad_three_digit_vocabulary():
     """A vocabulary of more than 2^22 rows is sorted in three passes."""
     vocab = (1 << 22) + 1000
-    for n in (100, 5000, 10000, 17000):
+    for n in (100, 5000, 9000, 70000):
         tokens = torch.randint(0, vocab, (n,), device="cuda")
         tokens[:3] = torch.tensor([vocab - 1, 0, vocab - 1])
         g = randn(n, 4)
         got = fs.flagsparse_embedding_grad(tokens, g, vocab)
         want = torch.zeros(vocab, 4, dtype=torch.float64, device="cuda")
         want.index_add_(0, tokens, g.double())
-        assert (got - want).abs().max() < 1e-5       # at most ten rows of a token, each below 6
+        assert (got - want).abs().max() < 1e-5       # at most a few rows of a token, each below 6
         assert torch.equal(got != 0, want != 0)
     fs.check_selection_ids()
 
