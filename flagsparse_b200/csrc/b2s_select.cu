@@ -969,12 +969,12 @@ constexpr int64_t kMaxGrid = 0x7fffffff;
 // How the sorted list is cut: ranges of 24 entries (rows that are also read and written take
 // longer than others: the more ranges a warp slot gets, the more even the work; with ranges of 64
 // the sums above took 127 us, with 16 the joining of runs grew by what they gained), longer ones
-// where every slot has eight ranges already, and down to 2 entries where half the slots would have
-// none (256 tokens: 7.7 us with ranges of 2, 10 us with 8).
+// where every slot has eight ranges already, and down to 2 entries where three quarters of the
+// slots would have none (256 tokens: 7.7 us with ranges of 2, 10 us with 8).
 inline int64_t grad_ranges(int64_t n, int64_t slabs, int64_t ctas_per_sm) {
   const int64_t slots = 148 * ctas_per_sm * kSelWarps;
   const int64_t most = std::min(8 * slots / slabs, ceil_div(n, 24));
-  const int64_t least = std::min(slots / (2 * slabs), ceil_div(n, 2));
+  const int64_t least = std::min(slots / (4 * slabs), ceil_div(n, 2));
   return std::max<int64_t>(std::max(most, least), 1);
 }
 struct GradLayout {

@@ -646,6 +646,73 @@ def test_other_streams_and_a_freed_route():
     assert torch.equal(back, (x.float() * 4).bfloat16())
 
 
+def test_kernels_wait_for_the_ones_before_them():
+    """Kernels are put in place while their inputs are still being written: long ones in front of
+    short ones, and inputs that change between calls."""
+    n, k, dim, vocab = 8192, 8, 1024, 9000
+    experts = random_experts(n, k, 32)
+    x = torch.zeros(n, dim, dtype=torch.bfloat16, device="cuda")
+    tokens = torch.randperm(vocab, device="cuda")[:n]
+    table = torch.zeros(vocab, dim, dtype=torch.bfloat16, device="cuda")
+    results = []
+    for turn in range(1, 9):
+        x.fill_(turn)
+        table.fill_(2 * turn)
+        r = fs.prepare_token_route(experts, 32)
+        rows = fs.flagsparse_token_dispatch(x, r)
+        out = fs.flagsparse_token_combine(rows, r)
+        gy, gw = fs.flagsparse_token_combine_grad(out, rows, r, torch.ones(n, k, device="cuda"))
+        picked = fs.flagsparse_embedding(tokens, table)
+        grad = fs.flagsparse_embedding_grad(tokens, picked, vocab)
+        results.append((turn, out, gy, gw, picked, grad))
+        experts = experts.roll(1, 0)
+    for turn, out, gy, gw, picked, grad in results:
+        assert torch.equal(out, torch.full_like(out, 8 * turn))
+        assert torch.equal(gy, torch.full_like(gy, 8 * turn))
+        assert torch.equal(gw, torch.full_like(gw, 8 * turn * turn * dim))
+        assert torch.equal(picked, torch.full_like(picked, 2 * turn))
+        want = torch.zeros_like(grad)
+        want[tokens] = 2 * turn
+        assert torch.equal(grad, want)
+
+
+def test_random_calls():
+    """Sizes, types, layouts and masks at random (the calls above, held to the same bounds)."""
+    import random
+    for seed in range(150):
+        rng = random.Random(seed)
+        torch.manual_seed(seed)
+        dtype, index = rng.choice(TYPES), rng.choice([torch.int32, torch.int64])
+        dim = rng.choice([1, 2, 7, 8, 33, 64, 100, 255, 256, 257, 512, 513, 1030])
+
+        def matrix(rows):
+            pad, off = rng.choice([0, 0, 1, 3, 8]), rng.choice([0, 0, 1, 2, 8])
+            return torch.randn(rows, off + dim + pad, device="cuda").to(dtype)[:, off:off + dim]
+
+        if seed % 2:
+            n, vocab = int(2**rng.uniform(0, 14)), int(2**rng.uniform(0, 12))
+            tokens = (torch.rand(n, device="cuda")**rng.choice([1, 4, 20]) * vocab).to(index)
+            ignore = rng.choice([None, rng.randrange(vocab)])
+            g = matrix(n)
+            got = fs.flagsparse_embedding_grad(tokens, g, vocab, alpha=0.5, ignore_index=ignore)
+            total, terms, m = plain_grad(tokens, g, vocab, 0.5, ignore=ignore)
+            assert_close(got, total, terms, m)
+            continue
+        n, k, n_experts = int(2**rng.uniform(0, 10)), rng.choice([1, 2, 3, 8, 33]), 64
+        experts = random_experts(n, k, n_experts, rng.choice([0.0, 0.2, 1.0]), seed, index)
+        r = fs.prepare_token_route(experts, n_experts)
+        slots, indptr, _ = plain_route(experts, n_experts)
+        assert torch.equal(r.slots.cpu().long(), slots)
+        live, held = slots >= 0, int(indptr[-1])
+        y, w = matrix(n * k), torch.randn(n, k, device="cuda")
+        y[held:] = float("nan")
+        picked = torch.where(live[..., None], cpu(y)[torch.where(live, slots, 0)], 0.0)
+        parts = torch.where(live, cpu(w), 0.0)[..., None] * picked
+        assert_close(fs.flagsparse_token_combine(y, r, w), parts.sum(1), parts.abs().sum(1), 2 * k)
+        assert_close(fs.flagsparse_token_dispatch_grad(y, r), picked.sum(1), picked.abs().sum(1), k)
+    fs.check_selection_ids()
+
+
 def test_captured_and_replayed_with_new_inputs():
     """Two graphs of the same calls, replayed in turn on changed inputs, keep their own
     workspaces; ids outside their range are reported after a replay."""
