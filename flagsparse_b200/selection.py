@@ -298,7 +298,7 @@ def flagsparse_embedding(tokens, table, alpha=1.0, ignore_index=None, out=None, 
         _refuse_capture()
         if beta != 0:
             raise ValueError("beta != 0 requires out= holding the rows to scale")
-        return _Embedding.apply(tokens, table, alpha, has_ignore, ignore)
+        return _Embedding.apply(tokens, table, alpha, ignore_index)
     return _embedding(tokens, table, alpha, has_ignore, ignore, out, beta, index)
 
 
@@ -384,10 +384,10 @@ def flagsparse_embedding_grad(tokens, grad, n_rows, alpha=1.0, ignore_index=None
 
 class _Embedding(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, tokens, table, alpha, has_ignore, ignore):
+    def forward(ctx, tokens, table, alpha, ignore_index):   # (gradients are disabled in here)
         ctx.save_for_backward(tokens)
-        ctx.args = (table.shape[0], alpha, ignore if has_ignore else None)
-        return _embedding(tokens, table, alpha, has_ignore, ignore, None, 0.0, table.get_device())
+        ctx.args = (table.shape[0], alpha, ignore_index)
+        return flagsparse_embedding(tokens, table, alpha, ignore_index)
 
     @staticmethod
     @once_differentiable
@@ -396,7 +396,7 @@ class _Embedding(torch.autograd.Function):
         n_rows, alpha, ignore = ctx.args
         grad_table = flagsparse_embedding_grad(ctx.saved_tensors[0], grad, n_rows, alpha=alpha,
                                                ignore_index=ignore)
-        return None, grad_table, None, None, None
+        return None, grad_table, None, None
 
 
 # -------------------------------------------------------------------------------------------------
@@ -696,7 +696,7 @@ class _Dispatch(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, route):
         ctx.route = route
-        return _dispatch(x, route, None)
+        return flagsparse_token_dispatch(x, route)
 
     @staticmethod
     @once_differentiable
@@ -713,12 +713,15 @@ class _Combine(torch.autograd.Function):
         ctx.wants_weights = wants_weights
         # y is read by the gradient of the weights only
         ctx.save_for_backward(y if wants_weights else None, weights)
-        return _combine(y, route, weights, alpha, None, 0.0)
+        return flagsparse_token_combine(y, route, weights, alpha)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
         _refuse_capture()
         y, weights = ctx.saved_tensors
-        grad_y, grad_w = _combine_grad(grad, y, ctx.route, weights, ctx.alpha, ctx.wants_weights)
+        if ctx.wants_weights:
+            grad_y, grad_w = flagsparse_token_combine_grad(grad, y, ctx.route, weights, ctx.alpha)
+        else:
+            grad_y, grad_w = _combine_grad(grad, None, ctx.route, weights, ctx.alpha, False)
         return grad_y, grad_w, None, None
