@@ -41,7 +41,8 @@ int32_t* clean_status(int device) {
   return *reinterpret_cast<volatile int32_t*>(status_of[device]) ? nullptr : status_of[device];
 }
 
-// a plain CUDA tensor that no transform or mode has wrapped, or NULL
+// a plain CUDA tensor that no transform or mode has wrapped and that has no tangent (forward-mode
+// derivatives: such a tensor does not require a gradient), or NULL
 const at::Tensor* plain(PyObject* o) {
   if (!THPVariable_CheckExact(o) && Py_TYPE(o) != parameter_type) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
@@ -50,7 +51,7 @@ const at::Tensor* plain(PyObject* o) {
   if (keys.has(c10::DispatchKey::Python) || keys.has(c10::DispatchKey::FuncTorchBatched) ||
       keys.has(c10::DispatchKey::FuncTorchGradWrapper) ||
       keys.has(c10::DispatchKey::Functionalize) || keys.has(c10::DispatchKey::Conjugate) ||
-      keys.has(c10::DispatchKey::Negative))
+      keys.has(c10::DispatchKey::Negative) || t._fw_grad(0).defined())
     return nullptr;
   return &t;
 }

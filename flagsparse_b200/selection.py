@@ -18,7 +18,8 @@ FlagSparse has no counterpart (its gather / scatter take one vector, gather_scat
 The lookup, the dispatch and the combine are differentiable: when an input requires a gradient
 and gradients are enabled they record themselves for ``torch.autograd``.  Inside a CUDA graph
 capture that is refused (autograd may run a leaf's accumulation on a stream outside the capture);
-captured training steps call the ``*_grad`` functions.
+captured training steps call the ``*_grad`` functions.  Forward-mode derivatives are not
+supported: a tensor with a tangent is refused.
 
 Nothing synchronises.  Ids are checked by the kernels: one outside its range selects nothing, and
 IndexError is raised by the next call on that device that takes ids (a lookup, its gradient, a
@@ -31,6 +32,7 @@ import ctypes
 import threading
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -132,6 +134,13 @@ def _check_values(t, name):
         raise TypeError(f"{name} must be a torch.Tensor")
     if t.dtype not in SUPPORTED_SELECTION_VALUE_DTYPES:
         raise TypeError(f"{name} dtype must be one of: float16, bfloat16, float32, float64")
+    _refuse_tangent(t, name)
+
+
+def _refuse_tangent(t, name):
+    # (such a tensor does not require a gradient: without this its tangent would be lost)
+    if unpack_dual(t).tangent is not None:
+        raise NotImplementedError(f"{name} has a tangent: forward-mode derivatives are not supported")
 
 
 def _check_first_device(t, name):
@@ -175,6 +184,7 @@ def _refuse_capture():
 
 
 def _refuse_out(out, t, other=None):
+    _refuse_tangent(out, "out")
     if _wants_grad(out, t) or _wants_grad(out, other):
         raise RuntimeError("out= does not support automatic differentiation, but one of the "
                            "arguments requires grad")

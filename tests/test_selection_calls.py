@@ -1,0 +1,36 @@
+"""Selection products on the CPU: calls beside the usual one, up to where the device begins."""
+
+import pytest
+import torch
+
+import flagsparse_b200 as fs
+from flagsparse_b200 import selection
+
+TOK = torch.zeros(3, dtype=torch.int64)
+TABLE = torch.zeros(5, 4)
+
+
+def _route(n_tokens=3, k=2, n_experts=4):
+    n = n_tokens * k
+    return fs.TokenRoute(torch.zeros(2 * n + n_experts + 1, dtype=torch.int32), n_tokens, k,
+                         n_experts, 0)
+
+
+def test_tangents_are_refused():
+    import torch.autograd.forward_ad as forward
+    r, x, y, w = _route(), torch.zeros(3, 4), torch.zeros(6, 4), torch.zeros(3, 2)
+    with forward.dual_level():
+        dual = lambda t: forward.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: fs.flagsparse_embedding(TOK, dual(TABLE)),
+                     lambda: fs.flagsparse_embedding_grad(TOK, dual(x), 5),
+                     lambda: fs.flagsparse_token_dispatch(dual(x), r),
+                     lambda: fs.flagsparse_token_dispatch_grad(dual(y), r),
+                     lambda: fs.flagsparse_token_combine(dual(y), r, w),
+                     lambda: fs.flagsparse_token_combine(y, r, dual(w)),
+                     lambda: fs.flagsparse_token_combine_grad(dual(x), y, r, w),
+                     lambda: fs.flagsparse_token_combine_grad(x, y, r, dual(w)),
+                     lambda: fs.flagsparse_embedding(TOK, TABLE, out=dual(x))):
+            with pytest.raises(NotImplementedError, match="tangent"):
+                call()
+        with pytest.raises(ValueError, match="must be a CUDA tensor"):
+            fs.flagsparse_embedding(TOK, TABLE)

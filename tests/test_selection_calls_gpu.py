@@ -1,0 +1,58 @@
+"""Selection products on the GPU: calls beside the usual one.  What has to be refused, what a mask
+leaves, views of other tensors, the interpreter during a launch, and the forms of the gradient and
+of the combine that take 16 bytes at a time.  Bounds as in test_selection_gpu.py."""
+
+import numpy as np
+import pytest
+import torch
+
+import flagsparse_b200 as fs
+from flagsparse_b200 import selection
+from test_selection_gpu import (PATTERNS, TYPES, assert_close, cpu, ids, plain_grad, plain_route,
+                                randn, random_experts)
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True, params=["host module", "python"])
+def way(request, monkeypatch):
+    """Every test runs with the calls made by the C++ host module and by the Python code."""
+    if request.param == "python":
+        monkeypatch.setattr(selection, "_host", None)
+    return request.param
+
+
+def test_tangents_are_refused():
+    """A result without the tangent of its input would stand for a derivative of zero."""
+    import torch.autograd.forward_ad as forward
+    tokens = torch.tensor([1, 3, 3], device="cuda")
+    r = fs.prepare_token_route(torch.tensor([[0, 1], [1, -1], [1, 0]], device="cuda"), 2)
+    table, x, y, w = randn(4, 8), randn(3, 8, seed=1), randn(6, 8, seed=2), randn(3, 2, seed=3)
+    fs.flagsparse_embedding(tokens, table)                   # (the usual call is bound by now)
+    with forward.dual_level():
+        dual = lambda t: forward.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for call in (lambda: fs.flagsparse_embedding(tokens, dual(table)),
+                     lambda: fs.flagsparse_embedding(tokens, dual(torch.nn.Parameter(table))),
+                     lambda: fs.flagsparse_embedding_grad(tokens, dual(x), 4),
+                     lambda: fs.flagsparse_token_dispatch(dual(x), r),
+                     lambda: fs.flagsparse_token_dispatch_grad(dual(y), r),
+                     lambda: fs.flagsparse_token_combine(dual(y), r, w),
+                     lambda: fs.flagsparse_token_combine(y, r, dual(w)),
+                     lambda: fs.flagsparse_token_combine_grad(dual(x), y, r, w),
+                     lambda: fs.flagsparse_token_combine_grad(x, dual(y), r, w),
+                     lambda: fs.flagsparse_token_combine_grad(x, y, r, dual(w)),
+                     lambda: fs.flagsparse_embedding(tokens, table, out=dual(x)),
+                     lambda: fs.flagsparse_embedding_grad(tokens, x, 4, out=dual(table)),
+                     lambda: fs.flagsparse_token_dispatch(x, r, out=dual(y)),
+                     lambda: fs.flagsparse_token_combine(y, r, out=dual(x))):
+            with pytest.raises(NotImplementedError, match="tangent"):
+                call()
+        assert torch.equal(fs.flagsparse_embedding(tokens, table), table[tokens])
+        assert torch.equal(fs.flagsparse_token_dispatch(x, r)[0], x[0])
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda t: fs.flagsparse_embedding(tokens, t), (table,),
+                       (torch.ones_like(table),))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda t: fs.flagsparse_embedding(tokens, t))(table[None])
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda t: fs.flagsparse_embedding(tokens, t).sum())(table)
