@@ -733,7 +733,8 @@ __device__ inline typename acc_of<T>::type route_weight(const void* w, bool w_is
 // out[t] = alpha * sum_j w[t, j] * y[slots[t, j]] + beta * out[t].  A warp takes a range of tokens
 // and one slab of columns; the assignments of its tokens are one stretch of `slots`, read 32 at a
 // time and a stretch ahead, and their rows stream through the warp's queue without a pause
-// between tokens.  A masked assignment is a part of zeros with weight zero.  (8192 x 8 rows of 4096
+// between tokens.  A masked assignment is a part of zeros with weight zero; a token that has no
+// other is beta * out whatever alpha is (alpha * 0 is not zero where alpha is not finite).  (8192 x 8 rows of 4096
 // bf16: 101 us, 6.0 TB/s; 16384 x 4 rows of 2048: 55 us, 6.1 TB/s.  With 16 bytes a lane and a wait
 // for every row, 134 us: 82 % of the issue slots were taken.)
 template <class T, int VE>
@@ -768,16 +769,19 @@ route_combine_kernel(const T* y, int64_t ld_y, const int32_t* slots,
   const uint32_t rows = static_cast<uint32_t>(n * k);
 
   // stretches of 32 assignments: the one that rows are asked for from, the one behind it; the
-  // weights of the one that is summed from, and of the one behind it
+  // weights of the one that is summed from, and which of them are not masked, and of the one behind
   auto slot_of = [&](int a) {  // a valid slot, or -1
     const int32_t s = a < count ? my_slots[a] : -1;
     return static_cast<uint32_t>(s) < rows ? s : -1;
   };
-  auto weight_of = [&](int a) {
-    return slot_of(a) >= 0 ? route_weight<T>(weights, w_is_f32, w0 + a) : A(0);
+  auto weight_of = [&](int a, uint32_t* live) {
+    const bool held = slot_of(a) >= 0;
+    *live = __ballot_sync(0xffffffffu, held);
+    return held ? route_weight<T>(weights, w_is_f32, w0 + a) : A(0);
   };
   int32_t ask_slot = slot_of(lane), next_slot = slot_of(32 + lane);
-  A weight = weight_of(lane), next_weight = weight_of(32 + lane);
+  uint32_t live, next_live;
+  A weight = weight_of(lane, &live), next_weight = weight_of(32 + lane, &next_live);
   int ask = 0;
   auto send = [&] {
 #pragma unroll
@@ -797,22 +801,27 @@ route_combine_kernel(const T* y, int64_t ld_y, const int32_t* slots,
   acc.clear();
   if (k == 0)
     for (; t < t1; ++t)
-      store_axpby<T, VE, A, E>(out + t * ld_out, col0, dim, acc, alpha, has_beta, beta);
+      store_axpby<T, VE, A, E>(out + t * ld_out, col0, dim, acc, A(1), has_beta, beta);
   int j = 0;
+  uint32_t any = 0;  // whether the token has an assignment that is not masked
   for (int a = 0; a < count; a += B) {
     send();
     if ((a & 31) == 0 && a > 0) {
       weight = next_weight;
-      next_weight = weight_of(a + 32 + lane);
+      live = next_live;
+      next_weight = weight_of(a + 32 + lane, &next_live);
     }
     queue.wait();
 #pragma unroll
     for (int q = 0; q < B; ++q) {
       acc.fma(__shfl_sync(0xffffffffu, weight, (a + q) & 31), queue.part(q));
+      any |= (live >> ((a + q) & 31)) & 1;
       if (++j == k) {
         if (a + q < count)
-          store_axpby<T, VE, A, E>(out + t * ld_out, col0, dim, acc, alpha, has_beta, beta);
+          store_axpby<T, VE, A, E>(out + t * ld_out, col0, dim, acc, any ? alpha : A(1), has_beta,
+                                   beta);
         acc.clear();
+        any = 0;
         j = 0;
         ++t;
       }
@@ -845,6 +854,7 @@ route_combine_plain_kernel(const T* y, int64_t ld_y,
   const int col0 = static_cast<int>(slab) * kSelCols;
   Sums<A, 8> acc;
   acc.clear();
+  bool any = false;  // whether the token has an assignment that is not masked
   for (int c = 0; c < k; c += 32) {
     int32_t my_slot = -1;
     A my_weight = A(0);
@@ -865,11 +875,14 @@ route_combine_plain_kernel(const T* y, int64_t ld_y,
 #pragma unroll
       for (int q = 0; q < kAhead; ++q) {
         const A w = __shfl_sync(0xffffffffu, my_weight, (j0 + q) & 31);
-        if (is_row(s[q], n * k)) acc.fma(w, r[q]);
+        if (is_row(s[q], n * k)) {
+          acc.fma(w, r[q]);
+          any = true;
+        }
       }
     }
   }
-  store_axpby<T, 1, A, 8>(out + t * ld_out, col0, dim, acc, alpha, has_beta, beta);
+  store_axpby<T, 1, A, 8>(out + t * ld_out, col0, dim, acc, any ? alpha : A(1), has_beta, beta);
 }
 
 // grad_y[slots[a]] = alpha * w[a] * g[a / k], grad_w[a] = alpha * <g[a / k], y[slots[a]]>: one
@@ -921,7 +934,8 @@ route_combine_grad_kernel(const T* g, int64_t ld_g, const T* y,
     }
   }
   if (grad_w) {
-    dot = alpha * group_sum(dot, 32);
+    dot = group_sum(dot, 32);
+    if (is_row(s, n * k)) dot = alpha * dot;  // (a masked one is zero whatever alpha is)
     if (lane == 0) {
       if (w_is_f32)
         static_cast<float*>(grad_w)[a] = static_cast<float>(dot);

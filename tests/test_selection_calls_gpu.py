@@ -56,3 +56,38 @@ def test_tangents_are_refused():
         torch.func.vmap(lambda t: fs.flagsparse_embedding(tokens, t))(table[None])
     with pytest.raises(RuntimeError):
         torch.func.grad(lambda t: fs.flagsparse_embedding(tokens, t).sum())(table)
+
+
+@pytest.mark.parametrize("alpha", [float("inf"), float("nan"), -2.0])
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("n, k, dim", [(3, 2, 264), (3, 2, 33), (6000, 5, 264), (900, 37, 5),
+                                       (40, 3, 4096), (4, 0, 16)])
+def test_a_mask_that_leaves_nothing_meets_no_alpha(dtype, alpha, n, k, dim):
+    """A token without assignments gets beta * out, the weight of a masked one a gradient of zero,
+    also where alpha is not finite.  The other tokens' sums are a quarter at least: alpha decides
+    on which side of beta * out they lie."""
+    rng = np.random.default_rng(n + k)
+    experts = random_experts(n, k, 7, 0.3, seed=n)
+    experts[torch.from_numpy(rng.random(n) < 0.5).cuda()] = -1
+    r = fs.prepare_token_route(experts, 7)
+    none = (experts < 0).all(1)
+    y = randn(n * k, dim, dtype=dtype).abs() + 0.5
+    w = randn(n, k, dtype=dtype, seed=1).abs() + 0.5
+    for weights in (None, w, w.float()):
+        got = fs.flagsparse_token_combine(y, r, weights, alpha=alpha)
+        assert torch.equal(got[none], torch.zeros_like(got[none]))
+        out = torch.full((n, dim), 3.0, dtype=dtype, device="cuda")
+        fs.flagsparse_token_combine(y, r, weights, alpha=alpha, beta=0.5, out=out)
+        assert torch.equal(out[none], torch.full_like(out[none], 1.5))
+        for rest, beside in ((got[~none], 0.0), (out[~none], 1.5)):
+            assert (rest.isnan() if alpha != alpha
+                    else rest == alpha if alpha > 0 else rest < beside).all()
+        if weights is not None:
+            g = torch.ones(n, dim, dtype=dtype, device="cuda")
+            gy, gw = fs.flagsparse_token_combine_grad(g, y, r, weights, alpha=alpha)
+            gone = experts < 0
+            assert torch.equal(gw[gone], torch.zeros_like(gw[gone]))
+            assert (gw[~gone].isnan() if alpha != alpha
+                    else gw[~gone].sign() == np.sign(alpha)).all()
+            held = int(r.indptr[-1])
+            assert not gy[held:].any() and gy[:held].all()
