@@ -212,7 +212,14 @@ def _refuse_overlap(out, *inputs):
 
 def _rows(t):
     """`t` (2-D) with unit stride inside a row and rows that do not overlap; copied if need be."""
+    t = _as_stored(t)
     return t if t.is_contiguous() or _row_major_ok(t) else t.contiguous()
+
+
+def _as_stored(t):
+    """`t` with the values that its memory holds: a view that stands for the negative of them (the
+    imaginary part of a conjugate) is written out."""
+    return t.resolve_neg() if t.is_neg() else t
 
 
 def _pitch(t):
@@ -221,7 +228,7 @@ def _pitch(t):
 
 def _result(out, shape, like, dtype, beta):
     """(tensor the kernels write, its address, its pitch) for the result of a call: a new tensor,
-    `out` itself, or (when the kernels cannot write its layout) a contiguous stand-in, which
+    `out` itself, or (when the kernels cannot write it as it lies) a contiguous stand-in, which
     _finish copies into `out`.  `like`: a tensor on the device."""
     if out is None:
         if beta != 0:
@@ -236,7 +243,7 @@ def _result(out, shape, like, dtype, beta):
             flat = out.view(-1 if out.numel() else 0, shape[-1])
         except RuntimeError:
             flat = None
-    if flat is None or not _row_major_ok(flat):
+    if flat is None or out.is_neg() or not _row_major_ok(flat):
         flat = out.clone(memory_format=torch.contiguous_format) if beta != 0 else like.new_empty(
             shape, dtype=dtype)
         return flat, flat.data_ptr(), shape[-1]
@@ -638,8 +645,7 @@ def _combine(y, route, weights, alpha, out, beta):
     y = _rows(y)
     wcode, waddress = 0, None
     if weights is not None:
-        if not weights.is_contiguous():
-            weights = weights.contiguous()
+        weights = _as_stored(weights).contiguous()
         wcode, waddress = _lib.VALUE_CODE[weights.dtype], weights.data_ptr()
     route._use()
     _call(route._index, _lib.load().b2s_route_combine, _lib.VALUE_CODE[y.dtype], y.data_ptr(),
@@ -687,8 +693,7 @@ def _combine_grad(grad, y, route, weights, alpha, want_weights):
     grad_w, wcode, waddress, gaddress = None, 0, None, None
     yaddress, ypitch = None, 0
     if weights is not None:
-        if not weights.is_contiguous():
-            weights = weights.contiguous()
+        weights = _as_stored(weights).contiguous()
         wcode, waddress = _lib.VALUE_CODE[weights.dtype], weights.data_ptr()
         if want_weights:
             y = _rows(y)

@@ -34,3 +34,16 @@ def test_tangents_are_refused():
                 call()
         with pytest.raises(ValueError, match="must be a CUDA tensor"):
             fs.flagsparse_embedding(TOK, TABLE)
+
+
+def test_views_that_stand_for_the_negative_are_written_out():
+    z = torch.complex(torch.arange(6.0).reshape(6, 1), torch.arange(6.0).reshape(6, 1) + 1)
+    view = z.conj().imag                                     # rows that a kernel could read as they lie
+    assert view.is_neg() and selection._row_major_ok(view)
+    for rows in (selection._rows(view), selection._as_stored(torch._neg_view((-view).resolve_neg()))):
+        assert not rows.is_neg() and torch.equal(rows, view)
+    assert selection._rows(TABLE) is TABLE
+    flat, address, _ = selection._result(view, (6, 1), view, torch.float32, 1.0)
+    assert address != view.data_ptr() and not flat.is_neg() and torch.equal(flat, view)
+    flat.fill_(5.0)
+    assert selection._finish(view, flat) is view and (view == 5).all() and (z.imag == -5).all()

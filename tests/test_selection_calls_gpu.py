@@ -91,3 +91,34 @@ def test_a_mask_that_leaves_nothing_meets_no_alpha(dtype, alpha, n, k, dim):
                     else gw[~gone].sign() == np.sign(alpha)).all()
             held = int(r.indptr[-1])
             assert not gy[held:].any() and gy[:held].all()
+
+
+def test_views_that_stand_for_the_negative():
+    """The imaginary part of a conjugate is a view with a sign that only PyTorch knows of."""
+    view = lambda n, seed: torch.complex(randn(n, 1, seed=seed),  # noqa: E731
+                                         randn(n, 1, seed=seed + 1)).conj().imag
+    table, x, y = view(9, 0), view(4, 2), view(8, 4)
+    assert table.is_neg() and table.stride(0) == 2
+    plain = lambda t: t.resolve_neg().contiguous()  # noqa: E731
+    tokens = torch.tensor([1, 8, 1, 4], device="cuda")
+    r = fs.prepare_token_route(torch.tensor([[0, 1], [1, -1], [1, 0], [0, 0]], device="cuda"), 2)
+    w = randn(4, 2)
+    same = lambda fn, *args: torch.equal(fn(*args), fn(*map(  # noqa: E731
+        lambda a: plain(a) if isinstance(a, torch.Tensor) and a.is_neg() else a, args)))
+    assert torch.equal(fs.flagsparse_embedding(tokens, table), plain(table)[tokens])
+    assert same(fs.flagsparse_embedding_grad, tokens, x, 9)
+    assert same(fs.flagsparse_token_dispatch, x, r)
+    assert same(fs.flagsparse_token_dispatch_grad, y, r)
+    assert same(fs.flagsparse_token_combine, y, r, w)
+    assert same(fs.flagsparse_token_combine, y, r, torch._neg_view(w))
+    for a, b in zip(fs.flagsparse_token_combine_grad(x, y, r, w),
+                    fs.flagsparse_token_combine_grad(plain(x), plain(y), r, w)):
+        assert torch.equal(a, b)
+    for beta in (0.0, 0.5):
+        out, want = view(4, 6), plain(view(4, 6))
+        assert fs.flagsparse_embedding(tokens, plain(table), out=out, beta=beta) is out
+        assert torch.equal(out, fs.flagsparse_embedding(tokens, plain(table), out=want, beta=beta))
+        out, want = view(9, 6), plain(view(9, 6))
+        assert fs.flagsparse_embedding_grad(tokens, plain(x), 9, out=out, beta=beta) is out
+        assert torch.equal(out, fs.flagsparse_embedding_grad(tokens, plain(x), 9, out=want,
+                                                             beta=beta))
