@@ -76,6 +76,16 @@ bool row_major(const at::Tensor& t, int64_t* pitch) {
   *pitch = rows > 1 ? t.stride(0) : cols;
   return (cols <= 1 || t.stride(1) == 1) && (rows <= 1 || *pitch >= (cols > 1 ? cols : 1));
 }
+// whether two arrays of rows of `dim` values have addresses in common (storage objects do not say:
+// one memory can have several of them); rows of one array side by side count as meeting
+bool meet(const at::Tensor& a, int64_t rows_a, int64_t pitch_a, const at::Tensor& b, int64_t rows_b,
+          int64_t pitch_b, int64_t dim) {
+  if (rows_a <= 0 || rows_b <= 0 || dim <= 0) return false;
+  const auto at_a = reinterpret_cast<uintptr_t>(a.const_data_ptr());
+  const auto at_b = reinterpret_cast<uintptr_t>(b.const_data_ptr());
+  return at_a < at_b + ((rows_b - 1) * pitch_b + dim) * b.element_size() &&
+         at_b < at_a + ((rows_a - 1) * pitch_a + dim) * a.element_size();
+}
 bool number(PyObject* o, double* v) {
   if (PyFloat_CheckExact(o)) {
     *v = PyFloat_AS_DOUBLE(o);
@@ -192,7 +202,8 @@ PyObject* embedding_grad(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       out = plain(a[5]);
       if (!out || out->get_device() != dev || out->dim() != 2 || out->size(0) != n_rows ||
           out->size(1) != dim || recorded(*out) || recorded(*grad) ||
-          out->storage().is_alias_of(grad->storage()) || !row_major(*out, &out_pitch))
+          !row_major(*out, &out_pitch) ||
+          meet(*out, n_rows, out_pitch, *grad, dim > 0 ? grad->numel() / dim : 0, pitch, dim))
         NOT_HERE;
       if (a[7] == Py_None) {
         if (out->scalar_type() != out_type && !(out->scalar_type() == at::kFloat &&

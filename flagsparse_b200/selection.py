@@ -191,22 +191,22 @@ def _refuse_out(out, t, other=None):
 
 
 def _refuse_overlap(out, *inputs):
-    """The kernels read their inputs while they write `out`."""
+    """The kernels read their inputs while they write `out`.  Addresses are compared: one memory
+    can have several storage objects (DLPack)."""
     for t in inputs:
-        if (t is None or not t.numel() or not out.numel()
-                or t.untyped_storage().data_ptr() != out.untyped_storage().data_ptr()):
+        if t is None or not t.numel() or not out.numel():
             continue
-        size = out.element_size()
-        ends = [(v.data_ptr(), v.data_ptr() + size * (1 + sum(
-            (n - 1) * abs(s) for n, s in zip(v.shape, v.stride())))) for v in (out, t)]
+        ends = [(v.data_ptr(), v.data_ptr() + v.element_size() * (1 + sum(
+            (n - 1) * s for n, s in zip(v.shape, v.stride())))) for v in (out, t)]
         if ends[0][1] <= ends[1][0] or ends[1][1] <= ends[0][0]:
             continue
         # rows of one array side by side: columns that do not meet
         if out.dim() == t.dim() == 2 and t.dtype == out.dtype and out.stride() == t.stride():
             pitch = out.stride(0)
-            apart = (ends[1][0] - ends[0][0]) // size % pitch
-            if out.stride(1) == 1 and out.shape[1] <= apart <= pitch - t.shape[1]:
-                continue
+            if pitch > 0 and out.stride(1) == 1:
+                apart = (ends[1][0] - ends[0][0]) // out.element_size() % pitch
+                if out.shape[1] <= apart <= pitch - t.shape[1]:
+                    continue
         raise ValueError("out must not overlap the tensors that are read")
 
 
@@ -327,10 +327,10 @@ def _embedding(tokens, table, alpha, has_ignore, ignore, out, beta, index):
         _check_size("the number of rows of table", n_rows, MAX_ROWS)
         _check_size("dim", dim, MAX_DIM)
     flat, address, pitch = _result(out, (*tokens.shape, dim), table, table.dtype, beta)
-    if out is not None:
-        _refuse_overlap(out, table)
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
+    if out is not None:
+        _refuse_overlap(out, table, tokens)
     table = _rows(table)
     _call(index, _lib.load().b2s_select_rows, _lib.VALUE_CODE[table.dtype],
           _lib.INDEX_CODE[tokens.dtype], tokens.data_ptr(), n, has_ignore, ignore,
@@ -383,7 +383,7 @@ def flagsparse_embedding_grad(tokens, grad, n_rows, alpha=1.0, ignore_index=None
     _check_size("n_rows", n_rows, MAX_ROWS)
     _check_size("dim", dim, MAX_DIM)
     flat, address, pitch = _result(out, (n_rows, dim), grad, out_dtype, beta)
-    if out is not None:
+    if out is not None:     # (the tokens have been read before a row is written)
         _refuse_overlap(out, grad)
     if not tokens.is_contiguous():
         tokens = tokens.contiguous()
@@ -575,7 +575,7 @@ def _dispatch(x, route, out):
     dim = x.shape[1]
     flat, address, pitch = _result(out, (route.n_rows, dim), x, x.dtype, 0.0)
     if out is not None:
-        _refuse_overlap(out, x)
+        _refuse_overlap(out, x, route._buffer)
     x = _rows(x)
     route._use()
     _call(route._index, _lib.load().b2s_route_dispatch, _lib.VALUE_CODE[x.dtype], x.data_ptr(),
@@ -641,7 +641,7 @@ def _combine(y, route, weights, alpha, out, beta):
     dim = y.shape[1]
     flat, address, pitch = _result(out, (route.n_tokens, dim), y, y.dtype, beta)
     if out is not None:
-        _refuse_overlap(out, y, weights)
+        _refuse_overlap(out, y, weights, route._buffer)
     y = _rows(y)
     wcode, waddress = 0, None
     if weights is not None:

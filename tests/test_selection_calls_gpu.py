@@ -122,3 +122,33 @@ def test_views_that_stand_for_the_negative():
         assert fs.flagsparse_embedding_grad(tokens, plain(x), 9, out=out, beta=beta) is out
         assert torch.equal(out, fs.flagsparse_embedding_grad(tokens, plain(x), 9, out=want,
                                                              beta=beta))
+
+
+def test_out_may_not_be_what_is_read_under_another_name():
+    """The addresses decide, not which storage object a tensor was made from."""
+    other = torch.from_dlpack
+    table, tokens = randn(20, 8), torch.arange(20, device="cuda")
+
+    def refused(fn, *args, **kwargs):
+        with pytest.raises(ValueError, match="must not overlap"):
+            fn(*args, **kwargs)
+
+    refused(fs.flagsparse_embedding_grad, tokens, table, 20, out=other(table), beta=1.0)
+    refused(fs.flagsparse_embedding_grad, tokens[:15], table[5:], 20, out=other(table))
+    refused(fs.flagsparse_embedding, tokens[:15], table, out=other(table[5:]))
+    words = torch.zeros(20, 2, dtype=torch.int32, device="cuda")
+    refused(fs.flagsparse_embedding, words[:10].view(-1), randn(3, 2), out=words.view(torch.float32))
+    r = fs.prepare_token_route(torch.zeros(10, 2, dtype=torch.int64, device="cuda"), 2)
+    refused(fs.flagsparse_token_dispatch, table[:10], r, out=other(table))
+    slots = r.slots.view(torch.float32)
+    refused(fs.flagsparse_token_combine, randn(20, 2), r, out=slots)
+    refused(fs.flagsparse_token_dispatch_grad, randn(20, 2), r, out=slots)
+    refused(fs.flagsparse_token_dispatch, randn(10, 1), r, out=slots.view(20, 1))
+    row = randn(1, 8).expand(20, 8)
+    refused(fs.flagsparse_embedding, tokens, row, out=row)
+    into = torch.zeros(20, 8, device="cuda")                 # neighbours are taken as before
+    both = torch.zeros(40, 8, device="cuda")
+    both[:20] = table
+    fs.flagsparse_embedding_grad(tokens, both[:20], 20, out=other(both[20:]))
+    fs.flagsparse_embedding_grad(tokens, table, 20, out=into)
+    assert torch.equal(both[20:], table) and torch.equal(into, table)
