@@ -30,6 +30,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
+from types import SimpleNamespace
 
 import torch
 from torch.autograd.forward_ad import unpack_dual
@@ -46,15 +47,44 @@ MAX_ROWS = 2**31 - 2
 MAX_DIM = 1 << 22
 
 
-# The usual call (plain strided tensors, a new result, nothing to record) is made by a C++ module
-# (csrc/host/b2s_host.cpp): it returns None for every other one, which then takes the way below.
-# Without the module all calls do; the kernels are the same.
-def _load_host():
+class _Host:
+    """The usual call (plain strided tensors, a new result, nothing to record) is made by a C++ module
+    (csrc/host/b2s_host.cpp): it returns None for every other one, which then takes the way below.
+    Without the module all calls do; the kernels are the same.
+
+    The module and the library are loaded by the first call and not when the package is imported:
+    a library that lacks an entry point can be built anew by the package that it belongs to.  Then
+    the module takes this object's place (an attribute of it costs a call 0.3 us less)."""
+
+    def __getattr__(self, name):
+        global _host
+        if name.startswith("__"):
+            raise AttributeError(name)
+        if not _lib.LIB_PATH.exists():  # the call itself will say so, behind its own checks
+            return _not_here
+        with _HOST_LOCK:
+            host = _bound_host()
+            if _host is self:
+                _host = host
+        return getattr(host, name)
+
+
+def _not_here(*args):
+    return None
+
+
+# in the place of a module that has not been built
+_NO_HOST = SimpleNamespace(**dict.fromkeys(
+    ("embedding", "embedding_grad", "route_plan", "dispatch", "combine", "combine_grad",
+     "bind_status"), _not_here))
+
+
+def _bound_host():
+    lib = _lib.load()
     try:
         from . import _b2s_host
     except ImportError:
-        return None
-    lib = _lib.load()
+        return _NO_HOST
     address = [ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
         "b2s_select_rows", "b2s_select_grad_bytes", "b2s_select_grad", "b2s_route_plan_bytes",
         "b2s_route_plan", "b2s_route_dispatch", "b2s_route_combine", "b2s_route_combine_grad")]
@@ -62,7 +92,8 @@ def _load_host():
     return _b2s_host
 
 
-_host = _load_host() if _lib.LIB_PATH.exists() else None
+_host = _Host()
+_HOST_LOCK = threading.Lock()
 
 _WORDS = {}
 _WORDS_LOCK = threading.Lock()

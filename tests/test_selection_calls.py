@@ -1,10 +1,15 @@
 """Selection products on the CPU: calls beside the usual one, up to where the device begins."""
 
+import shutil
+import subprocess
+import sys
+
 import pytest
 import torch
 
 import flagsparse_b200 as fs
-from flagsparse_b200 import selection
+from conftest import ROOT
+from flagsparse_b200 import _lib, selection
 
 TOK = torch.zeros(3, dtype=torch.int64)
 TABLE = torch.zeros(5, 4)
@@ -83,3 +88,54 @@ def test_out_may_not_be_the_tokens(monkeypatch):
     words = torch.zeros(8, 2, dtype=torch.int64)
     with pytest.raises(ValueError, match="must not overlap"):
         fs.flagsparse_embedding(words[0], TABLE[:, :2], out=words.view(torch.float32)[:2, :2])
+
+
+def _run(code, cwd):
+    return subprocess.run([sys.executable, "-c", code], cwd=cwd, capture_output=True, text=True,
+                          timeout=300)
+
+
+def test_importing_the_package_loads_no_library():
+    """The libraries come with the first call: whoever imports the package for something else (its
+    build command, a workload's description) does not depend on them."""
+    res = _run("import flagsparse_b200, flagsparse_b200._build\n"
+               "maps = open('/proc/self/maps').read()\n"
+               "assert 'libb200sparse' not in maps and '_b2s_host' not in maps\n"
+               "from flagsparse_b200 import selection\n"
+               "assert selection._host.embedding(1, 2, 3) is None\n"
+               "maps = open('/proc/self/maps').read()\n"
+               "assert 'libb200sparse' in maps and '_b2s_host' in maps\n", ROOT)
+    assert res.returncode == 0, res.stderr[-1500:]
+
+
+def test_a_library_without_an_entry_point_can_be_built_anew(tmp_path):
+    """Importing the package, and with it the build command, works beside a library that is older
+    than its declarations; the first call says what the library lacks."""
+    package = tmp_path / "flagsparse_b200"
+    package.mkdir()
+    for path in (ROOT / "flagsparse_b200").iterdir():
+        if path.suffix == ".py":
+            shutil.copy(path, package / path.name)
+        elif path.suffix == ".so":
+            (package / path.name).symlink_to(path)
+    with open(package / "_lib.py", "a") as f:
+        f.write("\nSIGNATURES['b2s_of_a_later_version'] = (c_int, [])\n")
+    res = _run("import torch, flagsparse_b200, flagsparse_b200._build\n"
+               "assert flagsparse_b200.__file__.startswith(%r)\n"
+               "try:\n"
+               "    flagsparse_b200.flagsparse_embedding(torch.zeros(1).long(), torch.zeros(1, 1))\n"
+               "except AttributeError as e:\n"
+               "    print(e)\n" % str(tmp_path), tmp_path)
+    assert res.returncode == 0 and "b2s_of_a_later_version" in res.stdout, res.stderr[-1500:]
+
+
+def test_without_the_host_module_or_the_library(tmp_path, monkeypatch):
+    monkeypatch.setitem(sys.modules, "flagsparse_b200._b2s_host", None)    # an ImportError
+    monkeypatch.delattr(fs, "_b2s_host", raising=False)
+    monkeypatch.setattr(selection, "_host", selection._Host())
+    assert selection._host.embedding(TOK, TABLE, 1.0, None) is None
+    assert selection._host is selection._NO_HOST             # for good: no call asks again
+    assert selection._host.bind_status(0, 0) is None
+    monkeypatch.setattr(selection, "_host", selection._Host())
+    monkeypatch.setattr(_lib, "LIB_PATH", tmp_path / "libb200sparse.so")
+    assert selection._host.combine() is None and type(selection._host) is selection._Host

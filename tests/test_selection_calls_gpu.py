@@ -19,6 +19,8 @@ def way(request, monkeypatch):
     """Every test runs with the calls made by the C++ host module and by the Python code."""
     if request.param == "python":
         monkeypatch.setattr(selection, "_host", None)
+    else:
+        assert selection._host.embedding is not selection._not_here      # it is built
     return request.param
 
 
