@@ -97,7 +97,8 @@ def build(force: bool = False, verbose: bool = False, extra_flags=(), checked: b
 
 
 def build_host(force: bool = False, verbose: bool = False) -> Path:
-    """_b2s_host.so from csrc/host/b2s_host.cpp (host code only; needs PyTorch's headers)."""
+    """_b2s_host.so from csrc/host/b2s_host.cpp (host code only; needs PyTorch's headers).  It is
+    built anew when the PyTorch it was built for (BUILD_DIR/host_torch_version) is another one."""
     import sysconfig
 
     import torch
@@ -105,13 +106,16 @@ def build_host(force: bool = False, verbose: bool = False) -> Path:
 
     src = CSRC / "host" / "b2s_host.cpp"
     header = PKG_DIR.parent / "include" / "b200sparse.h"
-    if force or _newer(HOST_LIB_PATH, [src, header]):
+    stamp = BUILD_DIR / "host_torch_version"
+    same = stamp.exists() and stamp.read_text() == torch.__version__
+    if force or not same or _newer(HOST_LIB_PATH, [src, header]):
         torch_lib = Path(torch.__file__).resolve().parent / "lib"
         cuda_include = Path(_nvcc()).resolve().parent.parent / "include"
         includes = [*cpp_extension.include_paths(), str(cuda_include),
                     sysconfig.get_paths()["include"]]
         cmd = [os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
                "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+               f'-DB2S_TORCH_VERSION="{torch.__version__}"',
                *(f"-isystem{path}" for path in includes), str(src), "-o", str(HOST_LIB_PATH),
                f"-L{torch_lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-ltorch_cuda",
                "-lc10_cuda", "-lc10"]
@@ -120,6 +124,8 @@ def build_host(force: bool = False, verbose: bool = False) -> Path:
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError(f"g++ failed on {src.name}:\n{res.stdout}\n{res.stderr}")
+        BUILD_DIR.mkdir(parents=True, exist_ok=True)
+        stamp.write_text(torch.__version__)
     return HOST_LIB_PATH
 
 

@@ -437,5 +437,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_b2s_host", nullptr, -1, methods,
 }  // namespace
 
 extern "C" __attribute__((visibility("default"))) PyObject* PyInit__b2s_host(void) {
-  return PyModule_Create(&module);
+  PyObject* made = PyModule_Create(&module);
+  // the PyTorch whose structures this reads; nothing else may be called under another one
+  if (made && PyModule_AddStringConstant(made, "torch_version", B2S_TORCH_VERSION) != 0)
+    Py_CLEAR(made);
+  return made;
 }

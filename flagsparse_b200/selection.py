@@ -30,6 +30,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
+import warnings
 from types import SimpleNamespace
 
 import torch
@@ -84,6 +85,11 @@ def _bound_host():
     try:
         from . import _b2s_host
     except ImportError:
+        return _NO_HOST
+    if _b2s_host.torch_version != torch.__version__:     # it reads PyTorch's own structures
+        warnings.warn(f"flagsparse_b200/_b2s_host.so was built for PyTorch "
+                      f"{_b2s_host.torch_version}, this is {torch.__version__}: calls are made "
+                      "without it (run `python -m flagsparse_b200._build`)", stacklevel=4)
         return _NO_HOST
     address = [ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
         "b2s_select_rows", "b2s_select_grad_bytes", "b2s_select_grad", "b2s_route_plan_bytes",

@@ -3,6 +3,7 @@
 import shutil
 import subprocess
 import sys
+from types import SimpleNamespace
 
 import pytest
 import torch
@@ -139,3 +140,37 @@ def test_without_the_host_module_or_the_library(tmp_path, monkeypatch):
     monkeypatch.setattr(selection, "_host", selection._Host())
     monkeypatch.setattr(_lib, "LIB_PATH", tmp_path / "libb200sparse.so")
     assert selection._host.combine() is None and type(selection._host) is selection._Host
+
+
+def test_a_host_module_of_another_pytorch_is_not_used(monkeypatch):
+    """It reads PyTorch's structures by the headers it was built with."""
+    other = SimpleNamespace(torch_version="1.0", bind=lambda *a: pytest.fail("called"))
+    monkeypatch.setitem(sys.modules, "flagsparse_b200._b2s_host", other)
+    monkeypatch.setattr(fs, "_b2s_host", other, raising=False)
+    monkeypatch.setattr(selection, "_host", selection._Host())
+    with pytest.warns(UserWarning, match="built for PyTorch 1.0"):
+        assert selection._host.embedding(TOK, TABLE, 1.0, None) is None
+    assert selection._host is selection._NO_HOST
+
+
+def test_the_host_module_is_built_anew_for_another_pytorch(monkeypatch, tmp_path):
+    from flagsparse_b200 import _build
+    built = []
+
+    def run(cmd, **kwargs):
+        built.append(cmd)
+        return SimpleNamespace(returncode=0, stdout="", stderr="")
+
+    lib = tmp_path / "_b2s_host.so"
+    monkeypatch.setattr(_build, "HOST_LIB_PATH", lib)
+    monkeypatch.setattr(_build, "BUILD_DIR", tmp_path / "build")
+    monkeypatch.setattr(_build.subprocess, "run", run)
+    monkeypatch.setattr(_build, "_nvcc", lambda: "/usr/local/cuda/bin/nvcc")
+    _build.build_host()
+    assert len(built) == 1 and f'-DB2S_TORCH_VERSION="{torch.__version__}"' in built[0]
+    lib.touch()
+    _build.build_host()
+    assert len(built) == 1                                   # nothing has changed
+    monkeypatch.setattr(torch, "__version__", "99.0")
+    _build.build_host()
+    assert len(built) == 2 and '-DB2S_TORCH_VERSION="99.0"' in built[1]
