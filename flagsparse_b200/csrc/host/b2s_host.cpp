@@ -121,6 +121,15 @@ struct On {
   }
 };
 
+// The interpreter's lock is given up while a call allocates and launches: both may wait (for memory
+// that another stream frees, for room in the queue of launches), and other threads run meanwhile.
+struct Unlocked {
+  PyThreadState* state = PyEval_SaveThread();
+  Unlocked() = default;
+  Unlocked(const Unlocked&) = delete;
+  ~Unlocked() { PyEval_RestoreThread(state); }
+};
+
 // a new tensor beside `like`
 at::Tensor fresh(c10::IntArrayRef shape, at::ScalarType type, const at::Tensor& like) {
   return at::detail::empty_cuda(shape, type, like.device(), std::nullopt);
@@ -158,11 +167,16 @@ PyObject* embedding(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const int64_t dim = table->size(1);
     c10::DimVector shape(tokens->sizes().begin(), tokens->sizes().end());
     shape.push_back(dim);
-    at::Tensor out = fresh(shape, table->scalar_type(), *table);
-    if (p_select_rows(vcode, icode, tokens->const_data_ptr(), tokens->numel(), has, ignore,
-                      table->const_data_ptr(), table->size(0), pitch, dim, out.data_ptr(), dim,
-                      alpha, 0.0, status, on.stream) != B2S_OK)
-      NOT_HERE;
+    at::Tensor out;
+    int st;
+    {
+      const Unlocked unlocked;
+      out = fresh(shape, table->scalar_type(), *table);
+      st = p_select_rows(vcode, icode, tokens->const_data_ptr(), tokens->numel(), has, ignore,
+                         table->const_data_ptr(), table->size(0), pitch, dim, out.data_ptr(), dim,
+                         alpha, 0.0, status, on.stream);
+    }
+    if (st != B2S_OK) NOT_HERE;
     return THPVariable_Wrap(std::move(out));
   })
 }
@@ -215,16 +229,22 @@ PyObject* embedding_grad(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
       }
     } else {
       if (beta != 0) NOT_HERE;
-      made = fresh({n_rows, dim}, out_type, *grad);
-      out = &made;
       out_pitch = dim;
     }
-    const int64_t bytes = p_select_grad_bytes(vcode, n, n_rows, dim);
-    at::Tensor ws = fresh({bytes}, at::kByte, *grad);
-    if (p_select_grad(vcode, value_code(*out), icode, tokens->const_data_ptr(), n, has, ignore,
-                      grad->const_data_ptr(), pitch, n_rows, dim, out->data_ptr(), out_pitch,
-                      alpha, beta, ws.data_ptr(), bytes, status, on.stream) != B2S_OK)
-      NOT_HERE;
+    int st;
+    {
+      const Unlocked unlocked;
+      if (!out) {
+        made = fresh({n_rows, dim}, out_type, *grad);
+        out = &made;
+      }
+      const int64_t bytes = p_select_grad_bytes(vcode, n, n_rows, dim);
+      at::Tensor ws = fresh({bytes}, at::kByte, *grad);
+      st = p_select_grad(vcode, value_code(*out), icode, tokens->const_data_ptr(), n, has, ignore,
+                         grad->const_data_ptr(), pitch, n_rows, dim, out->data_ptr(), out_pitch,
+                         alpha, beta, ws.data_ptr(), bytes, status, on.stream);
+    }
+    if (st != B2S_OK) NOT_HERE;
     if (a[5] == Py_None) return THPVariable_Wrap(std::move(made));
     if (!out->is_inference()) out->unsafeGetTensorImpl()->bump_version();
     Py_INCREF(a[5]);
@@ -267,14 +287,19 @@ PyObject* route_plan(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const int64_t n_tokens = experts->size(0), k = experts->size(1), n = n_tokens * k;
     if (n > 0x7fffffff) NOT_HERE;
     const On on(static_cast<c10::DeviceIndex>(dev));
-    const int64_t bytes = p_route_plan_bytes(n_tokens, k, n_experts);
-    const int64_t scratch = (2 * n + n_experts + 1 + 63) / 64 * 64;
-    at::Tensor buffer = fresh({scratch + bytes / 4}, at::kInt, *experts);
-    int32_t* arrays = buffer.data_ptr<int32_t>();
-    if (p_route_plan(icode, experts->const_data_ptr(), n_tokens, k, n_experts, arrays, arrays + n,
-                     arrays + n + n_experts + 1, arrays + scratch, bytes, status,
-                     on.stream) != B2S_OK)
-      NOT_HERE;
+    at::Tensor buffer;
+    int st;
+    {
+      const Unlocked unlocked;
+      const int64_t bytes = p_route_plan_bytes(n_tokens, k, n_experts);
+      const int64_t scratch = (2 * n + n_experts + 1 + 63) / 64 * 64;
+      buffer = fresh({scratch + bytes / 4}, at::kInt, *experts);
+      int32_t* arrays = buffer.data_ptr<int32_t>();
+      st = p_route_plan(icode, experts->const_data_ptr(), n_tokens, k, n_experts, arrays,
+                        arrays + n, arrays + n + n_experts + 1, arrays + scratch, bytes, status,
+                        on.stream);
+    }
+    if (st != B2S_OK) NOT_HERE;
     PyObject* stream = PyLong_FromLongLong(reinterpret_cast<intptr_t>(on.stream));
     PyObject* wrapped = THPVariable_Wrap(std::move(buffer));
     PyObject* pair = stream && wrapped ? PyTuple_Pack(2, wrapped, stream) : nullptr;
@@ -299,10 +324,15 @@ PyObject* dispatch(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
     const On on(static_cast<c10::DeviceIndex>(r.dev));
     if (vcode < 0 || on.stream != made_on) NOT_HERE;
     const int64_t dim = x->size(1);
-    at::Tensor out = fresh({r.n_rows, dim}, x->scalar_type(), *x);
-    if (p_route_dispatch(vcode, x->const_data_ptr(), pitch, r.n_tokens, r.k, dim, r.slots, r.held,
-                         out.data_ptr(), dim, on.stream) != B2S_OK)
-      NOT_HERE;
+    at::Tensor out;
+    int st;
+    {
+      const Unlocked unlocked;
+      out = fresh({r.n_rows, dim}, x->scalar_type(), *x);
+      st = p_route_dispatch(vcode, x->const_data_ptr(), pitch, r.n_tokens, r.k, dim, r.slots,
+                            r.held, out.data_ptr(), dim, on.stream);
+    }
+    if (st != B2S_OK) NOT_HERE;
     return THPVariable_Wrap(std::move(out));
   })
 }
@@ -341,11 +371,16 @@ PyObject* combine(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         !weights_of(a[kRouteArgs + 1], r, vcode, &w, &wcode) || (w && recorded(*w)))
       NOT_HERE;
     const int64_t dim = y->size(1);
-    at::Tensor out = fresh({r.n_tokens, dim}, y->scalar_type(), *y);
-    if (p_route_combine(vcode, y->const_data_ptr(), pitch, r.slots, wcode,
-                        w ? w->const_data_ptr() : nullptr, r.n_tokens, r.k, dim, out.data_ptr(),
-                        dim, alpha, 0.0, on.stream) != B2S_OK)
-      NOT_HERE;
+    at::Tensor out;
+    int st;
+    {
+      const Unlocked unlocked;
+      out = fresh({r.n_tokens, dim}, y->scalar_type(), *y);
+      st = p_route_combine(vcode, y->const_data_ptr(), pitch, r.slots, wcode,
+                           w ? w->const_data_ptr() : nullptr, r.n_tokens, r.k, dim,
+                           out.data_ptr(), dim, alpha, 0.0, on.stream);
+    }
+    if (st != B2S_OK) NOT_HERE;
     return THPVariable_Wrap(std::move(out));
   })
 }
@@ -373,13 +408,17 @@ PyObject* combine_grad(PyObject*, PyObject* const* a, Py_ssize_t n_args) {
         !weights_of(a[kRouteArgs + 2], r, vcode, &w, &wcode))
       NOT_HERE;
     const int64_t dim = g->size(1);
-    at::Tensor grad_y = fresh({r.n_rows, dim}, g->scalar_type(), *g);
-    at::Tensor grad_w = fresh({r.n_tokens, r.k}, w->scalar_type(), *w);
-    if (p_route_combine_grad(vcode, g->const_data_ptr(), pitch, y->const_data_ptr(), y_pitch,
-                             r.slots, r.held, wcode, w->const_data_ptr(), r.n_tokens, r.k, dim,
-                             alpha, grad_y.data_ptr(), dim, grad_w.data_ptr(),
-                             on.stream) != B2S_OK)
-      NOT_HERE;
+    at::Tensor grad_y, grad_w;
+    int st;
+    {
+      const Unlocked unlocked;
+      grad_y = fresh({r.n_rows, dim}, g->scalar_type(), *g);
+      grad_w = fresh({r.n_tokens, r.k}, w->scalar_type(), *w);
+      st = p_route_combine_grad(vcode, g->const_data_ptr(), pitch, y->const_data_ptr(), y_pitch,
+                                r.slots, r.held, wcode, w->const_data_ptr(), r.n_tokens, r.k, dim,
+                                alpha, grad_y.data_ptr(), dim, grad_w.data_ptr(), on.stream);
+    }
+    if (st != B2S_OK) NOT_HERE;
     PyObject* first = THPVariable_Wrap(std::move(grad_y));
     PyObject* second = THPVariable_Wrap(std::move(grad_w));
     PyObject* pair = first && second ? PyTuple_Pack(2, first, second) : nullptr;

@@ -154,3 +154,51 @@ def test_out_may_not_be_what_is_read_under_another_name():
     fs.flagsparse_embedding_grad(tokens, both[:20], 20, out=other(both[20:]))
     fs.flagsparse_embedding_grad(tokens, table, 20, out=into)
     assert torch.equal(both[20:], table) and torch.equal(into, table)
+
+
+def test_other_threads_run_while_a_launch_waits():
+    """A launch that finds the queue of launches full waits for the GPU, not with the interpreter's
+    lock.  The GPU sleeps for some 0.7 seconds here, behind it there are more calls than the queue
+    takes; a thread that looks at the clock every millisecond may not miss half of the sleep."""
+    import threading
+    import time
+    n, k = 8, 2
+    table, tokens, y = randn(16, 8), torch.arange(n, device="cuda"), randn(n * k, 8)
+    experts, w = torch.zeros(n, k, dtype=torch.int64, device="cuda"), randn(n, k)
+    r = fs.prepare_token_route(experts, 2)
+    calls = [lambda: fs.flagsparse_embedding(tokens, table),
+             lambda: fs.flagsparse_embedding_grad(tokens, table[:n], 16),
+             lambda: fs.prepare_token_route(experts, 2),
+             lambda: fs.flagsparse_token_dispatch(table[:n], r),
+             lambda: fs.flagsparse_token_combine(y, r, w),
+             lambda: fs.flagsparse_token_combine_grad(table[:n], y, r, w)]
+    for call in calls:
+        call()
+    torch.cuda.synchronize()
+    start = time.perf_counter()
+    torch.cuda._sleep(100_000_000)
+    torch.cuda.synchronize()
+    cycles = int(0.7 / (time.perf_counter() - start) * 100_000_000)
+
+    def watch(stop, gaps):
+        last = time.perf_counter()
+        while not stop.is_set():
+            time.sleep(0.001)
+            now = time.perf_counter()
+            gaps.append(now - last)
+            last = now
+
+    for call in calls:
+        stop, gaps = threading.Event(), []
+        watcher = threading.Thread(target=watch, args=(stop, gaps))
+        watcher.start()
+        start = time.perf_counter()
+        torch.cuda._sleep(cycles)
+        for _ in range(4000):
+            call()
+        issued = time.perf_counter() - start
+        torch.cuda.synchronize()
+        stop.set()
+        watcher.join()
+        assert issued > 0.4, "the queue took every launch: more calls are needed"
+        assert max(gaps) < 0.35
