@@ -213,8 +213,16 @@ def _wants_grad(t, other=None):
             and torch.is_grad_enabled())
 
 
-def _refuse_capture():
-    if torch.cuda.is_current_stream_capturing():
+def _capturing(index):
+    """Whether the current stream of device `index` is captured into a graph."""
+    if torch.cuda.current_device() == index:
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(index):
+        return torch.cuda.is_current_stream_capturing()
+
+
+def _refuse_capture(index):
+    if _capturing(index):
         raise RuntimeError(
             "differentiable calls are not recorded inside a CUDA graph capture: call them under "
             "torch.no_grad() and take the gradients with the *_grad functions")
@@ -349,7 +357,7 @@ def flagsparse_embedding(tokens, table, alpha=1.0, ignore_index=None, out=None, 
     _check_same_device(tokens, "tokens", index, "table")
     _check_same_device(out, "out", index, "table")
     if _wants_grad(table):
-        _refuse_capture()
+        _refuse_capture(index)
         if beta != 0:
             raise ValueError("beta != 0 requires out= holding the rows to scale")
         return _Embedding.apply(tokens, table, alpha, ignore_index)
@@ -446,7 +454,7 @@ class _Embedding(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        _refuse_capture()
+        _refuse_capture(grad.get_device())
         n_rows, alpha, ignore = ctx.args
         grad_table = flagsparse_embedding_grad(ctx.saved_tensors[0], grad, n_rows, alpha=alpha,
                                                ignore_index=ignore)
@@ -518,7 +526,7 @@ class TokenRoute:
         """Called before a launch: keeps the arrays from being reused while a stream other than
         the one they were made on still reads them."""
         if _raw_stream(self._index) != self._stream:
-            if not torch.cuda.is_current_stream_capturing():
+            if not _capturing(self._index):
                 self._buffer.record_stream(torch.cuda.current_stream(self._index))
 
     def __repr__(self):
@@ -603,7 +611,7 @@ def flagsparse_token_dispatch(x, route, out=None):
     _check_same_device(x, "x", index, "route")
     _check_same_device(out, "out", index, "route")
     if _wants_grad(x):
-        _refuse_capture()
+        _refuse_capture(index)
         return _Dispatch.apply(x, route)
     return _dispatch(x, route, out)
 
@@ -667,7 +675,7 @@ def flagsparse_token_combine(y, route, weights=None, alpha=1.0, out=None, beta=0
     _check_same_device(weights, "weights", index, "route")
     _check_same_device(out, "out", index, "route")
     if _wants_grad(y, weights):
-        _refuse_capture()
+        _refuse_capture(index)
         if beta != 0:
             raise ValueError("beta != 0 requires out= holding the rows to scale")
         return _Combine.apply(y, weights, route, alpha)
@@ -753,7 +761,7 @@ class _Dispatch(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        _refuse_capture()
+        _refuse_capture(grad.get_device())
         return flagsparse_token_dispatch_grad(grad, ctx.route), None
 
 
@@ -770,7 +778,7 @@ class _Combine(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        _refuse_capture()
+        _refuse_capture(grad.get_device())
         y, weights = ctx.saved_tensors
         if ctx.wants_weights:
             grad_y, grad_w = flagsparse_token_combine_grad(grad, y, ctx.route, weights, ctx.alpha)

@@ -1,5 +1,6 @@
 """Selection products on the CPU: calls beside the usual one, up to where the device begins."""
 
+import contextlib
 import shutil
 import subprocess
 import sys
@@ -174,3 +175,50 @@ def test_the_host_module_is_built_anew_for_another_pytorch(monkeypatch, tmp_path
     monkeypatch.setattr(torch, "__version__", "99.0")
     _build.build_host()
     assert len(built) == 2 and '-DB2S_TORCH_VERSION="99.0"' in built[1]
+
+
+class _FakeCuda:
+    """Two devices; the current stream of the second is captured."""
+
+    def __init__(self, monkeypatch):
+        self.index = 0
+        for name in ("current_device", "is_current_stream_capturing", "device"):
+            monkeypatch.setattr(torch.cuda, name, getattr(self, name))
+
+    def current_device(self):
+        return self.index
+
+    def is_current_stream_capturing(self):
+        return self.index == 1
+
+    @contextlib.contextmanager
+    def device(self, index):
+        before, self.index = self.index, index
+        yield
+        self.index = before
+
+
+def test_the_stream_of_the_tensors_decides_whether_it_is_a_capture(monkeypatch):
+    """Recorded calls are refused where their own device's stream is captured, whichever device is
+    current; and a route's memory is not marked as used by a stream that is."""
+    cuda = _FakeCuda(monkeypatch)
+    monkeypatch.setattr(selection, "_check_first_device", lambda t, name: 1)
+    monkeypatch.setattr(selection, "_check_same_device", lambda *args: None)
+    x, y = torch.zeros(3, 4).requires_grad_(), torch.zeros(6, 4).requires_grad_()
+    for current in (0, 1):
+        cuda.index = current
+        for call in (lambda: fs.flagsparse_embedding(TOK, x), lambda: fs.flagsparse_token_dispatch(
+                x, _route()), lambda: fs.flagsparse_token_combine(y, _route())):
+            with pytest.raises(RuntimeError, match="not recorded inside a CUDA graph capture"):
+                call()
+        assert cuda.index == current
+    cuda.index = 1                                           # (the other device is free to record)
+    assert not selection._capturing(0) and selection._capturing(1)
+    marked = []
+    monkeypatch.setattr(selection, "_raw_stream", lambda index: 5)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda index: "stream")
+    for index, times in ((1, 0), (0, 1)):
+        for cuda.index in (0, 1):
+            fake = SimpleNamespace(get_device=lambda: index, record_stream=marked.append)
+            fs.TokenRoute(fake, 3, 2, 4, 0)._use()
+        assert len(marked) == 2 * times
