@@ -202,3 +202,142 @@ def test_other_threads_run_while_a_launch_waits():
         watcher.join()
         assert issued > 0.4, "the queue took every launch: more calls are needed"
         assert max(gaps) < 0.35
+
+
+@pytest.mark.parametrize("pattern", PATTERNS)
+@pytest.mark.parametrize("dtype, out_dtype, dim", [
+    (torch.float32, torch.float32, 264), (torch.bfloat16, torch.bfloat16, 264),
+    (torch.float16, torch.float16, 392), (torch.bfloat16, torch.float32, 264),
+    (torch.bfloat16, torch.float32, 4104), (torch.float16, torch.float32, 392),
+    (torch.float64, torch.float64, 130)], ids=ids)
+def test_embedding_grad_into_rows_taken_16_bytes_at_a_time(pattern, dtype, out_dtype, dim):
+    """Added to (rows that no token names stay as they are), scaled, written over: into an out whose
+    rows the kernels take 16 bytes at a time, with and without a pitch of its own."""
+    tokens, vocab = PATTERNS[pattern]
+    n = tokens.numel()
+    if n * dim > 1 << 24 or vocab * dim > 1 << 24:
+        dim = 392 if dim > 392 else 40
+    g, tok = randn(n, dim, dtype=dtype, seed=n), tokens.cuda()
+    named = torch.bincount(tokens, minlength=vocab) > 0
+    for pad, alpha, beta in ((0, 1.5, 1.0), (8, 1.0, 1.0), (8, 0.75, 0.5), (0, 1.0, -2.0),
+                             (8, 1.0, 0.0)):
+        out = randn(vocab, dim, dtype=out_dtype, seed=2, pad=pad)
+        if beta == 0.0:
+            out.fill_(float("nan"))
+        elif beta == 1.0:
+            out[~named.cuda()] = float("nan")
+        before, again = cpu(out), out.clone()
+        assert fs.flagsparse_embedding_grad(tok, g, vocab, alpha=alpha, beta=beta, out=out) is out
+        fs.flagsparse_embedding_grad(tok.int(), g, vocab, alpha=alpha, beta=beta, out=again)
+        assert torch.equal(again[named.cuda()], out[named.cuda()])       # one order of the sums
+        total, terms, m = plain_grad(tokens, g, vocab, alpha, before, beta)
+        if beta == 1.0:
+            assert torch.isnan(out[~named.cuda()]).all()
+            total, terms, m, out = total[named], terms[named], m[named], out[named.cuda()]
+        assert_close(out, total, terms, m, acc=dtype)
+    fs.check_selection_ids()
+
+
+def test_embedding_grad_random_calls():
+    """Sizes, types, layouts, masks, scalars and places of the result at random."""
+    import random
+    for seed in range(120):
+        rng = random.Random(1000 + seed)
+        torch.manual_seed(seed)
+        dtype, index = rng.choice(TYPES), rng.choice([torch.int32, torch.int64])
+        out_dtype = rng.choice([dtype, torch.float32]) if dtype.itemsize == 2 else dtype
+        dim = rng.choice([1, 2, 8, 33, 64, 256, 257, 512, 520, 1032])
+        n, vocab = int(2**rng.uniform(0, 14)), int(2**rng.uniform(0, 12))
+        tokens = (torch.rand(n, device="cuda")**rng.choice([1, 4, 20]) * vocab).to(index)
+        ignore = rng.choice([None, rng.randrange(vocab)])
+        alpha, beta = rng.choice([1.0, -0.5]), rng.choice([0.0, 1.0, 0.25])
+
+        def matrix(rows, kind):
+            pad, off = rng.choice([0, 0, 8, 3]), rng.choice([0, 0, 8, 1])
+            return torch.randn(rows, off + dim + pad, device="cuda").to(kind)[:, off:off + dim]
+
+        g, out = matrix(n, dtype), matrix(vocab, out_dtype)
+        before = cpu(out)
+        fs.flagsparse_embedding_grad(tokens, g, vocab, alpha=alpha, ignore_index=ignore, out=out,
+                                     beta=beta)
+        total, terms, m = plain_grad(tokens, g, vocab, alpha, before, beta, ignore)
+        assert_close(out, total, terms, m, acc=dtype)
+    fs.check_selection_ids()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=ids)
+@pytest.mark.parametrize("n, k, dim", [(9000, 3, 264), (20000, 2, 72), (11000, 1, 40),
+                                       (5000, 9, 8), (400, 70, 520)])
+def test_combine_of_several_tokens_a_warp(dtype, n, k, dim):
+    """More tokens than warps fit the GPU: a warp's queue goes on from token to token, with rows
+    that differ and tokens whose assignments are masked in part or all."""
+    experts = random_experts(n, k, 11, 0.2, seed=n)
+    experts[::17] = -1
+    r = fs.prepare_token_route(experts, 11)
+    slots, indptr, _ = plain_route(experts, 11)
+    live = slots >= 0
+    y, w = randn(n * k, dim, dtype=dtype, seed=1), randn(n, k, seed=2)
+    y[int(indptr[-1]):] = float("nan")
+    w[experts < 0] = float("nan")
+    picked = torch.where(live[..., None], cpu(y)[torch.where(live, slots, 0)], 0.0)
+    parts = torch.where(live, cpu(w), 0.0)[..., None] * picked
+    assert_close(fs.flagsparse_token_combine(y, r, w), parts.sum(1), parts.abs().sum(1), 2 * k)
+    out = randn(n, dim, dtype=dtype, seed=3)
+    before = cpu(out)
+    fs.flagsparse_token_combine(y, r, w, alpha=-0.5, beta=2.0, out=out)
+    assert_close(out, -0.5 * parts.sum(1) + 2.0 * before,
+                 0.5 * parts.abs().sum(1) + 2.0 * before.abs(), 2 * k)
+    assert_close(fs.flagsparse_token_dispatch_grad(y, r), picked.sum(1), picked.abs().sum(1), k)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32, torch.float64], ids=ids)
+def test_embedding_grad_and_the_transposed_product(dtype):
+    """The SpMM of this package with S written out: both within their bound of the 64-bit sum, so
+    within two of them of each other (the SpMM has the same: products and additions in any order in
+    float32 or float64, one rounding)."""
+    n, vocab, dim = 300, 90, 64
+    g = randn(n, dim, dtype=dtype, seed=1)
+    tokens = torch.randint(0, vocab, (n,), device="cuda")
+    ones, ptr = torch.ones(n, dtype=dtype, device="cuda"), torch.arange(n + 1, device="cuda")
+    dense = fs.flagsparse_spmm_csr(ones, tokens, ptr, g, (n, vocab), op="trans")
+    total, terms, m = plain_grad(tokens, g, vocab)
+    for got in (dense, fs.flagsparse_embedding_grad(tokens, g, vocab)):
+        assert_close(got, total, terms, m)
+
+
+def test_two_threads_each_finish_their_calls():
+    """Gradients, routes and the way there and back from two threads, each on a stream of its own
+    or both on one; what goes wrong in a thread fails the test."""
+    import threading
+    n, vocab, dim, k = 9000, 4000, 128, 2
+    g = randn(n, dim)
+    tokens = [torch.randint(0, vocab, (n,), device="cuda") for _ in range(2)]
+    experts = [random_experts(n, k, 16, 0.1, seed=i) for i in range(2)]
+
+    def calls(i):
+        r = fs.prepare_token_route(experts[i], 16)
+        rows = fs.flagsparse_token_dispatch(g, r)
+        return (fs.flagsparse_embedding_grad(tokens[i], g, vocab), r.slots, rows,
+                fs.flagsparse_token_combine(rows, r), fs.flagsparse_embedding(tokens[i], g[:vocab]))
+
+    want = [calls(i) for i in range(2)]
+    torch.cuda.synchronize()
+    for shared in (None, torch.cuda.Stream()):
+        done, wrong = [0, 0], []
+
+        def work(i):
+            try:
+                with torch.cuda.stream(shared or torch.cuda.Stream()):
+                    for _ in range(20):
+                        for a, b in zip(calls(i), want[i]):
+                            assert torch.equal(a, b)
+                        done[i] += 1
+            except BaseException as error:  # noqa: BLE001
+                wrong.append(error)
+
+        threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        assert not wrong and done == [20, 20]
