@@ -554,11 +554,15 @@ __device__ inline void grad_sum_plain(const GradRuns& runs, const GradRange& g,
   }
 }
 
-// CTAs that share an SM: as many as their queues allow.
+// CTAs that share an SM: as many as its 228 KB allow (a CTA takes 1 KB beside its queues), up to
+// four; two where the rows are in registers.
+constexpr int kSmemOfSm = 228 << 10;
 template <class T, class O, int VE, bool kBeta>
-constexpr int kGradCtas = !kQueued<T, VE> || (VE == 1 && sizeof(T) == 8) ? 2
-                          : !kBeta || sizeof(O) > sizeof(T)               ? kQueueCtas
-                                                                          : 3;
+constexpr int kGradCtas =
+    !kQueued<T, VE>
+        ? 2
+        : std::min(kQueueCtas,
+                   kSmemOfSm / (kSelWarps * kGradWarpBytes<T, O, VE, kBeta> + (1 << 10)));
 
 // CTAs that sum and CTAs that write the rows no token names (zero, or beta times what is there;
 // none when beta = 1 leaves them as they are) alternate from the first on, until one kind is used
@@ -1043,10 +1047,12 @@ int select_grad_go(const GradRuns& runs, const T* grad, int64_t ld_grad,
   using A = typename acc_of<T>::type;
   constexpr int E = kGradCols<T, O, VE, kBeta>;
   constexpr size_t smem = kQueued<T, VE> ? kSelWarps * kGradWarpBytes<T, O, VE, kBeta> : 0;
+  constexpr int kCtas = kGradCtas<T, O, VE, kBeta>;
+  static_assert(kCtas >= 1 && kCtas * (smem + (1 << 10)) <= kSmemOfSm);
   const int64_t slabs = ceil_div(to.dim, 32 * E);
   const int64_t ranges =
       runs.n == 0 ? 0
-                  : std::min(grad_ranges(runs.n, slabs, kGradCtas<T, O, VE, kBeta>), most_ranges);
+                  : std::min(grad_ranges(runs.n, slabs, kCtas), most_ranges);
   const int64_t sums = ceil_div(ranges * slabs, kSelWarps);
   const int64_t rest = to.beta == A(1) ? 0 : ceil_div(static_cast<int64_t>(runs.n_keys),
                                                         kRestRows<T, VE> * kSelWarps);
