@@ -1233,8 +1233,8 @@ int route_combine_go(const T* y, int64_t ld_y, const int32_t* slots, const void*
   constexpr int64_t kResident = 148 * kCombineCtas<T, VE> * kSelWarps;
   int64_t ranges = std::max<int64_t>(kResident / slabs, n * k / 16);
   ranges = ranges < 1 ? 1 : ranges > n ? n : ranges;
-  // a warp counts its assignments in 32 bits (with two stretches to spare)
-  while (ceil_div(n, ranges) * k > 0x7fff0000) ++ranges;
+  // (a warp counts its assignments in 32 bits, a stretch or two behind the last: check_route has
+  // held n * k to kSortMaxEntries, 2^25 below 2^31)
   const int64_t blocks = ceil_div(ranges * slabs, kSelWarps);
   if (blocks > kMaxGrid / kSelWarps) return B2S_ERR_RANGE;  // (warps are counted in 32 bits)
   const A b = static_cast<A>(beta);
