@@ -289,8 +289,8 @@ select_rows_kernel(IdKeys<I> ids, int64_t n, const T* table, int64_t ld_table,
 
 // ---- embedding gradient ----------------------------------------------------------------------
 // The sorted (token, position) list is cut into ranges of some 24 entries (grad_ranges); a warp
-// sums the rows of a range over one slab of columns and writes each token's row when its run of equal
-// tokens ends.  A run that crosses a border and ends within 31 entries behind it is read to its
+// sums the rows of a range over one slab of columns and writes each token's row when its run of
+// equal tokens ends.  A run that crosses a border and ends within 31 entries behind it is read to its
 // end by the warp in front of the border.  A longer one is cut there: each range writes its piece
 // as a partial row, and select_grad_long_kernel adds the pieces in order.  No floating-point
 // atomics: the sums have one order whatever the scheduling.  Sums and pieces are float32 (float64)
@@ -738,9 +738,9 @@ __device__ inline typename acc_of<T>::type route_weight(const void* w, bool w_is
 // and one slab of columns; the assignments of its tokens are one stretch of `slots`, read 32 at a
 // time and a stretch ahead, and their rows stream through the warp's queue without a pause
 // between tokens.  A masked assignment is a part of zeros with weight zero; a token that has no
-// other is beta * out whatever alpha is (alpha * 0 is not zero where alpha is not finite).  (8192 x 8 rows of 4096
-// bf16: 101 us, 6.0 TB/s; 16384 x 4 rows of 2048: 55 us, 6.1 TB/s.  With 16 bytes a lane and a wait
-// for every row, 134 us: 82 % of the issue slots were taken.)
+// other is beta * out whatever alpha is (alpha * 0 is not zero where alpha is not finite).
+// (8192 x 8 rows of 4096 bf16: 101 us, 6.0 TB/s; 16384 x 4 rows of 2048: 55 us, 6.1 TB/s.  With 16
+// bytes a lane and a wait for every row, 134 us: 82 % of the issue slots were taken.)
 template <class T, int VE>
 constexpr int kCombineCtas = VE == 1 && sizeof(T) == 8 ? 2 : kQueueCtas;
 template <class T, int VE>
@@ -1308,7 +1308,8 @@ extern "C" int b2s_route_dispatch(int val_type, const void* x_dev, int64_t ld_x,
   auto go = [&](auto kernel) {
     return launch_behind(kernel, dim3(static_cast<unsigned>(blocks)), kSelThreads, 0,
                          static_cast<cudaStream_t>(stream),
-                         static_cast<const unsigned char*>(x_dev), ld_x * static_cast<int64_t>(es), n_tokens, k, units, slots_dev, held_dev,
+                         static_cast<const unsigned char*>(x_dev),
+                         ld_x * static_cast<int64_t>(es), n_tokens, k, units, slots_dev, held_dev,
                          static_cast<unsigned char*>(rows_dev), ld_rows * static_cast<int64_t>(es),
                          slabs);
   };

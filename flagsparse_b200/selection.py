@@ -49,9 +49,9 @@ MAX_DIM = 1 << 22
 
 
 class _Host:
-    """The usual call (plain strided tensors, a new result, nothing to record) is made by a C++ module
-    (csrc/host/b2s_host.cpp): it returns None for every other one, which then takes the way below.
-    Without the module all calls do; the kernels are the same.
+    """The usual call (plain strided tensors, a new result, nothing to record) is made by a C++
+    module (csrc/host/b2s_host.cpp): it returns None for every other one, which then takes the way
+    below.  Without the module all calls do; the kernels are the same.
 
     The module and the library are loaded by the first call and not when the package is imported:
     a library that lacks an entry point can be built anew by the package that it belongs to.  Then
@@ -177,7 +177,8 @@ def _check_values(t, name):
 def _refuse_tangent(t, name):
     # (such a tensor does not require a gradient: without this its tangent would be lost)
     if unpack_dual(t).tangent is not None:
-        raise NotImplementedError(f"{name} has a tangent: forward-mode derivatives are not supported")
+        raise NotImplementedError(
+            f"{name} has a tangent: forward-mode derivatives are not supported")
 
 
 def _check_first_device(t, name):
@@ -632,7 +633,8 @@ def flagsparse_token_dispatch_grad(grad, route, out=None, beta=0.0):
     """The gradient of flagsparse_token_dispatch: row t is the sum of grad[route.slots[t, j]] over
     the j that are not masked (float32 / float64 sums, one rounding), plus beta * out.
 
-    grad: (n_tokens * k, dim); its rows from route.indptr[-1] on are not read.
+    grad: (n_tokens * k, dim); its rows from route.indptr[-1] on are not read.  The call itself is
+    not differentiable.
     """
     _check_route(route)
     if _host is not None and out is None and type(beta) in (float, int) and beta == 0:
@@ -656,7 +658,7 @@ def flagsparse_token_combine(y, route, weights=None, alpha=1.0, out=None, beta=0
 
     y: (n_tokens * k, dim); weights: (n_tokens, k) of y's dtype or float32, None for ones.  The
     result is (n_tokens, dim) of y's dtype: float32 (float64) sums, one rounding; a token whose
-    assignments are all masked gets beta * out.  Differentiable in y and weights.
+    assignments are all masked gets beta * out, whatever alpha is.  Differentiable in y and weights.
     """
     _check_route(route)
     if _host is not None and out is None and type(beta) in (float, int) and beta == 0:
@@ -705,6 +707,7 @@ def flagsparse_token_combine_grad(grad, y, route, weights=None, alpha=1.0):
     grad: (n_tokens, dim).  grad_y[route.slots[t, j]] = alpha * weights[t, j] * grad[t] (rows that
     belong to nobody are zero); grad_weights[t, j] = alpha * <grad[t], y[route.slots[t, j]]> in the
     dtype of weights, zero where masked.  Without weights, y may be None and grad_weights is None.
+    The call itself is not differentiable.
     """
     _check_route(route)
     if _host is not None and weights is not None:

@@ -391,7 +391,8 @@ int b2s_csr2csc(int val_type, int idx_type, int ptr_type,
  *
  * b2s_select_grad: out[v] = alpha * (sum of grad[i] over the i with idx[i] == v) + beta * out[v]
  * for every v < n_rows; the sum runs over ascending i, that of a frequent v in pieces which are
- * then added in order.  out_type is val_type, or B2S_F32 for the 16-bit types.  beta = 1 touches the rows that idx names only.
+ * then added in order.  out_type is val_type, or B2S_F32 for the 16-bit types.  beta = 1 touches the
+ * rows that idx names only.
  * ws: b2s_select_grad_bytes() bytes, 256-byte aligned. */
 int b2s_select_rows(int val_type, int idx_type, const void* idx_dev, int64_t n, int has_ignore,
                     int64_t ignore, const void* table_dev, int64_t n_rows, int64_t ld_table,
@@ -409,12 +410,14 @@ int b2s_select_grad(int val_type, int out_type, int idx_type, const void* idx_de
  *   slots[a]     place of a among the sorted rows, -1 for a masked one
  *   indptr[e]    first place of expert e; indptr[n_experts] = number of places held
  *   indices[p]   token of place p; (indptr, indices) is the experts x tokens matrix in CSR form
- * All int32; n_experts <= 2047.  The arrays may lie one behind the other.  ws: b2s_route_plan_bytes() bytes, 256-byte aligned.
+ * All int32; n_experts <= 2047.  The arrays may lie one behind the other.
+ * ws: b2s_route_plan_bytes() bytes, 256-byte aligned.
  *
  * b2s_route_dispatch: rows[slots[a]] = x[a / k]; the rows from *held_dev (= indptr[n_experts]) to
  * n_tokens * k are zeroed.
  * b2s_route_combine: out[t] = alpha * sum_j w[t, j] * y[slots[t, j]] + beta * out[t], without the
- * masked j.  weights NULL: all one (with beta = 0 that is the gradient of the dispatch).
+ * masked j (beta * out[t], whatever alpha is, where all are).  weights NULL: all one (with beta = 0
+ * that is the gradient of the dispatch).
  * w_type: val_type or B2S_F32.
  * b2s_route_combine_grad: grad_y[slots[a]] = alpha * w[a] * g[a / k], the rows behind the held
  * ones zeroed; grad_w[a] (w_type; may be NULL, y is then not read) = alpha * <g[a / k],

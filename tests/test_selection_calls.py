@@ -45,9 +45,10 @@ def test_tangents_are_refused():
 
 def test_views_that_stand_for_the_negative_are_written_out():
     z = torch.complex(torch.arange(6.0).reshape(6, 1), torch.arange(6.0).reshape(6, 1) + 1)
-    view = z.conj().imag                                     # rows that a kernel could read as they lie
+    view = z.conj().imag                                 # rows that a kernel could read as they lie
     assert view.is_neg() and selection._row_major_ok(view)
-    for rows in (selection._rows(view), selection._as_stored(torch._neg_view((-view).resolve_neg()))):
+    same = torch._neg_view((-view).resolve_neg())
+    for rows in (selection._rows(view), selection._as_stored(same)):
         assert not rows.is_neg() and torch.equal(rows, view)
     assert selection._rows(TABLE) is TABLE
     flat, address, _ = selection._result(view, (6, 1), view, torch.float32, 1.0)
@@ -57,8 +58,12 @@ def test_views_that_stand_for_the_negative_are_written_out():
 
 
 def test_overlap_is_a_matter_of_addresses():
-    refuse = lambda out, *t: pytest.raises(ValueError, selection._refuse_overlap, out, *t)  # noqa: E731
     wide = torch.zeros(6, 10)
+
+    def refuse(*tensors):
+        with pytest.raises(ValueError, match="must not overlap"):
+            selection._refuse_overlap(*tensors)
+
     alias = torch.from_dlpack(wide[1:])                      # the same memory, another storage
     assert alias.untyped_storage().data_ptr() != wide.untyped_storage().data_ptr()
     refuse(wide, alias)
